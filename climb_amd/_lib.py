@@ -45,7 +45,7 @@ def torch_h16():
     return torch.float16 if h16() == "fp16" else torch.bfloat16
 
 
-_PROTO = re.compile(r"^\s*(int|const char\*)\s+(climb_\w+)\s*\(([^)]*)\)\s*;", re.M)
+_PROTO = re.compile(r"^\s*(int|long|const char\*)\s+(climb_\w+)\s*\(([^)]*)\)\s*;", re.M)
 
 
 def parse_header(path: str = HEADER) -> Dict[str, Tuple[str, List[str]]]:
@@ -81,7 +81,7 @@ def load():
     _protos = parse_header()
     for name, (ret, types) in _protos.items():
         fn = getattr(lib, name)   # AttributeError here == header/library mismatch
-        fn.restype = ctypes.c_int if ret == "int" else ctypes.c_char_p
+        fn.restype = {"int": ctypes.c_int, "long": ctypes.c_long}.get(ret, ctypes.c_char_p)
         fn.argtypes = [_CT[t] for t in types]
     _lib = lib
     # developer knob for A/B measurements: CLIMB_AMD_OPTIONS="7=0,5=1" -> climb_set_option(7, 0); climb_set_option(5, 1)

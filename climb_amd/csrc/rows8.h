@@ -1,0 +1,88 @@
+// Rows in 8 bits: the two code formats and the helpers their kernels share (rows8.hip, gemm_i8.hip, act8_wgrad.hip).  gfx950 only.
+//
+//   row codes (the operands of the int8 product): one fp32 scale a row, s = max(fl32(max|x| / 127), 2^-126), code = the multiple of s nearest to x
+//     (quotient x / s of the real numbers, ties to even).  A row that holds a NaN or an infinity has s = NaN and codes 0: whatever is computed from
+//     it is NaN, an overflow is not turned into a number.
+//   group codes (checkpoints): columns in groups of 64 that share a scale 2^e, e the smallest with max|x| <= 127 2^e, stored as the byte e + 127; a
+//     group that holds a NaN or an infinity has the byte 255 and codes 0, and reads back as NaN.  The power of two costs up to one bit of the step
+//     against max / 127 and buys two things: x 2^-e is exact, so no division decides a code, and code * 2^e has 7 significant bits, so it IS a number of
+//     the 16-bit operand type -- a matrix product reads a checkpoint without rounding it a second time.
+#pragma once
+#include "common.h"
+
+#define ACT8_GROUP 64
+#define ACT8_BAD 255u
+#define ACT8_EMAX 249u          // 2^122, the step of numbers above 127 * 2^121: their codes stop at 63, the largest that stands for a finite fp32 number
+// smallest stored exponent: 2^-126 keeps every step a normal fp32 / bf16 number; IEEE half has none below 2^-24 (its own smallest subnormal), so the
+// half build stops there -- an activation that came in that type has no finer bits
+#if CLIMB_H16_F16
+#define ACT8_EMIN (127 - 24)
+#else
+#define ACT8_EMIN 1
+#endif
+
+// biased exponent byte for the largest |x| of a group, given as fp32 bits without the sign (integer order = order of magnitude, NaN above inf above all
+// numbers, so one integer maximum carries "holds a NaN").  max = 1.f 2^k: 127 = 1.984375 * 2^6, so e = k - 6 while 1.f <= 1.984375, else k - 5.
+__device__ __forceinline__ unsigned act8_exp(unsigned mx) {
+  if (mx >= 0x7f800000u) return ACT8_BAD;
+  const int e = (int)(mx >> 23) - 6 + ((mx & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  return (unsigned)(e < ACT8_EMIN ? ACT8_EMIN : e);
+}
+__device__ __forceinline__ float act8_step(unsigned e) { return __uint_as_float(e == ACT8_BAD ? 0x7fc00000u : e << 23); }      // 2^(e - 127); NaN
+__device__ __forceinline__ float act8_inv(unsigned e) { return e == ACT8_BAD ? 0.f : __uint_as_float((254u - e) << 23); }
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// four codes in a word: x * inv (exact) + 1.5 * 2^23 rounds to the nearest integer, ties to even, in ONE fma and leaves it as the low byte in two's complement
+__device__ __forceinline__ unsigned act8_pack4(float a, float b, float c, float d, unsigned e) {
+  const float inv = act8_inv(e), magic = 12582912.f;
+  if (e == ACT8_EMAX) {          // (64 steps of 2^122 would be 2^128, which reads back as an infinity)
+    const float top = 63.f * 0x1p122f;
+    a = fminf(fmaxf(a, -top), top); b = fminf(fmaxf(b, -top), top); c = fminf(fmaxf(c, -top), top); d = fminf(fmaxf(d, -top), top);
+  }
+  const unsigned ua = __float_as_uint(fmaf(a, inv, magic)), ub = __float_as_uint(fmaf(b, inv, magic));
+  const unsigned uc = __float_as_uint(fmaf(c, inv, magic)), ud = __float_as_uint(fmaf(d, inv, magic));
+  const unsigned r = __builtin_amdgcn_perm(ub, ua, 0x0c0c0400u) | __builtin_amdgcn_perm(ud, uc, 0x04000c0cu);
+  return e == ACT8_BAD ? 0u : r;
+}
+__device__ __forceinline__ float4 act8_unpack4(unsigned w, float step) {
+  return make_float4((float)(signed char)(w & 255u) * step, (float)(signed char)((w >> 8) & 255u) * step, (float)(signed char)((w >> 16) & 255u) * step,
+                     (float)(signed char)(w >> 24) * step);
+}
+
+// Phi(-|x|) = exp(-x^2 / 2) R(1 / (1 + p |x|)), R a polynomial without constant term fitted to erfcx(|x| / sqrt 2) / 2 on [0, 14] for the smallest largest
+// RELATIVE error (weighted least squares, own fit): the tail keeps its digits, where 1 + erf would cancel them.  DEG 6: 8.3e-6 (results that are stored
+// in 16 bits: a 470th of their half step), DEG 8: 1.5e-7 (fp32 results).  e2 returns exp(-x^2 / 2).
+template <int DEG>
+__device__ __forceinline__ float phi_lower(float x, float& e2) {
+  const float z = fabsf(x);
+  float r, t;
+  if constexpr (DEG == 6) {
+    t = __builtin_amdgcn_rcpf(fmaf(0.30f, z, 1.0f));
+    r = fmaf(fmaf(fmaf(fmaf(fmaf(-0.07709959f, t, 0.21604484f), t, -0.01695827f), t, 0.1442025f), t, 0.11374025f), t, 0.1200744f);
+  } else {
+    t = __builtin_amdgcn_rcpf(fmaf(0.30f, z, 1.0f));
+    r = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(0.03567617f, t, -0.15720912f), t, 0.20636429f), t, -0.05369389f), t, 0.1285672f), t, 0.09991176f), t, 0.12075424f), t,
+             0.11962928f);
+  }
+  e2 = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170368f);
+  return r * t * e2;
+}
+template <typename T> struct GeluDeg { static constexpr int v = 6; };
+template <> struct GeluDeg<float> { static constexpr int v = 8; };
+// gelu(x) = x Phi(x): x >= 0: x - x q, x < 0: x q, q = Phi(-|x|)  =  max(x, 0) - |x| q.  (q and exp(-x^2 / 2) are 0 beyond |x| = 14.4: the factor is held
+// at 64 there, so that an infinity gives its limit and not inf * 0)
+template <int DEG>
+__device__ __forceinline__ float gelu_phi(float x) {
+  float e2;
+  const float q = phi_lower<DEG>(x, e2);
+  return fmaf(-fminf(fabsf(x), 64.f), q, fmaxf(x, 0.f));
+}
+// ... and gelu'(x) = Phi(x) + x exp(-x^2 / 2) / sqrt(2 pi)
+template <int DEG>
+__device__ __forceinline__ float gelu_phi_pair(float x, float& d) {
+  float e2;
+  const float q = phi_lower<DEG>(x, e2);
+  const float z = fminf(fabsf(x), 64.f);
+  d = fmaf(copysignf(z, x) * 0.39894228040143267794f, e2, x < 0.f ? q : 1.0f - q);
+  return fmaf(-z, q, fmaxf(x, 0.f));
+}

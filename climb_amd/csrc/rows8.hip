@@ -1,0 +1,457 @@
+// Row-wise kernels of the 8-bit formats (rows8.h): row codes for the int8 product, checkpoints, and the LayerNorm and GELU that write a checkpoint in
+// their forward and read it in their backward.  All are bound by HBM; each input is read once and each output written once.
+#include "rows8.h"
+
+static inline bool al(const void* p, long ld, int elems_per_16b) { return !((uintptr_t)p & 15) && ld % elems_per_16b == 0; }
+
+// N consecutive elements of a row (N = 4 or 8), `left` = columns that exist from p on.  VEC: whole rows of 16-byte pieces (the launcher's condition).
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void row_ld(const T* __restrict__ p, int left, float (&v)[N]) {
+  if constexpr (VEC) {
+    if (left > 0) {
+      if constexpr (N == 8 && sizeof(T) == 2) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        v[0] = h16lo_to_f32(r.x); v[1] = h16hi_to_f32(r.x); v[2] = h16lo_to_f32(r.y); v[3] = h16hi_to_f32(r.y);
+        v[4] = h16lo_to_f32(r.z); v[5] = h16hi_to_f32(r.z); v[6] = h16lo_to_f32(r.w); v[7] = h16hi_to_f32(r.w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 r = ld4(p + i);
+          v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+  } else {
+    if (left >= N) {          // rows at any address: the hardware reads unaligned words, hipcc makes wide loads of the copy
+      T r[N];
+      __builtin_memcpy(r, p, sizeof(r));
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = Act<T>::ld(r + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = i < left ? Act<T>::ld(p + i) : 0.f;
+    }
+  }
+}
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void row_st(T* __restrict__ p, int left, const float (&v)[N]) {
+  if constexpr (VEC) {
+    if (left > 0) {
+      if constexpr (N == 8 && sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) st4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+      }
+    }
+  } else {
+    if (left >= N) {
+      T r[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) Act<T>::st(r + i, v[i]);
+      __builtin_memcpy(p, r, sizeof(r));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) Act<T>::st(p + i, v[i]);
+    }
+  }
+}
+// largest absolute value (as bits) over the W lanes that hold a group
+template <int W>
+__device__ __forceinline__ unsigned lanes_umax(unsigned m) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    const unsigned t = __shfl_xor(m, o, 64);
+    m = t > m ? t : m;
+  }
+  return m;
+}
+
+// ------------------------------------------------------------------------------------------------ row codes
+// true-quotient rounding: k = rint(x / s) from a reciprocal may miss a tie by its rounding; the remainder x - k s is exact in one fma and settles it
+__device__ __forceinline__ int rowq(float x, float s, float rs) {
+  const float k = rintf(x * rs), r = fmaf(-k, s, x), a = 2.f * fabsf(r);
+  int q = (int)k;
+  if (a > s || (a == s && (q & 1))) q += r > 0.f ? 1 : -1;
+  return q;
+}
+__device__ __forceinline__ float row_scale(unsigned mx) {
+  return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
+}
+__device__ __forceinline__ unsigned rowq4(const float (&v)[4], float s, float rs, bool bad) {
+  const unsigned w = ((unsigned)rowq(v[0], s, rs) & 255u) | (((unsigned)rowq(v[1], s, rs) & 255u) << 8) | (((unsigned)rowq(v[2], s, rs) & 255u) << 16) |
+                     (((unsigned)rowq(v[3], s, rs) & 255u) << 24);
+  return bad ? 0u : w;
+}
+// One wave owns a row of C <= 256 NV and keeps it in registers; columns [C, Kp) of the code row are written as zeros (the product runs over whole
+// 128-byte pieces).
+template <typename T, bool VEC, int NV>
+__global__ __launch_bounds__(256) void rows8_quant_kernel(const T* __restrict__ x, long ldx, signed char* __restrict__ q, long ldq, float* __restrict__ s,
+                                                          int M, int C, int Kp) {
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= M) return;
+  float v[NV][4];
+  unsigned mx = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4;
+    row_ld<VEC, 4>(x + row * ldx + c, C - c, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[i][j]));
+  mx = lanes_umax<64>(mx);
+  const float sc = row_scale(mx), rs = 1.f / sc;
+  if (lane == 0) s[row] = sc;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4;
+    if (c < Kp) *reinterpret_cast<unsigned*>(q + row * ldq + c) = rowq4(v[i], sc, rs, mx >= 0x7f800000u);
+  }
+}
+// rows too long for one wave's registers: a workgroup a row, read twice (the second time from the caches)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void rows8_quant_long_kernel(const T* __restrict__ x, long ldx, signed char* __restrict__ q, long ldq, float* __restrict__ s,
+                                                               int C, int Kp) {
+  __shared__ unsigned red[4];
+  const long row = blockIdx.x;
+  unsigned mx = 0;
+  float v[4];
+  for (int c = threadIdx.x * 4; c < C; c += 1024) {
+    row_ld<VEC, 4>(x + row * ldx + c, C - c, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[j]));
+  }
+  mx = lanes_umax<64>(mx);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  mx = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float sc = row_scale(mx), rs = 1.f / sc;
+  if (threadIdx.x == 0) s[row] = sc;
+  for (int c = threadIdx.x * 4; c < Kp; c += 1024) {
+    row_ld<VEC, 4>(x + row * ldx + c, C - c, v);
+    *reinterpret_cast<unsigned*>(q + row * ldq + c) = rowq4(v, sc, rs, mx >= 0x7f800000u);
+  }
+}
+template <typename T, bool VEC>
+static int rows8_quant_launch(const T* x, long ldx, signed char* q, long ldq, float* s, int M, int C, hipStream_t st) {
+  const int Kp = (C + 127) / 128 * 128;
+  const dim3 grid((M + 3) / 4), blk(256);
+#define RQ(NV_) hipLaunchKernelGGL((rows8_quant_kernel<T, VEC, NV_>), grid, blk, 0, st, x, ldx, q, ldq, s, M, C, Kp)
+  if (Kp <= 256) RQ(1);
+  else if (Kp <= 768) RQ(3);
+  else if (Kp <= 1536) RQ(6);
+  else if (Kp <= 12 * 256) RQ(12);
+  else hipLaunchKernelGGL((rows8_quant_long_kernel<T, VEC>), dim3(M), blk, 0, st, x, ldx, q, ldq, s, C, Kp);
+#undef RQ
+  LAUNCH_CHECK();
+  return CLIMB_OK;
+}
+extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream) {
+  if (M < 0 || C <= 0 || C > (1 << 30) || ldx < C || ldq < (C + 127) / 128 * 128 || ldq % 16 || ((uintptr_t)q & 15)) return CLIMB_EINVAL;
+  if (M == 0) return CLIMB_OK;
+  if (!x || !q || !s) return CLIMB_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  signed char* qc = (signed char*)q;
+  if (dtype == CLIMB_DT_F32)
+    return (C % 4 == 0 && al(x, ldx, 4)) ? rows8_quant_launch<float, true>((const float*)x, ldx, qc, ldq, s, M, C, st)
+                                         : rows8_quant_launch<float, false>((const float*)x, ldx, qc, ldq, s, M, C, st);
+  if (dtype == CLIMB_DT_BF16)
+    return (C % 4 == 0 && al(x, ldx, 4)) ? rows8_quant_launch<bf16_t, true>((const bf16_t*)x, ldx, qc, ldq, s, M, C, st)
+                                         : rows8_quant_launch<bf16_t, false>((const bf16_t*)x, ldx, qc, ldq, s, M, C, st);
+  return CLIMB_EINVAL;
+}
+
+// ------------------------------------------------------------------------------------------------ checkpoints, and GELU on them
+// Eight lanes hold a group of 64 columns (8 each: 16-byte loads in 16 bits); a thread's unit is (row, group).
+//   OP 0  codes <- x                    OP 1  codes <- x, y = gelu(x)
+//   OP 2  y <- codes                    OP 3  y = x gelu'(codes), y2 = gelu(codes) if y2
+template <typename T, bool VEC, int OP>
+__global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long ldx, T* __restrict__ y, long ldy, T* __restrict__ y2, long ldy2,
+                                                   signed char* __restrict__ q, long ldq, unsigned char* __restrict__ e, long lde, unsigned units, int C, unsigned G) {
+  constexpr int DEG = GeluDeg<T>::v;
+  const unsigned u = blockIdx.x * 32u + (threadIdx.x >> 3);
+  const unsigned uu = u < units ? u : units - 1;      // (every lane takes part in the group maxima)
+  const long row = uu / G;
+  const unsigned g = uu - (unsigned)row * G;
+  const int c = (int)(g * ACT8_GROUP + (threadIdx.x & 7) * 8), left = u < units ? C - c : 0;
+  float v[8], o[8];
+  if constexpr (OP == 0 || OP == 1) {
+    row_ld<VEC, 8>(x + row * ldx + c, left, v);
+    unsigned mx = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = max(mx, abs_bits(v[i]));
+    const unsigned ex = act8_exp(lanes_umax<8>(mx));
+    if (left > 0)      // (a piece of 8 that starts inside the row lies inside ldq, a multiple of 16)
+      *reinterpret_cast<uint2*>(q + row * ldq + c) = make_uint2(act8_pack4(v[0], v[1], v[2], v[3], ex), act8_pack4(v[4], v[5], v[6], v[7], ex));
+    if ((threadIdx.x & 7) == 0 && u < units) e[row * lde + g] = (unsigned char)ex;
+    if constexpr (OP == 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = gelu_phi<DEG>(v[i]);
+      row_st<VEC, 8>(y + row * ldy + c, left, o);
+    }
+  } else {
+    uint2 w = make_uint2(0u, 0u);
+    if (left > 0) w = *reinterpret_cast<const uint2*>(q + row * ldq + c);
+    const float step = act8_step(e[row * lde + g]);
+    if constexpr (OP == 3) row_ld<VEC, 8>(x + row * ldx + c, left, v);
+    const float4 a = act8_unpack4(w.x, step), b = act8_unpack4(w.y, step);
+    const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if constexpr (OP == 2) {
+      row_st<VEC, 8>(y + row * ldy + c, left, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float dg;
+        o[i] = gelu_phi_pair<DEG>(d[i], dg);
+        v[i] *= dg;
+      }
+      row_st<VEC, 8>(y + row * ldy + c, left, v);
+      if (y2) row_st<VEC, 8>(y2 + row * ldy2 + c, left, o);
+    }
+  }
+}
+static bool ck_ok(const void* q, long ldq, const void* e, long lde, int M, int C) {
+  return M >= 0 && C > 0 && C <= (1 << 30) && ldq >= C && ldq % 16 == 0 && !((uintptr_t)q & 15) && lde >= (C + ACT8_GROUP - 1) / ACT8_GROUP && (M == 0 || (q && e));
+}
+template <int OP>
+static int act8_launch(const void* x, long ldx, int dtype, void* y, long ldy, void* y2, long ldy2, void* q, long ldq, void* e, long lde, int M, int C, void* stream) {
+  if (dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) return CLIMB_EINVAL;
+  if (!ck_ok(q, ldq, e, lde, M, C) || (OP != 2 && ldx < C) || (OP != 0 && ldy < C) || (y2 && ldy2 < C)) return CLIMB_EINVAL;
+  if (M == 0) return CLIMB_OK;
+  if ((OP != 2 && !x) || (OP != 0 && !y)) return CLIMB_EINVAL;
+  const unsigned G = (C + ACT8_GROUP - 1) / ACT8_GROUP;
+  const long units = (long)M * G;
+  if (units >= (1L << 31)) return CLIMB_EUNSUPPORTED;      // 32-bit unit numbers (137 G elements)
+  const int pe = dtype == CLIMB_DT_F32 ? 4 : 8;
+  const bool vec = C % 8 == 0 && (OP == 2 || al(x, ldx, pe)) && (OP == 0 || al(y, ldy, pe)) && (!y2 || al(y2, ldy2, pe));
+  const dim3 grid((unsigned)((units + 31) / 32)), blk(256);
+  hipStream_t st = (hipStream_t)stream;
+#define AL_(T_, V_)                                                                                                                                              \
+  hipLaunchKernelGGL((act8_kernel<T_, V_, OP>), grid, blk, 0, st, (const T_*)x, ldx, (T_*)y, ldy, (T_*)y2, ldy2, (signed char*)q, ldq, (unsigned char*)e, lde, \
+                     (unsigned)units, C, G)
+  if (dtype == CLIMB_DT_F32) { if (vec) AL_(float, true); else AL_(float, false); }
+  else { if (vec) AL_(bf16_t, true); else AL_(bf16_t, false); }
+#undef AL_
+  LAUNCH_CHECK();
+  return CLIMB_OK;
+}
+extern "C" int climb_act8_group(void) { return ACT8_GROUP; }
+extern "C" int climb_act8_save(const void* x, long ldx, int dtype, void* q, long ldq, void* e, long lde, int M, int C, void* stream) {
+  return act8_launch<0>(x, ldx, dtype, nullptr, 0, nullptr, 0, q, ldq, e, lde, M, C, stream);
+}
+extern "C" int climb_act8_load(const void* q, long ldq, const void* e, long lde, void* y, long ldy, int dtype, int M, int C, void* stream) {
+  return act8_launch<2>(nullptr, 0, dtype, y, ldy, nullptr, 0, (void*)q, ldq, (void*)e, lde, M, C, stream);
+}
+extern "C" int climb_act8_gelu_fwd(const void* u, long ldu, int dtype, void* a, long lda, void* q, long ldq, void* e, long lde, int M, int C, void* stream) {
+  return act8_launch<1>(u, ldu, dtype, a, lda, nullptr, 0, q, ldq, e, lde, M, C, stream);
+}
+extern "C" int climb_act8_gelu_bwd(const void* da, long ldda, int dtype, const void* q, long ldq, const void* e, long lde, void* du, long lddu, void* a, long lda, int M,
+                                   int C, void* stream) {
+  return act8_launch<3>(da, ldda, dtype, du, lddu, a, lda, (void*)q, ldq, (void*)e, lde, M, C, stream);
+}
+
+// ------------------------------------------------------------------------------------------------ LayerNorm
+// One wave owns a row (4 columns a lane, 256 a step); 16 lanes hold a checkpoint group.
+template <typename TO, bool VEC, int NV>
+__global__ __launch_bounds__(256) void act8_ln_fwd_kernel(const float* __restrict__ x, long ldx, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                          float eps, TO* __restrict__ y, long ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                          signed char* __restrict__ q, long ldq, unsigned char* __restrict__ e, long lde, int M, int C) {
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= M) return;
+  float v[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4;
+    row_ld<VEC, 4>(x + row * ldx + c, C - c, v[i]);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) s += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+  const float mean = wave_sum(s) / (float)C;
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int left = C - (i * 64 + lane) * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = v[i][j] - mean;
+      if (j < left) ss += d * d;
+    }
+  }
+  const float rstd = rsqrtf(wave_sum(ss) / (float)C + eps);
+  if (lane == 0) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4, left = C - c;
+    unsigned mx = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[i][j]));
+    const unsigned ex = act8_exp(lanes_umax<16>(mx));
+    if (left > 0) {
+      *reinterpret_cast<unsigned*>(q + row * ldq + c) = act8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], ex);
+      if ((lane & 15) == 0) e[row * lde + i * 4 + (lane >> 4)] = (unsigned char)ex;
+      float g[4], b[4], o[4];
+      row_ld<VEC, 4>(gamma + c, left, g);
+      row_ld<VEC, 4>(beta + c, left, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[j], b[j]);
+      row_st<VEC, 4>(y + row * ldy + c, left, o);
+    }
+  }
+}
+template <typename TO, bool VEC>
+static int act8_ln_fwd_launch(const float* x, long ldx, const float* gamma, const float* beta, float eps, TO* y, long ldy, float* mean, float* rstd, signed char* q, long ldq,
+                              unsigned char* e, long lde, int M, int C, hipStream_t st) {
+  const dim3 grid((M + 3) / 4), blk(256);
+#define LF(NV_) hipLaunchKernelGGL((act8_ln_fwd_kernel<TO, VEC, NV_>), grid, blk, 0, st, x, ldx, gamma, beta, eps, y, ldy, mean, rstd, q, ldq, e, lde, M, C)
+  if (C <= 256) LF(1);
+  else if (C <= 768) LF(3);
+  else LF(6);
+#undef LF
+  LAUNCH_CHECK();
+  return CLIMB_OK;
+}
+extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* gamma, const float* beta, float eps, void* y, long ldy, int y_dtype, float* mean, float* rstd,
+                                        void* q, long ldq, void* e, long lde, int M, int C, void* stream) {
+  if ((y_dtype != CLIMB_DT_F32 && y_dtype != CLIMB_DT_BF16) || !ck_ok(q, ldq, e, lde, M, C) || ldx < C || ldy < C) return CLIMB_EINVAL;
+  if (C > 1536) return CLIMB_EUNSUPPORTED;
+  if (M == 0) return CLIMB_OK;
+  if (!x || !gamma || !beta || !y || !mean || !rstd) return CLIMB_EINVAL;
+  // 4 elements a lane: 16-byte pieces of fp32, 8-byte pieces of the 16-bit type
+  const bool vec = C % 4 == 0 && al(x, ldx, 4) && al(y, ldy, 4) && al(gamma, 0, 4) && al(beta, 0, 4);
+  hipStream_t st = (hipStream_t)stream;
+  signed char* qc = (signed char*)q;
+  unsigned char* ec = (unsigned char*)e;
+  if (y_dtype == CLIMB_DT_F32)
+    return vec ? act8_ln_fwd_launch<float, true>(x, ldx, gamma, beta, eps, (float*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st)
+               : act8_ln_fwd_launch<float, false>(x, ldx, gamma, beta, eps, (float*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st);
+  return vec ? act8_ln_fwd_launch<bf16_t, true>(x, ldx, gamma, beta, eps, (bf16_t*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st)
+             : act8_ln_fwd_launch<bf16_t, false>(x, ldx, gamma, beta, eps, (bf16_t*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st);
+}
+
+// dx = dres + rstd (g - mean_c(g) - xh mean_c(g xh)),  g = dy gamma,  xh = (codes - mean) rstd;  partial column sums {dgamma, dbeta, colsum(dx)} of the
+// workgroup's rows in part[workgroup][3][C], summed by climb_colreduce3 in a fixed order.
+#define A8LN_WAVES 8
+#define A8LN_RPW 3          // rows a wave
+#define A8LN_ROWS (A8LN_WAVES * A8LN_RPW)
+template <typename T, bool VEC, int NV>
+__global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* __restrict__ dy, long lddy, const signed char* __restrict__ q, long ldq,
+                                                                      const unsigned char* __restrict__ e, long lde, const float* __restrict__ mean,
+                                                                      const float* __restrict__ rstd, const float* __restrict__ gamma, const float* dres, long ldr,
+                                                                      float* dx, long ldo, T* __restrict__ dcast, long ldc, float* __restrict__ part, int M, int C) {
+  __shared__ __attribute__((aligned(16))) float red[A8LN_WAVES][NV * 256];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  float ag[NV][4], ab[NV][4], as[NV][4], gm[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4;
+    row_ld<VEC, 4>(gamma + c, C - c, gm[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ag[i][j] = ab[i][j] = as[i][j] = 0.f;
+  }
+  for (int rr = 0; rr < A8LN_RPW; ++rr) {
+    const long row = (long)blockIdx.x * A8LN_ROWS + rr * A8LN_WAVES + wid;
+    if (row >= M) break;
+    const float mu = mean[row], rs = rstd[row];
+    float d[NV][4], rin[NV][4], xh[NV][4];
+    unsigned w[NV], ex[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * 64 + lane) * 4, left = C - c;
+      row_ld<VEC, 4>(dy + row * lddy + c, left, d[i]);
+      w[i] = left > 0 ? *reinterpret_cast<const unsigned*>(q + row * ldq + c) : 0u;
+      ex[i] = left > 0 ? e[row * lde + i * 4 + (lane >> 4)] : 1u;
+      if (dres) row_ld<VEC, 4>(dres + row * ldr + c, left, rin[i]);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rin[i][j] = 0.f;
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float4 xv = act8_unpack4(w[i], act8_step(ex[i]));
+      const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {          // (columns past C have d = gamma = 0: no contribution)
+        xh[i][j] = (xx[j] - mu) * rs;
+        const float g = d[i][j] * gm[i][j];
+        s1 += g;
+        s2 += g * xh[i][j];
+      }
+    }
+    const float m1 = wave_sum(s1) / (float)C, m2 = wave_sum(s2) / (float)C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * 64 + lane) * 4, left = C - c;
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j] = rin[i][j] + rs * (d[i][j] * gm[i][j] - m1 - xh[i][j] * m2);
+        ag[i][j] += d[i][j] * xh[i][j];
+        ab[i][j] += d[i][j];
+        as[i][j] += o[j];
+      }
+      row_st<VEC, 4>(dx + row * ldo + c, left, o);
+      if (dcast) row_st<VEC, 4>(dcast + row * ldc + c, left, o);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * 64 + lane) * 4;
+      const float* a = k == 0 ? ag[i] : (k == 1 ? ab[i] : as[i]);
+      *reinterpret_cast<float4*>(&red[wid][c]) = make_float4(a[0], a[1], a[2], a[3]);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += 64 * A8LN_WAVES) {
+      float t = red[0][c];
+#pragma unroll
+      for (int w = 1; w < A8LN_WAVES; ++w) t += red[w][c];
+      part[((long)blockIdx.x * 3 + k) * C + c] = t;
+    }
+  }
+}
+template <typename T, bool VEC>
+static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long ldq, const unsigned char* e, long lde, const float* mean, const float* rstd,
+                              const float* gamma, const float* dres, long ldr, float* dx, long ldo, T* dcast, long ldc, float* part, int M, int C, hipStream_t st) {
+  const dim3 grid((M + A8LN_ROWS - 1) / A8LN_ROWS), blk(64 * A8LN_WAVES);
+#define LB(NV_) \
+  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, VEC, NV_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C)
+  if (C <= 256) LB(1);
+  else if (C <= 768) LB(3);
+  else LB(6);
+#undef LB
+  LAUNCH_CHECK();
+  return CLIMB_OK;
+}
+extern "C" int climb_act8_layernorm_bwd_rows_per_block(void) { return A8LN_ROWS; }
+extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd,
+                                        const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, int M, int C,
+                                        void* stream) {
+  if ((dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) || !ck_ok(q, ldq, e, lde, M, C) || lddy < C || ldo < C || (dres_in && ldr < C) || (dcast && ldc < C))
+    return CLIMB_EINVAL;
+  if (C > 1536) return CLIMB_EUNSUPPORTED;
+  if (M == 0) return CLIMB_OK;
+  if (!dy || !mean || !rstd || !gamma || !dx || !part) return CLIMB_EINVAL;
+  const bool vec = C % 4 == 0 && al(dy, lddy, 4) && al(dx, ldo, 4) && al(gamma, 0, 4) && (!dres_in || al(dres_in, ldr, 4)) && (!dcast || al(dcast, ldc, 4));
+  hipStream_t st = (hipStream_t)stream;
+#define LBT(T_, V_)                                                                                                                                                   \
+  act8_ln_bwd_launch<T_, V_>((const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc, \
+                             part, M, C, st)
+  if (dtype == CLIMB_DT_F32) return vec ? LBT(float, true) : LBT(float, false);
+  return vec ? LBT(bf16_t, true) : LBT(bf16_t, false);
+#undef LBT
+}

@@ -252,6 +252,40 @@ int climb_gemm_split_tn_grouped_adamw(const void* probs, const void* items, cons
 int climb_attn_fwd_split(const float* qkv, const float* key_bias, float* ctx, void* ctx_split, long ctx_lo, float* lse, int B, int S_pad, int heads, int head_dim, void* stream);
 int climb_attn_bwd_split(const float* qkv, const float* key_bias, const float* dctx, const float* lse, const float* delta, float* dqkv, void* dqkv_split, long dqkv_lo, int B, int S_pad, int heads, int head_dim, void* stream);
 
+/* ---- 8-bit rows (csrc/rows8.h, gemm_i8.hip, act8_wgrad.hip; Python: climb_amd/rows8.py) ------------------------------------------------------
+ * No counterpart in the reference, which trains and evaluates in fp32.  Two formats:
+ *   row codes    q int8 [M, ldq], s fp32 [M]: x[m,k] ~ q s, s = max(max_k |x| / 127, 2^-126), q = x / s rounded to nearest even.  A row that holds a
+ *                NaN or an infinity has s = NaN, q = 0.  ldq % 16 == 0, ldq >= roundup(K, 128); columns K .. roundup(K, 128) are zero.
+ *   checkpoint   q int8 [M, ldq], e uint8 [M, lde], lde >= ceil(C / 64): x[m,c] ~ q 2^(e[m, c / 64] - 127), the smallest power of two that keeps |q| <= 127
+ *                (at least 2^-126; 2^-24 in the fp16 build).  e = 255: that group held a NaN or an infinity and reads back as NaN;
+ *                numbers beyond 63 2^122 are kept as that.  ldq % 16 == 0,
+ *                ldq >= C.  Code matrices are 16-byte aligned; the other matrices may have any row stride and alignment of their type.
+ * M = 0 is allowed everywhere (nothing is launched, except that climb_act8_weight_grad still scales C and dbias by beta). */
+/* row codes of x [M, C] (dtype 0 / 1); C <= 2^30 */
+int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);
+/* C[m,n] (c_dtype) = epi(sum_k A[m,k] B[n,k] sa[m] sb[n] + bias[n]); A / B row codes of the tokens and of the weight's rows (one scale an output channel), the
+ * sum exact in int32 (K <= 2^17).  epi: 0 none, 1 GELU (erf form; no aux_out), 2 + aux (fp32 [M,N], may be C).  bias may be NULL. */
+int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const void* B, long ldb, const float* sb, void* C, long ldc, int c_dtype, int M, int N, int K, const float* bias, int epi, const float* aux, long ldaux, void* stream);
+/* checkpoints: write one, read one back (dtype 0 / 1).  climb_act8_group() = 64, the columns that share a scale */
+int climb_act8_group(void);
+int climb_act8_save(const void* x, long ldx, int dtype, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
+int climb_act8_load(const void* q, long ldq, const void* e, long lde, void* y, long ldy, int dtype, int M, int C, void* stream);
+/* climb_layernorm_fwd that also keeps its input as a checkpoint (C <= 1536), and climb_layernorm_bwd's contract with the checkpoint in place of x: dtype = that of dy
+ * and dcast; dx fp32 (may be dres_in); part[ceil(M / R)][3][C] = { dgamma, dbeta, colsum(dx) } partials, R = climb_act8_layernorm_bwd_rows_per_block(),
+ * reduced by climb_colreduce3 */
+int climb_act8_layernorm_fwd(const float* x, long ldx, const float* gamma, const float* beta, float eps, void* y, long ldy, int y_dtype, float* mean, float* rstd, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
+int climb_act8_layernorm_bwd_rows_per_block(void);
+int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd, const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, int M, int C, void* stream);
+/* a = gelu(u) (erf form) and the checkpoint of u; du = da gelu'(checkpoint) and, if a != NULL, a = gelu(checkpoint) (the operand of the next layer's weight
+ * gradient).  dtype = that of every matrix */
+int climb_act8_gelu_fwd(const void* u, long ldu, int dtype, void* a, long lda, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
+int climb_act8_gelu_bwd(const void* da, long ldda, int dtype, const void* q, long ldq, const void* e, long lde, void* du, long lddu, void* a, long lda, int M, int C, void* stream);
+/* weight gradient from a checkpoint [M, K]: C[N,K] (fp32) = beta C + dY^T x, dbias[N] (may be NULL) = beta dbias + column sums of dY; dY [M,N] 16-bit, fp32
+ * accumulation, no atomics (run-to-run identical).  beta 0: C and dbias are not read.  workspace: 16-byte aligned, at least
+ * climb_act8_weight_grad_workspace(M, N, K) bytes (0: none needed), scratch of this call alone */
+long climb_act8_weight_grad_workspace(int M, int N, int K);
+int climb_act8_weight_grad(const void* dY, long lddy, const void* q, long ldq, const void* e, long lde, float* C, long ldc, float* dbias, int M, int N, int K, float beta, void* workspace, long workspace_bytes, void* stream);
+
 /* ---- image pre-processing on the device (replaces the host call REF/modeling/vilt.py:86-96 -> ViltProcessor ->
  * transformers image_processing_pil_vilt.py:127-242 -> Pillow Resample.c).  All images of a batch live in byte arenas; `table` holds
  * 16 longs per image: byte offsets of its raw [sh][sw][3] pixels, its [sh][dw][3] intermediate and its [dh][dw][3] result, then

@@ -1,0 +1,113 @@
+"""8-bit rows, host side: what the C entry points and the tensor calls refuse (nothing here reaches a GPU)."""
+import ctypes
+
+import pytest
+import torch
+
+from climb_amd import _lib, rows8
+
+EINVAL, EUNSUPPORTED = -1, -2
+
+
+def _rc(name, *args):
+    return int(getattr(_lib.load(), name)(*args))
+
+
+@pytest.fixture(scope="module")
+def mem():
+    """a host address that stands for a device buffer: every call below must return before it touches one"""
+    buf = ctypes.create_string_buffer(4096)
+    return (ctypes.addressof(buf) + 63) & ~63, buf
+
+
+@pytest.mark.parametrize("change", [dict(M=-1), dict(C=0), dict(ldx=99), dict(ldq=100), dict(ldq=120), dict(dtype=2), dict(x=None), dict(q=None), dict(s=None), dict(qoff=1)])
+def test_quantiser_refuses(mem, change):
+    p = mem[0]
+    a = dict(M=4, C=100, ldx=100, ldq=128, dtype=1, x=p, q=p, s=p, qoff=0)
+    a.update(change)
+    q = None if a["q"] is None else a["q"] + a["qoff"]
+    assert _rc("climb_rows8_quant", a["x"], a["ldx"], a["dtype"], q, a["ldq"], a["s"], a["M"], a["C"], None) == EINVAL
+
+
+@pytest.mark.parametrize("change,rc", [(dict(M=-1), EINVAL), (dict(N=0), EINVAL), (dict(K=0), EINVAL), (dict(lda=64), EINVAL), (dict(ldb=120), EINVAL), (dict(lda=136), EINVAL),
+                                       (dict(ldc=31), EINVAL), (dict(epi=3), EINVAL), (dict(epi=2), EINVAL), (dict(epi=2, aux=1, ldaux=8), EINVAL), (dict(c_dtype=2), EINVAL),
+                                       (dict(sa=None), EINVAL), (dict(A=None), EINVAL), (dict(C=None), EINVAL), (dict(aoff=8), EINVAL),
+                                       (dict(K=(1 << 17) + 1, lda=1 << 18, ldb=1 << 18), EUNSUPPORTED), (dict(lda=1 << 22), EUNSUPPORTED)])
+def test_int8_product_refuses(mem, change, rc):
+    p = mem[0]
+    a = dict(M=4, N=32, K=100, lda=128, ldb=128, ldc=32, epi=0, aux=None, ldaux=0, c_dtype=0, A=p, B=p, C=p, sa=p, sb=p, aoff=0)
+    a.update(change)
+    A = None if a["A"] is None else a["A"] + a["aoff"]
+    aux = p if a["aux"] else None
+    assert _rc("climb_gemm_i8_nt", A, a["lda"], a["sa"], a["B"], a["ldb"], a["sb"], a["C"], a["ldc"], a["c_dtype"], a["M"], a["N"], a["K"], None, a["epi"], aux, a["ldaux"],
+               None) == rc
+
+
+@pytest.mark.parametrize("change", [dict(M=-1), dict(C=0), dict(ldq=96), dict(ldq=104), dict(lde=1), dict(dtype=2), dict(x=None), dict(q=None), dict(e=None), dict(ldx=99)])
+def test_checkpoint_calls_refuse(mem, change):
+    p = mem[0]
+    a = dict(M=4, C=100, ldx=100, ldq=112, lde=2, dtype=0, x=p, q=p, e=p)
+    a.update(change)
+    ck = (a["q"], a["ldq"], a["e"], a["lde"])
+    mc = (a["M"], a["C"], None)
+    assert _rc("climb_act8_save", a["x"], a["ldx"], a["dtype"], *ck, *mc) == EINVAL
+    assert _rc("climb_act8_load", *ck, a["x"], a["ldx"], a["dtype"], *mc) == EINVAL
+    assert _rc("climb_act8_gelu_fwd", a["x"], a["ldx"], a["dtype"], p, 100, *ck, *mc) == EINVAL
+    assert _rc("climb_act8_gelu_bwd", a["x"], a["ldx"], a["dtype"], *ck, p, 100, None, 0, *mc) == EINVAL
+    assert _rc("climb_act8_layernorm_fwd", p, 100, p, p, 1e-5, a["x"], a["ldx"], a["dtype"], p, p, *ck, *mc) == EINVAL
+    assert _rc("climb_act8_layernorm_bwd", a["x"], a["ldx"], a["dtype"], *ck, p, p, p, None, 0, p, 100, None, 0, p, *mc) == EINVAL
+
+
+def test_layernorm_refuses_rows_it_cannot_hold(mem):
+    p = mem[0]
+    assert _rc("climb_act8_layernorm_fwd", p, 1540, p, p, 1e-5, p, 1540, 0, p, p, p, 1552, p, 25, 4, 1540, None) == EUNSUPPORTED
+    assert _rc("climb_act8_layernorm_bwd", p, 1540, 0, p, 1552, p, 25, p, p, p, None, 0, p, 1540, None, 0, p, 4, 1540, None) == EUNSUPPORTED
+
+
+def test_weight_gradient_refuses_and_asks_for_its_workspace(mem):
+    p = mem[0]
+    ok = dict(dY=p, lddy=96, q=p, ldq=112, e=p, lde=2, C=p, ldc=100, M=4096, N=96, K=100, ws=p)
+    need = _rc("climb_act8_weight_grad_workspace", 4096, 96, 100)
+    assert need > 0 and need % (4 * (96 * 100 + 96)) == 0
+    assert _rc("climb_act8_weight_grad_workspace", 100, 96, 100) == 0          # one token range: straight into C
+    assert _rc("climb_act8_weight_grad_workspace", -1, 96, 100) == EINVAL
+
+    def call(nbytes=need, **change):
+        a = dict(ok, **change)
+        return _rc("climb_act8_weight_grad", a["dY"], a["lddy"], a["q"], a["ldq"], a["e"], a["lde"], a["C"], a["ldc"], None, a["M"], a["N"], a["K"], 0.0, a["ws"], nbytes, None)
+    for change in (dict(M=-1), dict(N=0), dict(K=0), dict(lddy=95), dict(ldq=96), dict(ldq=104), dict(lde=1), dict(ldc=99), dict(dY=None), dict(q=p + 1), dict(e=None),
+                   dict(C=None), dict(C=p + 2), dict(dY=p + 1), dict(ws=None), dict(ws=p + 4)):
+        assert call(**change) == EINVAL, change
+    assert call(nbytes=need - 1) == EINVAL
+
+
+def test_nothing_is_launched_for_no_rows():
+    z = (0, 64, None)
+    assert _rc("climb_rows8_quant", None, 64, 0, None, 128, None, *z) == 0
+    assert _rc("climb_act8_save", None, 64, 0, None, 64, None, 1, *z) == 0
+    assert _rc("climb_gemm_i8_nt", None, 128, None, None, 128, None, None, 32, 0, 0, 32, 64, None, 0, None, 0, None) == 0
+
+
+def test_tensor_calls_refuse():
+    x = torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="HIP device"):
+        rows8.quantize_rows(x)
+    with pytest.raises(ValueError, match="HIP device"):
+        rows8.checkpoint_save(x)
+    with pytest.raises(ValueError, match="HIP device"):
+        rows8.gelu_fwd(x)
+    with pytest.raises(TypeError, match="tensor"):
+        rows8.checkpoint_save([1.0])
+    with pytest.raises(RuntimeError, match="autograd"):
+        rows8.gelu_fwd(torch.zeros(4, 8, requires_grad=True))
+    w = rows8.RowCodes(torch.zeros(3, 128, dtype=torch.int8), torch.ones(3), 8, (3,))
+    with pytest.raises(ValueError, match="epilogue"):
+        rows8.linear_i8(x, w, epi="tanh")
+    with pytest.raises(ValueError, match="resid"):
+        rows8.linear_i8(x, w, epi="resid")
+    with pytest.raises(TypeError, match="RowCodes"):
+        rows8.linear_i8(x, x)
+    ck = rows8.Checkpoint(4, 8, (4,), torch.float32, torch.device("cpu"))
+    with pytest.raises(ValueError, match="row statistics"):
+        rows8.layernorm_bwd(x, ck, torch.ones(8))
+    assert ck.nbytes == 4 * 16 + 4 and rows8.GROUP == _lib.query("climb_act8_group")
