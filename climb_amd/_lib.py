@@ -108,7 +108,15 @@ def _conv(a):
 def call(name: str, *args):
     """Invoke an `int climb_*` launcher; tensors are passed as raw device pointers; non-zero -> RuntimeError."""
     fn = getattr(load(), name)
-    rc = fn(*[_conv(a) for a in args])
+    check(name, fn(*[_conv(a) for a in args]))
+
+
+def bound(name: str):
+    """The ctypes function itself, for callers on a hot path that convert their own arguments (device pointers as ints) and check() what it returns."""
+    return getattr(load(), name)
+
+
+def check(name: str, rc: int):
     if rc != 0:
         raise RuntimeError(f"{name} failed: {error_string(rc)} (code {rc})")
 

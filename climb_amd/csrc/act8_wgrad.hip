@@ -168,58 +168,309 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restric
     }
   }
 }
-// C = beta C + the splits' sums, in the order of the splits
+// C = beta C + the splits' sums, in the order of the splits; the bias sums lie behind the splits' planes, `bplanes` of them.  V columns a thread.
+template <int V>
 __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __restrict__ part, float* __restrict__ C, long ldc, float* __restrict__ dbias, int N, int K,
-                                                                int splits, float beta) {
+                                                                int splits, int bplanes, float beta) {
   const long NK = (long)N * K;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < NK + (dbias ? N : 0); i += (long)gridDim.x * 256) {
-    const bool w = i < NK;
-    const float* p = w ? part + i : part + splits * NK + (i - NK);
-    const long stride = w ? NK : N;
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += p[k * stride];
-    const long n = w ? i / K : 0;
-    float* o = w ? C + n * ldc + (i - n * K) : dbias + (i - NK);
-    *o = beta != 0.f ? fmaf(beta, *o, s) : s;
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * V; i < NK; i += (long)gridDim.x * 256 * V) {
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      float v[V];
+      __builtin_memcpy(v, part + (long)k * NK + i, sizeof(v));
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += v[j];
+    }
+    const long n = i / K;          // (V divides K: one row)
+    float* o = C + n * ldc + (i - n * K);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = beta != 0.f ? fmaf(beta, o[j], s[j]) : s[j];
+  }
+  if (dbias)
+    for (int n = blockIdx.x * 256 + threadIdx.x; n < N; n += gridDim.x * 256) {
+      float s = 0.f;
+      for (int k = 0; k < bplanes; ++k) s += part[(long)splits * NK + (long)k * N + n];
+      dbias[n] = beta != 0.f ? fmaf(beta, dbias[n], s) : s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ large, aligned problems
+// The same sum on 256 (n) x 256 (k) tiles, one workgroup of 8 waves a CU (4 x 2 waves of 64 x 128): a code is expanded once for 256 channels (the 128-tile
+// kernel is bound by that VALU work).  Everything comes to LDS by DMA: a ring of 5 stages { gradients [32 tokens][256] , codes [32][256], exponents }, and two
+// images of expanded codes.  The step that multiplies token tile t (two groups of 8 MFMAs)
+//   - expands the codes of tile t + 1 between the MFMAs of its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
+//   - meets the workgroup in the second group; behind the barrier the ring slot of tile t takes the DMA of tile t + 5, and the first fragments of tile t + 1
+//     are read under the rest of the group.
+// As in gemm_i8.hip fragments are read behind the first MFMA of the group before, and no load goes to registers: hipcc would wait for all DMA with it.
+#define WB_T 256
+#define WB_BR 32
+#define WB_PITCH 512
+#define WB_IMG (WB_BR * WB_PITCH)                       // 16 KB
+#define WB_CODES (WB_BR * WB_T)                         // 8 KB
+#define WB_STAGE (WB_IMG + WB_CODES + 256)
+#define WB_RING 5
+#define WB_LDS (WB_RING * WB_STAGE + 2 * WB_IMG)
+#define WB_LPT 4                                        // DMA instructions of a stage and lane: 2 gradients, 1 codes, 1 exponents
+__device__ __forceinline__ bf16x8 wb_frag(const unsigned char* __restrict__ p) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  union { s16x4 h[2]; bf16x8 b; } c;
+  c.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+  c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * WB_PITCH));
+  return c.b;
+}
+// 16 codes -> 16 numbers of the operand type.  Offset binary: byte ^ 128 is code + 128 in 0 .. 255, one conversion, and one fma takes the offset out (exact)
+__device__ __forceinline__ void wb_expand(u32x4 q, unsigned e4, bool live, unsigned char* __restrict__ Bs) {
+  const int row = threadIdx.x >> 4, c16 = threadIdx.x & 15;
+  const float step = live ? act8_step((e4 >> ((c16 >> 2) * 8)) & 255u) : 0.f, off = -128.f * step;
+  unsigned h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned w = q[i] ^ 0x80808080u;
+    const float a = fmaf((float)(w & 255u), step, off), b = fmaf((float)((w >> 8) & 255u), step, off);
+    const float c = fmaf((float)((w >> 16) & 255u), step, off), d = fmaf((float)(w >> 24), step, off);
+    h[2 * i] = pack_bf16x2(a, b);
+    h[2 * i + 1] = pack_bf16x2(c, d);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<u32x4*>(Bs + row * WB_PITCH + (((c16 * 2 + i) ^ wg_swz(row)) << 4)) = (u32x4){h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]};
+}
+__global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __restrict__ dY, long lddy, const signed char* __restrict__ q, long ldq,
+                                                             const unsigned char* __restrict__ e, long lde, float* __restrict__ out, int want_bias, int M, int N, int K,
+                                                             int rows, int splits) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // the ring, then the two expanded images
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wid >> 1, wk = wid & 1, half = lane >> 5, l31 = lane & 31;
+  const int nbn = (N + WB_T - 1) / WB_T, nbk = (K + WB_T - 1) / WB_T, tiles = nbn * nbk;
+  int bid = blockIdx.x;
+  {          // XCD-contiguous chunks: the workgroups of an XCD belong to the same token range, whose panels its L2 then holds once
+    const int nwg = gridDim.x, c = nwg / 8, rr = nwg % 8, xcd = bid % 8, idx = bid / 8;
+    bid = (xcd < rr ? xcd * (c + 1) : rr * (c + 1) + (xcd - rr) * c) + idx;
+  }
+  const int split = bid / tiles, tile = bid - split * tiles;
+  const int ntile = nbn > nbk ? tile / nbk : tile % nbn, ktile = nbn > nbk ? tile % nbk : tile / nbn;
+  const int n0 = ntile * WB_T, k0 = ktile * WB_T, mbeg = split * rows, mend = min(M, mbeg + rows);
+  const int nt = (mend - mbeg + WB_BR - 1) / WB_BR;          // (the launcher leaves no split empty)
+  // DMA sources of a lane, relative to the first token of a stage; columns past the end repeat the last piece (their results are not stored), tokens past the
+  // end the last one (their codes expand to zeros, their gradients are cleared)
+  const int arow = threadIdx.x >> 5;          // rows arow and arow + 16 of the gradients
+  const unsigned acol = (unsigned)min(n0 + (int)((threadIdx.x & 31) ^ wg_swz(arow)) * 8, N - 8) * 2, ldb = (unsigned)lddy * 2;
+  const int qrow = threadIdx.x >> 4;
+  const unsigned qcol = (unsigned)min(k0 + (int)(threadIdx.x & 15) * 16, (K - 1) & ~15);
+  // running sources of the next stage to fetch, and its distance from the end
+  const unsigned char* ap = reinterpret_cast<const unsigned char*>(dY + (long)mbeg * lddy);
+  const signed char* qp = q + (long)mbeg * ldq;
+  const unsigned char* ep = e + (long)mbeg * lde + (k0 >> 6);
+  const long astep = (long)WB_BR * lddy * 2, qstep = (long)WB_BR * ldq, estep = (long)WB_BR * lde;
+  int dleft = mend - mbeg;
+  const unsigned av0 = (unsigned)arow * ldb + acol, av1 = (unsigned)(arow + 16) * ldb + acol, qv = (unsigned)qrow * (unsigned)ldq + qcol, ev = (unsigned)l31 * (unsigned)lde;
+  auto dma = [&](unsigned char* S) {
+    unsigned a0 = av0, a1 = av1, qo = qv, eo = ev;
+    if (dleft < WB_BR) {
+      const int last = dleft - 1;
+      a0 = (unsigned)min(arow, last) * ldb + acol;
+      a1 = (unsigned)min(arow + 16, last) * ldb + acol;
+      qo = (unsigned)min(qrow, last) * (unsigned)ldq + qcol;
+      eo = (unsigned)min(l31, last) * (unsigned)lde;
+    }
+    __builtin_amdgcn_global_load_lds((gbl_void_t*)(ap + a0), (lds_void_t*)(S + wid * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gbl_void_t*)(ap + a1), (lds_void_t*)(S + 8192 + wid * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gbl_void_t*)(qp + qo), (lds_void_t*)(S + WB_IMG + wid * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gbl_void_t*)(ep + eo), (lds_void_t*)(S + WB_IMG + WB_CODES), 4, 0, 0);          // (every wave fetches the 32 words of exponents: it
+    ap += astep; qp += qstep; ep += estep; dleft -= WB_BR;                                                            // waits for its own loads only)
+  };
+  unsigned char* bimg = smem + WB_RING * WB_STAGE;
+  // fragment addresses: A blocks 2 (n), B blocks 4 (k), rows ms * 16 + frow
+  const int g16 = lane >> 4, i16 = lane & 15, frow = (g16 >> 1) * 8 + (i16 >> 2), fcol = (g16 & 1) * 16 + 4 * (i16 & 3);
+  unsigned aoff[2], boff[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) { const int c = wn * 64 + i * 32 + fcol; aoff[i] = frow * WB_PITCH + (((c >> 3) ^ wg_swz(frow)) << 4) + (c & 7) * 2; }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { const int c = wk * 128 + j * 32 + fcol; boff[j] = frow * WB_PITCH + (((c >> 3) ^ wg_swz(frow)) << 4) + (c & 7) * 2; }
+  f32x16 acc[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  float bsum[2] = {0.f, 0.f};
+  bf16x8 fa[2][2], fb[2][4];
+  auto frags = [&](bf16x8(&a)[2], bf16x8(&b)[4], const unsigned char* stage, const unsigned char* img, int ms) {
+    const unsigned char *A = stage + ms * (16 * WB_PITCH), *B = img + ms * (16 * WB_PITCH);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) a[i] = wb_frag(A + aoff[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = wb_frag(B + boff[j]);
+  };
+  u32x4 raw;
+  unsigned e4;
+  auto raw_read = [&](const unsigned char* stage) {
+    raw = *reinterpret_cast<const u32x4*>(stage + WB_IMG + threadIdx.x * 16);
+    e4 = *reinterpret_cast<const unsigned*>(stage + WB_IMG + WB_CODES + qrow * 4);
+  };
+  // the gradients of tokens past the end become zero rows (an infinity must not meet a zero code, and the bias sums run over all rows): every lane clears what
+  // it fetched itself, once that has landed and before the barrier behind which the stage is read
+  const int valid = (mend - mbeg - 1) % WB_BR + 1;          // tokens of the last stage
+  auto clear_tail = [&](unsigned char* stage) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (arow + 16 * i >= valid) *reinterpret_cast<u32x4*>(stage + i * 8192 + threadIdx.x * 16) = (u32x4){0u, 0u, 0u, 0u};
+  };
+  for (int t = 0; t < WB_RING && t < nt; ++t) dma(smem + t * WB_STAGE);
+  if (nt >= WB_RING) wait_vmcnt<(WB_RING - 2) * WB_LPT>();          // stages 0 and 1 have landed
+  else wait_vmcnt<0>();
+  if (valid < WB_BR && nt <= 2) clear_tail(smem + (nt - 1) * WB_STAGE);
+  raw_read(smem);
+  int qm = mend - mbeg - qrow;          // > 0: this lane's token of the tile it expands exists
+  wb_expand(raw, e4, qm > 0, bimg);
+  raw_read(smem + (nt > 1 ? WB_STAGE : 0));
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  frags(fa[0], fb[0], smem, bimg, 0);
+  unsigned char *s0 = smem, *s1 = smem + WB_STAGE, *s2 = smem + 2 * WB_STAGE, *img = bimg, *img1 = bimg + WB_IMG;          // stages t, t + 1, t + 2; images t, t + 1
+  int bias_in = want_bias && wk == 0 ? ktile : 1 << 30;          // tiles until this workgroup's next share of the bias sums
+  // (the last steps expand and read what is left in LDS from earlier tiles: nothing of it is used)
+  for (int t = 0; t < nt; ++t) {
+    const bool bias_tile = bias_in == 0;
+    bias_in = bias_tile ? nbk - 1 : bias_in - 1;
+    qm -= WB_BR;
+#pragma unroll
+    for (int ms = 0; ms < 2; ++ms) {
+      acc[0][0] = CLIMB_MFMA_H16(fa[ms][0], fb[ms][0], acc[0][0], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (ms == 0) {
+        frags(fa[1], fb[1], s0, img, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        wb_expand(raw, e4, qm > 0, img1);
+      } else {
+        if (t + WB_RING - 1 < nt) wait_vmcnt<(WB_RING - 3) * WB_LPT>();          // stage t + 2 has landed, t + 3 and t + 4 may be out
+        else wait_vmcnt<0>();
+        if (t + 3 == nt && valid < WB_BR) clear_tail(s2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        frags(fa[0], fb[0], s1, img1, 0);
+        raw_read(s2);
+        if (t + WB_RING < nt) dma(s0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i || j) acc[i][j] = CLIMB_MFMA_H16(fa[ms][i], fb[ms][j], acc[i][j], 0, 0, 0);
+      if (ms == 0) {          // the expansion's ~50 VALU operations between the 7 MFMAs
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (bias_tile) {          // (a fragment holds 8 tokens of one channel; the tiles are dealt to the workgroups that share the channels)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          union { bf16x8 b; unsigned u[4]; } c;
+          c.b = fa[ms][i];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) bsum[i] += h16lo_to_f32(c.u[w]) + h16hi_to_f32(c.u[w]);
+        }
+      }
+    }
+    s0 = s1; s1 = s2;
+    s2 = s2 == smem + (WB_RING - 1) * WB_STAGE ? smem : s2 + WB_STAGE;
+    unsigned char* x = img; img = img1; img1 = x;
+  }
+  float* o = out + (long)split * N * K;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + wk * 128 + j * 32 + l31;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+        if (n < N && k < K) o[(long)n * K + k] = acc[i][j][r];
+      }
+    }
+  if (want_bias && wk == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float s = bsum[i] + __shfl_xor(bsum[i], 32, 64);
+      const int n = n0 + wn * 64 + i * 32 + l31;
+      if (half == 0 && n < N) out[(long)splits * N * K + ((long)split * nbk + ktile) * N + n] = s;
+    }
   }
 }
 
-// token ranges the reduction is cut into: enough for two workgroups a CU, none shorter than 256 tokens (below that the second launch costs more)
-static int wgrad_splits(int M, int N, int K) {
-  const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
-  const long s = 512 / tiles, most = M / 256;
-  const long r = s < most ? s : most;
-  return r < 1 ? 1 : (int)r;
+// The plan of a problem: which kernel, and into how many token ranges the reduction is cut.
+//   small: 128 x 128 tiles, two workgroups a CU, no range below 256 tokens (below that the second launch costs more)
+//   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, and enough tokens for every
+//          CU to have 512 of them
+struct WgPlan { bool big; int splits, rows; long ws; };
+static_assert(WB_LDS <= 160 * 1024, "LDS");
+static WgPlan wgrad_plan(int M, int N, int K, bool aligned) {
+  WgPlan p;
+  const long bt = (long)((N + WB_T - 1) / WB_T) * ((K + WB_T - 1) / WB_T), st = (long)((N + 127) / 128) * ((K + 127) / 128);
+  const long mtiles = ((long)M + WG_BR - 1) / WG_BR, bs = bt <= 256 ? 256 / bt : 1;
+  p.big = aligned && N % 8 == 0 && N >= 256 && K >= 256 && bt <= 256 && bs * bt >= 192 && mtiles >= 8 * bs;
+  long s = 512 / st, most = M / 256;
+  s = p.big ? bs : (s < most ? s : most);
+  if (s < 1) s = 1;
+  p.rows = M > 0 ? (int)((mtiles + s - 1) / s * WG_BR) : 1;
+  p.splits = M > 0 ? (int)(((long)M + p.rows - 1) / p.rows) : 1;          // (no range is empty)
+  const long bplanes = p.big ? (long)p.splits * ((K + WB_T - 1) / WB_T) : p.splits;
+  p.ws = p.splits == 1 && !p.big ? 0 : ((long)p.splits * N * K + bplanes * N) * 4;
+  return p;
 }
 extern "C" long climb_act8_weight_grad_workspace(int M, int N, int K) {
-  if (M < 0 || N <= 0 || K <= 0) return CLIMB_EINVAL;
-  const int s = wgrad_splits(M, N, K);
-  return s == 1 ? 0 : (long)s * ((long)N * K + N) * 4;
+  if (M < 0 || M > (1 << 30) || N <= 0 || K <= 0) return CLIMB_EINVAL;
+  const long a = wgrad_plan(M, N, K, true).ws, b = wgrad_plan(M, N, K, false).ws;          // (alignments are not known here)
+  return a > b ? a : b;
 }
 extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, long ldq, const void* e, long lde, float* C, long ldc, float* dbias, int M, int N, int K,
                                       float beta, void* workspace, long workspace_bytes, void* stream) {
-  if (M < 0 || M > (1 << 30) || N <= 0 || K <= 0 || lddy < N || ldc < K || ldq < K || ldq % 16 || ((uintptr_t)q & 15) || lde < (K + ACT8_GROUP - 1) / ACT8_GROUP || !C) return CLIMB_EINVAL;
+  if (M < 0 || M > (1 << 30) || N <= 0 || K <= 0 || lddy < N || ldc < K || ldq < K || ldq % 16 || ((uintptr_t)q & 15) || lde < (K + ACT8_GROUP - 1) / ACT8_GROUP || !C)
+    return CLIMB_EINVAL;
   if (M > 0 && (!dY || !q || !e)) return CLIMB_EINVAL;
   if (((uintptr_t)dY & 1) || ((uintptr_t)C & 3) || ((uintptr_t)dbias & 3)) return CLIMB_EINVAL;
-  const int splits = wgrad_splits(M, N, K);
+  const WgPlan p = wgrad_plan(M, N, K, lddy % 8 == 0 && !((uintptr_t)dY & 15) && lde % 4 == 0 && !((uintptr_t)e & 3) && lddy < (1L << 24) && ldq < (1L << 24));
   const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
-  if (tiles * splits >= (1L << 31)) return CLIMB_EUNSUPPORTED;
+  if (tiles * p.splits >= (1L << 31)) return CLIMB_EUNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(tiles * splits)), blk(256);
-  if (splits == 1) {
-    hipLaunchKernelGGL((act8_wgrad_kernel<false>), grid, blk, 0, st, (const bf16_t*)dY, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, C, ldc, dbias, M, N, K,
-                       M > 0 ? M : 1, 1, beta);
+  const bf16_t* dy = (const bf16_t*)dY;
+  const signed char* qc = (const signed char*)q;
+  const unsigned char* ec = (const unsigned char*)e;
+  if (p.ws == 0) {
+    hipLaunchKernelGGL((act8_wgrad_kernel<false>), dim3((unsigned)tiles), dim3(256), 0, st, dy, lddy, qc, ldq, ec, lde, C, ldc, dbias, M, N, K, M > 0 ? M : 1, 1, beta);
     LAUNCH_CHECK();
     return CLIMB_OK;
   }
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < climb_act8_weight_grad_workspace(M, N, K)) return CLIMB_EINVAL;
-  const int rows = ((M + splits - 1) / splits + WG_BR - 1) / WG_BR * WG_BR;
-  hipLaunchKernelGGL((act8_wgrad_kernel<true>), grid, blk, 0, st, (const bf16_t*)dY, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, (float*)workspace, K, dbias,
-                     M, N, K, rows, splits, 0.f);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.ws) return CLIMB_EINVAL;
+  float* ws = (float*)workspace;
+  int bplanes = p.splits;
+  if (p.big) {
+    const int nbk = (K + WB_T - 1) / WB_T, lds = WB_LDS;
+    bplanes *= nbk;
+    hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(act8_wgrad_big_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (err != hipSuccess) return (int)err;
+    hipLaunchKernelGGL(act8_wgrad_big_kernel, dim3((N + WB_T - 1) / WB_T * nbk * p.splits), dim3(512), lds, st, dy, lddy, qc, ldq, ec, lde, ws, dbias != nullptr, M, N, K, p.rows,
+                       p.splits);
+  } else {
+    hipLaunchKernelGGL((act8_wgrad_kernel<true>), dim3((unsigned)(tiles * p.splits)), dim3(256), 0, st, dy, lddy, qc, ldq, ec, lde, ws, K, dbias, M, N, K, p.rows, p.splits, 0.f);
+  }
   LAUNCH_CHECK();
-  const long work = (long)N * K + N;
-  const unsigned rg = (unsigned)((work + 255) / 256 < 4096 ? (work + 255) / 256 : 4096);
-  hipLaunchKernelGGL(act8_wgrad_reduce_kernel, dim3(rg), blk, 0, st, (const float*)workspace, C, ldc, dbias, N, K, splits, beta);
+  const bool v4 = K % 4 == 0 && ldc % 4 == 0;
+  const long pieces = ((long)N * K / (v4 ? 4 : 1) + 255) / 256;
+  const dim3 rg((unsigned)(pieces < 1 ? 1 : (pieces < 4096 ? pieces : 4096)));
+  if (v4) hipLaunchKernelGGL((act8_wgrad_reduce_kernel<4>), rg, dim3(256), 0, st, ws, C, ldc, dbias, N, K, p.splits, bplanes, beta);
+  else hipLaunchKernelGGL((act8_wgrad_reduce_kernel<1>), rg, dim3(256), 0, st, ws, C, ldc, dbias, N, K, p.splits, bplanes, beta);
   LAUNCH_CHECK();
   return CLIMB_OK;
 }

@@ -8,23 +8,25 @@
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(16))) int i32x16;
 
-#define I8_BK 128          // bytes of K in a stage: one 128-byte line of every operand row
+#define I8_BK 128          // the code rows are whole 128-byte pieces
 
-// LDS image of an operand tile: [rows][128 B], 16-byte chunk c of row r at position c ^ (r & 7): the fragment reads (16 bytes a lane, 32 rows x 2
-// neighbouring chunks) then touch every bank group once.  global_load_lds writes LDS linearly, so the swizzle is applied to the SOURCE address.
-template <int ROWS, int NT>
+// LDS image of an operand tile: [rows][BK bytes], 16-byte chunk c of row r at position c ^ i8_swz(r): the 16 rows that a fragment read (16 bytes a lane, 32 rows
+// of one chunk) takes in a cycle lie in 16 different 16-byte slots of the 256-byte bank line.  global_load_lds writes LDS linearly, so the swizzle is applied to the
+// SOURCE address.
+template <int BK> __device__ __forceinline__ int i8_swz(int row) { return BK == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+template <int ROWS, int NT, int BK>
 struct I8Src {
-  static constexpr int CNT = ROWS * 8 / NT;
+  static constexpr int CPR = BK / 16, CNT = ROWS * CPR / NT;
   unsigned off[CNT];          // per lane: byte offsets from the tile's first row
   __device__ __forceinline__ void init(int row0, int R, long ld) {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int slot = i * NT + threadIdx.x, row = slot >> 3, c = (slot & 7) ^ (row & 7);
+      const int slot = i * NT + threadIdx.x, row = slot / CPR, c = (slot % CPR) ^ i8_swz<BK>(row);
       off[i] = (unsigned)(min(row, R - 1 - row0) * (unsigned)ld) + c * 16;          // rows past the end repeat the last one: their results are not stored
     }
   }
   __device__ __forceinline__ void issue(const signed char* __restrict__ base, unsigned char* __restrict__ S) const {
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < CNT; ++i)
       __builtin_amdgcn_global_load_lds((gbl_void_t*)(base + off[i]), (lds_void_t*)(S + (i * NT + wave * 64) * 16), 16, 0, 0);
@@ -49,31 +51,31 @@ __device__ __forceinline__ void i8_load4(const float* __restrict__ p, float (&v)
 }
 
 // WN x WM waves of (32 NI channels) x (32 MJ tokens); S stages in LDS.
-template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int S>
-__global__ __launch_bounds__(64 * WN * WM) void gemm_i8_kernel(const signed char* __restrict__ A, long lda, const float* __restrict__ sa,
+template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
+__global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed char* __restrict__ A, long lda, const float* __restrict__ sa,
                                                                const signed char* __restrict__ B, long ldb, const float* __restrict__ sb, TO* __restrict__ C,
                                                                long ldc, int M, int N, int nk, const float* __restrict__ bias, const float* __restrict__ aux,
                                                                long ldaux, int vec) {
-  constexpr int NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * I8_BK, LPT = I8Src<BN, NT>::CNT + I8Src<BM, NT>::CNT;
+  constexpr int NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * BK, LPT = I8Src<BN, NT, BK>::CNT + I8Src<BM, NT, BK>::CNT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // S stages, then BM token scales
   float* sas = reinterpret_cast<float*>(smem + S * STAGE);
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wn = wid % WN, wm = wid / WN, half = lane >> 5, l31 = lane & 31;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wid % WN, wm = wid / WN, half = lane >> 5, l31 = lane & 31;
   int tm, tn;
   const int nbm = (M + BM - 1) / BM, nbn = (N + BN - 1) / BN;
   nt_tile<8>(nbm, nbn, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  I8Src<BN, NT> srcB;
-  I8Src<BM, NT> srcA;
+  I8Src<BN, NT, BK> srcB;
+  I8Src<BM, NT, BK> srcA;
   srcB.init(n0, N, ldb);
   srcA.init(m0, M, lda);
   const signed char* Bp = B + (long)n0 * ldb;
   const signed char* Ap = A + (long)m0 * lda;
   for (int i = threadIdx.x; i < BM; i += NT) sas[i] = sa[min(m0 + i, M - 1)];
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s)
+  for (int s = 0; s < S; ++s)
     if (s < nk) {
-      srcB.issue(Bp + s * I8_BK, smem + s * STAGE);
-      srcA.issue(Ap + s * I8_BK, smem + s * STAGE + BN * I8_BK);
+      srcB.issue(Bp + s * BK, smem + s * STAGE);
+      srcA.issue(Ap + s * BK, smem + s * STAGE + BN * BK);
     }
   i32x16 acc[NI][MJ];
 #pragma unroll
@@ -82,32 +84,59 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_i8_kernel(const signed char
     for (int j = 0; j < MJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    if (S > 2 && kt + S - 2 < nk) wait_vmcnt<(S - 2) * LPT>();
+  // The fragments of a 32-byte step are read while the step before multiplies, behind its FIRST MFMA: while LDS DMA is on its way hipcc waits for every LDS
+  // read before it uses one (lgkmcnt(0)), so reads issued ahead of that MFMA would be waited for with an idle matrix unit.  In the last step of a stage all of
+  // its fragments are in registers, so that is where the workgroup meets: behind the barrier the stage's buffer takes the loads of the stage S ahead, and
+  // the first fragments of the next one are read under this step's MFMAs.
+  constexpr int KS = BK / 32;
+  static_assert(KS % 2 == 0, "two fragment sets, the first of a stage always in set 0");
+  i32x4 fb[2][NI], fa[2][MJ];
+  const unsigned char* lbase = smem + l31 * BK;
+  unsigned co[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) co[ks] = ((ks * 2 + half) ^ i8_swz<BK>(l31)) << 4;
+  auto frags = [&](i32x4(&b)[NI], i32x4(&a)[MJ], const unsigned char* buf, unsigned c) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) b[i] = *reinterpret_cast<const i32x4*>(buf + (wn * NI + i) * 32 * BK + c);
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) a[j] = *reinterpret_cast<const i32x4*>(buf + (BN + (wm * MJ + j) * 32) * BK + c);
+  };
+  auto arrive = [&](int more) {          // the oldest stage on its way has landed, `more` younger ones may still be out
+    if (more >= S - 1) wait_vmcnt<(S - 1) * LPT>();
+    else if (S > 2 && more == 1) wait_vmcnt<LPT>();
     else wait_vmcnt<0>();
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();          // tile kt is in LDS for every wave, and every wave is done with the buffer the next loads go to
+    __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (kt + S - 1 < nk) {
-      unsigned char* nb = smem + ((kt + S - 1) % S) * STAGE;
-      srcB.issue(Bp + (long)(kt + S - 1) * I8_BK, nb);
-      srcA.issue(Ap + (long)(kt + S - 1) * I8_BK, nb + BN * I8_BK);
-    }
-    const unsigned char* buf = smem + (kt % S) * STAGE + l31 * I8_BK;
+  };
+  static_assert(S == 2 || S == 3, "arrive()");
+  arrive(min(nk, S) - 1);
+  frags(fb[0], fa[0], lbase, co[0]);
+  int cur = 0;          // stage buffer
+  for (int kt = 0; kt < nk; ++kt) {
+    const int nxt = cur + 1 == S ? 0 : cur + 1;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const unsigned co = (((ks * 2 + half) ^ (l31 & 7)) << 4);
-      i32x4 fb[NI], fa[MJ];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) fb[i] = *reinterpret_cast<const i32x4*>(buf + (wn * NI + i) * 32 * I8_BK + co);
-#pragma unroll
-      for (int j = 0; j < MJ; ++j) fa[j] = *reinterpret_cast<const i32x4*>(buf + (BN + (wm * MJ + j) * 32) * I8_BK + co);
+    for (int ks = 0; ks < KS; ++ks) {
+      acc[0][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks & 1][0], fa[ks & 1][0], acc[0][0], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);          // (one MFMA is under way; nothing is out of LDS now, see below)
+      if (ks + 1 < KS) frags(fb[(ks + 1) & 1], fa[(ks + 1) & 1], lbase + cur * STAGE, co[ks + 1]);
+      else if (kt + 1 < nk) {
+        arrive(min(nk - kt - 2, S - 2));
+        if (kt + S < nk) {
+          srcB.issue(Bp + (long)(kt + S) * BK, smem + cur * STAGE);
+          srcA.issue(Ap + (long)(kt + S) * BK, smem + cur * STAGE + BN * BK);
+        }
+        frags(fb[0], fa[0], lbase + nxt * STAGE, co[0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[i], fa[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < MJ; ++j)
+          if (i || j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks & 1][i], fa[ks & 1][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
+    cur = nxt;
   }
   __syncthreads();          // the epilogue turns its blocks through the stage buffers
   // Epilogue: a wave turns 32 tokens x 32 NI channels at a time through a private LDS region, so that bias, residual and C are read and written as whole
@@ -152,7 +181,7 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_i8_kernel(const signed char
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[i] = fmaf((float)a[i], s * sbv[p % PERIOD][i], bv[p % PERIOD][i]);
-        if (EPI == EPI_GELU) v[i] = gelu_phi<GeluDeg<TO>::v>(v[i]);
+        if (EPI == EPI_GELU) v[i] = gelu_phi<TO>(v[i]);
         if (EPI == EPI_RESID) v[i] += rv[EPI == EPI_RESID ? p : 0][i];
       }
       i8_store4(C + (long)m * ldc + n, v, N - n, vec);
@@ -160,19 +189,19 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_i8_kernel(const signed char
   }
 }
 
-template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int S>
+template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
 static int i8_launch(const signed char* A, long lda, const float* sa, const signed char* B, long ldb, const float* sb, TO* C, long ldc, int M, int N, int Kp,
                      const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
-  constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * I8_BK + BM * 4;
-  static_assert(LDS <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * I8_BK, "LDS");
+  constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + BM * 4;
+  static_assert(LDS * OCC <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * BK, "LDS");
   const long tiles = (long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles >= (1L << 31)) return CLIMB_EUNSUPPORTED;
-  auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, S>;
+  auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, BK, S, OCC>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * WN * WM), LDS, st, A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp / I8_BK, bias, aux, ldaux, vec);
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * WN * WM), LDS, st, A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp / BK, bias, aux, ldaux, vec);
   LAUNCH_CHECK();
   return CLIMB_OK;
 }
@@ -180,10 +209,10 @@ template <typename TO, int EPI>
 static int i8_pick(const signed char* A, long lda, const float* sa, const signed char* B, long ldb, const float* sb, TO* C, long ldc, int M, int N, int Kp,
                    const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
   auto tiles = [&](int bm, int bn) { return (long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-#define I8_GO(NI_, MJ_, WN_, WM_, S_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, S_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
-  if (tiles(192, 192) >= 192) I8_GO(3, 3, 2, 2, 3);
-  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 3);
-  I8_GO(1, 1, 2, 2, 3);
+#define I8_GO(NI_, MJ_, WN_, WM_, BK_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, BK_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
+  if (Kp >= 1536 && tiles(192, 192) >= 192) I8_GO(3, 1, 2, 6, 128, 3, 1);
+  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 64, 3, 2);
+  I8_GO(1, 1, 2, 2, 128, 3, 3);
 #undef I8_GO
 }
 template <typename TO>
@@ -214,4 +243,101 @@ extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const 
   if (c_dtype == CLIMB_DT_F32) return i8_epi<float>(a, lda, sa, b, ldb, sb, (float*)C, ldc, M, N, Kp, bias, epi, aux, ldaux, vec, st);
   if (c_dtype == CLIMB_DT_BF16) return i8_epi<bf16_t>(a, lda, sa, b, ldb, sb, (bf16_t*)C, ldc, M, N, Kp, bias, epi, aux, ldaux, vec, st);
   return CLIMB_EINVAL;
+}
+
+// ------------------------------------------------------------------------------------------------ few tokens
+// y = epi(rows8(x) W^T + bias) for M <= 16 tokens in ONE launch: a workgroup owns 16 channels, quantises the tokens itself (its weights are already on their
+// way by then), its four waves share the reduction in 64-byte steps of v_mfma_i32_16x16x64_i8 and add their int32 sums through LDS.  Bound by latency: two
+// dependent trips to memory and the launch.
+#define FEW_M 16
+#define FEW_STEPS 12          // 64-byte steps of a wave: K <= 4 * 12 * 64
+template <typename T>
+__global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict__ x, long ldx, const signed char* __restrict__ W, long ldw, const float* __restrict__ sw,
+                                                            void* __restrict__ y, long ldy, int y_dtype, int M, int N, int K, int Kp, const float* __restrict__ bias,
+                                                            int epi, const float* aux, long ldaux) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // codes [16][Kp + 16], sums [4][16][17], scales [16]
+  const int pitch = Kp + 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, n0 = blockIdx.x * 16;
+  int* red = reinterpret_cast<int*>(smem + FEW_M * pitch);
+  float* sc = reinterpret_cast<float*>(red + 4 * 16 * 17);
+  const int steps = Kp / 64;
+  i32x4 wf[FEW_STEPS];
+  {
+    const signed char* wp = W + (long)min(n0 + l15, N - 1) * ldw + (lane >> 4) * 16;
+#pragma unroll
+    for (int i = 0; i < FEW_STEPS; ++i)
+      if (wave + 4 * i < steps) wf[i] = *reinterpret_cast<const i32x4*>(wp + (wave + 4 * i) * 64);
+  }
+  for (int r = wave; r < M; r += 4) {
+    const T* xr = x + (long)r * ldx;
+    unsigned mx = 0;
+    float v[4];
+#pragma unroll 3
+    for (int c = lane * 4; c < K; c += 256) {
+      row_ld<false, 4>(xr + c, K - c, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[j]));
+    }
+    mx = lanes_umax<64>(mx);
+    const float s = row_scale(mx), rs = 1.f / s;
+    if (lane == 0) sc[r] = s;
+#pragma unroll 3
+    for (int c = lane * 4; c < Kp; c += 256) {
+      row_ld<false, 4>(xr + c, K - c, v);
+      *reinterpret_cast<unsigned*>(smem + r * pitch + c) = rowq4(v, s, rs, mx >= 0x7f800000u);
+    }
+  }
+  __syncthreads();
+  i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < FEW_STEPS; ++i)
+    if (wave + 4 * i < steps) {          // (rows M .. 15 of the image are whatever LDS held: their columns of the result are not read)
+      const i32x4 tf = *reinterpret_cast<const i32x4*>(smem + l15 * pitch + (wave + 4 * i) * 64 + (lane >> 4) * 16);
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], tf, acc, 0, 0, 0);
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[(wave * 16 + (lane >> 4) * 4 + i) * 17 + l15] = acc[i];
+  __syncthreads();
+  const int m = threadIdx.x >> 4, n = n0 + l15;
+  if (m >= M || n >= N) return;
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) sum += red[(w * 16 + l15) * 17 + m];
+  float v = fmaf((float)sum, sc[m] * sw[n], bias ? bias[n] : 0.f);
+  if (epi == EPI_GELU) v = y_dtype == CLIMB_DT_F32 ? gelu_phi<float>(v) : gelu_phi<bf16_t>(v);
+  if (epi == EPI_RESID) v += aux[(long)m * ldaux + n];
+  if (y_dtype == CLIMB_DT_F32) static_cast<float*>(y)[(long)m * ldy + n] = v;
+  else static_cast<bf16_t*>(y)[(long)m * ldy + n] = f32_to_bf16(v);
+}
+static bool i8_few(int M, int K) { return M <= FEW_M && (K + I8_BK - 1) / I8_BK * I8_BK <= 4 * FEW_STEPS * 64; }
+
+extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);
+extern "C" long climb_linear_i8_workspace(int M, int K) {
+  if (M < 0 || K <= 0) return CLIMB_EINVAL;
+  return i8_few(M, K) ? 0 : (long)M * ((K + I8_BK - 1) / I8_BK * I8_BK + 4);
+}
+extern "C" int climb_linear_i8(const void* x, long ldx, int dtype, const void* W, long ldw, const float* sw, void* y, long ldy, int y_dtype, int M, int N, int K,
+                               const float* bias, int epi, const float* aux, long ldaux, void* workspace, long workspace_bytes, void* stream) {
+  if (M < 0 || N <= 0 || K <= 0 || K > (1 << 17) || ldx < K || (dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) || (y_dtype != CLIMB_DT_F32 && y_dtype != CLIMB_DT_BF16))
+    return K > (1 << 17) ? CLIMB_EUNSUPPORTED : CLIMB_EINVAL;
+  const int Kp = (K + I8_BK - 1) / I8_BK * I8_BK;
+  if (ldw < Kp || ldw % 16 || ((uintptr_t)W & 15) || ldy < N || (epi != EPI_NONE && epi != EPI_GELU && epi != EPI_RESID) || (epi == EPI_RESID && ldaux < N)) return CLIMB_EINVAL;
+  if (ldw >= (1L << 22)) return CLIMB_EUNSUPPORTED;
+  if (M == 0) return CLIMB_OK;
+  if (!x || !W || !sw || !y || (epi == EPI_RESID && !aux)) return CLIMB_EINVAL;
+  if (i8_few(M, K)) {
+    const int lds = FEW_M * (Kp + 16) + (4 * 16 * 17 + 16) * 4;
+    const dim3 grid((N + 15) / 16), blk(256);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == CLIMB_DT_F32)
+      hipLaunchKernelGGL((linear_i8_few_kernel<float>), grid, blk, lds, st, (const float*)x, ldx, (const signed char*)W, ldw, sw, y, ldy, y_dtype, M, N, K, Kp, bias, epi, aux, ldaux);
+    else
+      hipLaunchKernelGGL((linear_i8_few_kernel<bf16_t>), grid, blk, lds, st, (const bf16_t*)x, ldx, (const signed char*)W, ldw, sw, y, ldy, y_dtype, M, N, K, Kp, bias, epi, aux,
+                         ldaux);
+    LAUNCH_CHECK();
+    return CLIMB_OK;
+  }
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < climb_linear_i8_workspace(M, K)) return CLIMB_EINVAL;
+  float* s = reinterpret_cast<float*>((char*)workspace + (long)M * Kp);
+  const int rc = climb_rows8_quant(x, ldx, dtype, workspace, Kp, s, M, K, stream);
+  return rc != CLIMB_OK ? rc : climb_gemm_i8_nt(workspace, Kp, s, W, ldw, sw, y, ldy, y_dtype, M, N, K, bias, epi, aux, ldaux, stream);
 }

@@ -71,11 +71,26 @@ template <typename T> struct GeluDeg { static constexpr int v = 6; };
 template <> struct GeluDeg<float> { static constexpr int v = 8; };
 // gelu(x) = x Phi(x): x >= 0: x - x q, x < 0: x q, q = Phi(-|x|)  =  max(x, 0) - |x| q.  (q and exp(-x^2 / 2) are 0 beyond |x| = 14.4: the factor is held
 // at 64 there, so that an infinity gives its limit and not inf * 0)
-template <int DEG>
-__device__ __forceinline__ float gelu_phi(float x) {
+template <typename T> __device__ __forceinline__ float gelu_phi(float x);
+template <> __device__ __forceinline__ float gelu_phi<float>(float x) {
   float e2;
-  const float q = phi_lower<DEG>(x, e2);
+  const float q = phi_lower<8>(x, e2);
   return fmaf(-fminf(fabsf(x), 64.f), q, fmaxf(x, 0.f));
+}
+// For results stored in 16 bits: log2 Phi(-z) is close to a parabola, so one polynomial of degree 8 on [0, 10] (own fit, as above) and ONE exponential give q to
+// 2.6e-5 (relative; a 150th of bf16's half step, a 10th of half's): 11 full-rate operations and a transcendental, against 13 and two.  Beyond 10, where
+// x q is below 1e-22, z stays at 10.  minimum / maximum: the NaN of a NaN argument goes through.
+template <> __device__ __forceinline__ float gelu_phi<bf16_t>(float x) {
+  const float z = __builtin_elementwise_minimum(__builtin_fabsf(x), 10.f);
+  float p = fmaf(6.00354042e-08f, z, -3.12999009e-06f);
+  p = fmaf(p, z, 7.17434377e-05f);
+  p = fmaf(p, z, -0.000961354177f);
+  p = fmaf(p, z, 0.00850201212f);
+  p = fmaf(p, z, -0.0537272729f);
+  p = fmaf(p, z, -0.458911031f);
+  p = fmaf(p, z, -1.15098619f);
+  p = fmaf(p, z, -1.00002384f);
+  return fmaf(-z, __builtin_amdgcn_exp2f(p), __builtin_elementwise_maximum(x, 0.f));
 }
 // ... and gelu'(x) = Phi(x) + x exp(-x^2 / 2) / sqrt(2 pi)
 template <int DEG>
@@ -85,4 +100,87 @@ __device__ __forceinline__ float gelu_phi_pair(float x, float& d) {
   const float z = fminf(fabsf(x), 64.f);
   d = fmaf(copysignf(z, x) * 0.39894228040143267794f, e2, x < 0.f ? q : 1.0f - q);
   return fmaf(-z, q, fmaxf(x, 0.f));
+}
+
+// N consecutive elements of a row (N = 4 or 8), `left` = columns that exist from p on.  VEC: whole rows of 16-byte pieces (the launcher's condition).
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void row_ld(const T* __restrict__ p, int left, float (&v)[N]) {
+  if constexpr (VEC) {
+    if (left > 0) {
+      if constexpr (N == 8 && sizeof(T) == 2) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        v[0] = h16lo_to_f32(r.x); v[1] = h16hi_to_f32(r.x); v[2] = h16lo_to_f32(r.y); v[3] = h16hi_to_f32(r.y);
+        v[4] = h16lo_to_f32(r.z); v[5] = h16hi_to_f32(r.z); v[6] = h16lo_to_f32(r.w); v[7] = h16hi_to_f32(r.w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 r = ld4(p + i);
+          v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+  } else {
+    if (left >= N) {          // rows at any address: the hardware reads unaligned words, hipcc makes wide loads of the copy
+      T r[N];
+      __builtin_memcpy(r, p, sizeof(r));
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = Act<T>::ld(r + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = i < left ? Act<T>::ld(p + i) : 0.f;
+    }
+  }
+}
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void row_st(T* __restrict__ p, int left, const float (&v)[N]) {
+  if constexpr (VEC) {
+    if (left > 0) {
+      if constexpr (N == 8 && sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) st4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+      }
+    }
+  } else {
+    if (left >= N) {
+      T r[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) Act<T>::st(r + i, v[i]);
+      __builtin_memcpy(p, r, sizeof(r));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) Act<T>::st(p + i, v[i]);
+    }
+  }
+}
+// largest absolute value (as bits) over the W lanes that hold a group
+template <int W>
+__device__ __forceinline__ unsigned lanes_umax(unsigned m) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    const unsigned t = __shfl_xor(m, o, 64);
+    m = t > m ? t : m;
+  }
+  return m;
+}
+
+// true-quotient rounding: k = rint(x / s) from a reciprocal may miss a tie by its rounding; the remainder x - k s is exact in one fma and settles it
+__device__ __forceinline__ int rowq(float x, float s, float rs) {
+  const float k = rintf(x * rs), r = fmaf(-k, s, x), a = 2.f * fabsf(r);
+  int q = (int)k;
+  if (a > s || (a == s && (q & 1))) q += r > 0.f ? 1 : -1;
+  return q;
+}
+__device__ __forceinline__ float row_scale(unsigned mx) {
+  return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
+}
+__device__ __forceinline__ unsigned rowq4(const float (&v)[4], float s, float rs, bool bad) {
+  const unsigned w = ((unsigned)rowq(v[0], s, rs) & 255u) | (((unsigned)rowq(v[1], s, rs) & 255u) << 8) | (((unsigned)rowq(v[2], s, rs) & 255u) << 16) |
+                     (((unsigned)rowq(v[3], s, rs) & 255u) << 24);
+  return bad ? 0u : w;
 }

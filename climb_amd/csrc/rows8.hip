@@ -4,89 +4,7 @@
 
 static inline bool al(const void* p, long ld, int elems_per_16b) { return !((uintptr_t)p & 15) && ld % elems_per_16b == 0; }
 
-// N consecutive elements of a row (N = 4 or 8), `left` = columns that exist from p on.  VEC: whole rows of 16-byte pieces (the launcher's condition).
-template <bool VEC, int N, typename T>
-__device__ __forceinline__ void row_ld(const T* __restrict__ p, int left, float (&v)[N]) {
-  if constexpr (VEC) {
-    if (left > 0) {
-      if constexpr (N == 8 && sizeof(T) == 2) {
-        const uint4 r = *reinterpret_cast<const uint4*>(p);
-        v[0] = h16lo_to_f32(r.x); v[1] = h16hi_to_f32(r.x); v[2] = h16lo_to_f32(r.y); v[3] = h16hi_to_f32(r.y);
-        v[4] = h16lo_to_f32(r.z); v[5] = h16hi_to_f32(r.z); v[6] = h16lo_to_f32(r.w); v[7] = h16hi_to_f32(r.w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          const float4 r = ld4(p + i);
-          v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
-        }
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-  } else {
-    if (left >= N) {          // rows at any address: the hardware reads unaligned words, hipcc makes wide loads of the copy
-      T r[N];
-      __builtin_memcpy(r, p, sizeof(r));
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = Act<T>::ld(r + i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = i < left ? Act<T>::ld(p + i) : 0.f;
-    }
-  }
-}
-template <bool VEC, int N, typename T>
-__device__ __forceinline__ void row_st(T* __restrict__ p, int left, const float (&v)[N]) {
-  if constexpr (VEC) {
-    if (left > 0) {
-      if constexpr (N == 8 && sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) st4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-      }
-    }
-  } else {
-    if (left >= N) {
-      T r[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) Act<T>::st(r + i, v[i]);
-      __builtin_memcpy(p, r, sizeof(r));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < left) Act<T>::st(p + i, v[i]);
-    }
-  }
-}
-// largest absolute value (as bits) over the W lanes that hold a group
-template <int W>
-__device__ __forceinline__ unsigned lanes_umax(unsigned m) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    const unsigned t = __shfl_xor(m, o, 64);
-    m = t > m ? t : m;
-  }
-  return m;
-}
-
 // ------------------------------------------------------------------------------------------------ row codes
-// true-quotient rounding: k = rint(x / s) from a reciprocal may miss a tie by its rounding; the remainder x - k s is exact in one fma and settles it
-__device__ __forceinline__ int rowq(float x, float s, float rs) {
-  const float k = rintf(x * rs), r = fmaf(-k, s, x), a = 2.f * fabsf(r);
-  int q = (int)k;
-  if (a > s || (a == s && (q & 1))) q += r > 0.f ? 1 : -1;
-  return q;
-}
-__device__ __forceinline__ float row_scale(unsigned mx) {
-  return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
-}
-__device__ __forceinline__ unsigned rowq4(const float (&v)[4], float s, float rs, bool bad) {
-  const unsigned w = ((unsigned)rowq(v[0], s, rs) & 255u) | (((unsigned)rowq(v[1], s, rs) & 255u) << 8) | (((unsigned)rowq(v[2], s, rs) & 255u) << 16) |
-                     (((unsigned)rowq(v[3], s, rs) & 255u) << 24);
-  return bad ? 0u : w;
-}
 // One wave owns a row of C <= 256 NV and keeps it in registers; columns [C, Kp) of the code row are written as zeros (the product runs over whole
 // 128-byte pieces).
 template <typename T, bool VEC, int NV>
@@ -193,7 +111,7 @@ __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long
     if ((threadIdx.x & 7) == 0 && u < units) e[row * lde + g] = (unsigned char)ex;
     if constexpr (OP == 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = gelu_phi<DEG>(v[i]);
+      for (int i = 0; i < 8; ++i) o[i] = gelu_phi<T>(v[i]);
       row_st<VEC, 8>(y + row * ldy + c, left, o);
     }
   } else {
@@ -343,13 +261,13 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
 // dx = dres + rstd (g - mean_c(g) - xh mean_c(g xh)),  g = dy gamma,  xh = (codes - mean) rstd;  partial column sums {dgamma, dbeta, colsum(dx)} of the
 // workgroup's rows in part[workgroup][3][C], summed by climb_colreduce3 in a fixed order.
 #define A8LN_WAVES 8
-#define A8LN_RPW 3          // rows a wave
-#define A8LN_ROWS (A8LN_WAVES * A8LN_RPW)
+// rows a wave: three where that still leaves two workgroups a CU (12288 rows: 512), else one -- fewer partial rows against more waves on a short launch
+static inline int a8ln_rpw(int M) { return M >= 8192 ? 3 : 1; }
 template <typename T, bool VEC, int NV>
 __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* __restrict__ dy, long lddy, const signed char* __restrict__ q, long ldq,
                                                                       const unsigned char* __restrict__ e, long lde, const float* __restrict__ mean,
                                                                       const float* __restrict__ rstd, const float* __restrict__ gamma, const float* dres, long ldr,
-                                                                      float* dx, long ldo, T* __restrict__ dcast, long ldc, float* __restrict__ part, int M, int C) {
+                                                                      float* dx, long ldo, T* __restrict__ dcast, long ldc, float* __restrict__ part, int M, int C, int rpw) {
   __shared__ __attribute__((aligned(16))) float red[A8LN_WAVES][NV * 256];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   float ag[NV][4], ab[NV][4], as[NV][4], gm[NV][4];
@@ -360,8 +278,8 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
 #pragma unroll
     for (int j = 0; j < 4; ++j) ag[i][j] = ab[i][j] = as[i][j] = 0.f;
   }
-  for (int rr = 0; rr < A8LN_RPW; ++rr) {
-    const long row = (long)blockIdx.x * A8LN_ROWS + rr * A8LN_WAVES + wid;
+  for (int rr = 0; rr < rpw; ++rr) {
+    const long row = ((long)blockIdx.x * rpw + rr) * A8LN_WAVES + wid;
     if (row >= M) break;
     const float mu = mean[row], rs = rstd[row];
     float d[NV][4], rin[NV][4], xh[NV][4];
@@ -427,9 +345,10 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
 template <typename T, bool VEC>
 static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long ldq, const unsigned char* e, long lde, const float* mean, const float* rstd,
                               const float* gamma, const float* dres, long ldr, float* dx, long ldo, T* dcast, long ldc, float* part, int M, int C, hipStream_t st) {
-  const dim3 grid((M + A8LN_ROWS - 1) / A8LN_ROWS), blk(64 * A8LN_WAVES);
+  const int rpw = a8ln_rpw(M);
+  const dim3 grid((M + A8LN_WAVES * rpw - 1) / (A8LN_WAVES * rpw)), blk(64 * A8LN_WAVES);
 #define LB(NV_) \
-  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, VEC, NV_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C)
+  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, VEC, NV_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C, rpw)
   if (C <= 256) LB(1);
   else if (C <= 768) LB(3);
   else LB(6);
@@ -437,7 +356,7 @@ static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long
   LAUNCH_CHECK();
   return CLIMB_OK;
 }
-extern "C" int climb_act8_layernorm_bwd_rows_per_block(void) { return A8LN_ROWS; }
+extern "C" int climb_act8_layernorm_bwd_blocks(int M) { return M <= 0 ? 0 : (int)(((long)M + A8LN_WAVES * a8ln_rpw(M) - 1) / (A8LN_WAVES * a8ln_rpw(M))); }
 extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd,
                                         const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, int M, int C,
                                         void* stream) {

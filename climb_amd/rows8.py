@@ -14,7 +14,10 @@ pass keeps for its backward: half the bytes of a 16-bit activation, a quarter of
 Matrices are [..., C] in fp32 or the library's 16-bit type, on one HIP device, any row stride; an input whose last dimension is strided or whose rows overlap
 (a broadcast view) is copied first.  Work goes to the current stream of the inputs' device; nothing synchronises, and every scratch buffer is the call's
 own (torch's allocator), so the calls can be captured.  Forward and backward are explicit calls as in climb_amd.engine: inputs that require grad are
-refused while autograd records."""
+refused while autograd records.
+
+The host's share of a call is kept small (a launch alone is 3 us, and a batch of one sequence runs in less): one allocation per code matrix with its scales,
+contiguous inputs taken as they are, the stream read as a plain number."""
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union
@@ -25,18 +28,24 @@ from . import _lib
 
 GROUP = 64          # columns of a checkpoint that share a scale (climb_act8_group)
 _EPI = {"none": 0, "gelu": 1, "resid": 2}
+_F32 = torch.float32
 
 
 class RowCodes:
-    """int8 codes [rows, ld] (columns cols .. ld are zero) and one fp32 scale a row"""
-    __slots__ = ("q", "scale", "cols", "lead")
+    """int8 codes [rows, ld] (columns cols .. ld are zero) and one fp32 scale a row, in one buffer"""
+    __slots__ = ("buf", "rows", "cols", "ld", "lead", "device")
 
-    def __init__(self, q: torch.Tensor, scale: torch.Tensor, cols: int, lead: Tuple[int, ...]):
-        self.q, self.scale, self.cols, self.lead = q, scale, cols, lead
+    def __init__(self, rows: int, cols: int, lead: Tuple[int, ...], device: torch.device):
+        self.rows, self.cols, self.ld, self.lead, self.device = rows, cols, _up(cols, 128), lead, device
+        self.buf = torch.empty((rows * (self.ld + 4),), dtype=torch.int8, device=device)
 
     @property
-    def rows(self) -> int:
-        return self.q.shape[0]
+    def q(self) -> torch.Tensor:
+        return self.buf[:self.rows * self.ld].view(self.rows, self.ld)
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self.buf[self.rows * self.ld:].view(_F32)
 
     def dequantize(self) -> torch.Tensor:
         """the fp32 values the codes stand for"""
@@ -44,29 +53,48 @@ class RowCodes:
 
 
 class Checkpoint:
-    """int8 codes [rows, ld], a biased exponent byte for each row and 64 columns, and the dtype the activation had"""
-    __slots__ = ("q", "exps", "cols", "lead", "dtype", "mean", "rstd")
+    """int8 codes [rows, ld], an exponent byte for each row and 64 columns, LayerNorm's row statistics if layernorm_fwd made it, in one buffer, and the dtype the
+    activation had"""
+    __slots__ = ("buf", "rows", "cols", "ld", "groups", "lead", "dtype", "device", "_stats")
 
-    def __init__(self, rows: int, cols: int, lead: Tuple[int, ...], dtype: torch.dtype, device: torch.device):
-        self.q = torch.empty((rows, _up(cols, 16)), dtype=torch.int8, device=device)
-        self.exps = torch.empty((rows, _up(cols, GROUP) // GROUP), dtype=torch.uint8, device=device)
-        self.cols, self.lead, self.dtype = cols, lead, dtype
-        self.mean: Optional[torch.Tensor] = None          # LayerNorm's row statistics (layernorm_fwd)
-        self.rstd: Optional[torch.Tensor] = None
+    def __init__(self, rows: int, cols: int, lead: Tuple[int, ...], dtype: torch.dtype, device: torch.device, stats: bool = False):
+        self.rows, self.cols, self.ld, self.groups = rows, cols, _up(cols, 16), _up(-(-cols // GROUP), 4)          # (whole words: the weight gradient fetches four at a time)
+        self.lead, self.dtype, self.device = lead, dtype, device
+        n = rows * (self.ld + self.groups)
+        self._stats = _up(n, 16) if stats else 0          # byte offset of mean [rows], rstd [rows]
+        self.buf = torch.empty((self._stats + 8 * rows if stats else n,), dtype=torch.uint8, device=device)
 
     @property
-    def rows(self) -> int:
-        return self.q.shape[0]
+    def q(self) -> torch.Tensor:
+        return self.buf[:self.rows * self.ld].view(torch.int8).view(self.rows, self.ld)
+
+    @property
+    def exps(self) -> torch.Tensor:
+        n = self.rows * self.ld
+        return self.buf[n:n + self.rows * self.groups].view(self.rows, self.groups)[:, :-(-self.cols // GROUP)]
+
+    @property
+    def mean(self) -> Optional[torch.Tensor]:
+        return self.buf[self._stats:self._stats + 4 * self.rows].view(_F32) if self._stats else None
+
+    @property
+    def rstd(self) -> Optional[torch.Tensor]:
+        return self.buf[self._stats + 4 * self.rows:].view(_F32) if self._stats else None
 
     @property
     def nbytes(self) -> int:
-        return self.q.numel() + self.exps.numel()
+        return self.buf.numel()
+
+    def _args(self) -> Tuple[int, int, int, int]:
+        p = self.buf.data_ptr()
+        return p, self.ld, p + self.rows * self.ld, self.groups
 
     def load(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """the activation the codes stand for (default: in the dtype it was saved from)"""
         dtype = dtype or self.dtype
-        y = torch.empty((*self.lead, self.cols), dtype=dtype, device=self.q.device)
-        _launch(self.q.device, "climb_act8_load", self.q, self.q.shape[1], self.exps, self.exps.shape[1], y, self.cols, _code(dtype), self.rows, self.cols)
+        code = _code(dtype)
+        y = torch.empty((*self.lead, self.cols), dtype=dtype, device=self.device)
+        _launch(self.device, "climb_act8_load", *self._args(), y.data_ptr(), self.cols, code, self.rows, self.cols)
         return y
 
 
@@ -74,126 +102,171 @@ def _up(x: int, m: int) -> int:
     return -(-x // m) * m
 
 
+_h16 = None
+
+
+def _h16_type() -> torch.dtype:
+    global _h16
+    if _h16 is None:
+        _h16 = _lib.torch_h16()
+    return _h16
+
+
 def _code(dtype: torch.dtype) -> int:
-    if dtype is torch.float32:
+    if dtype is _F32:
         return 0
-    if dtype is _lib.torch_h16():
+    if dtype is _h16_type():
         return 1
-    raise TypeError(f"rows8: {dtype} is not a type of this library build (torch.float32 or {_lib.torch_h16()})")
+    raise TypeError(f"rows8: {dtype} is not a type of this library build (torch.float32 or {_h16})")
+
+
+_fns = {}
 
 
 def _launch(dev: torch.device, name: str, *args):
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    """the launcher on the current stream of `dev` (also where another device is the current one); arguments are plain numbers"""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = _lib.bound(name)
+    i = dev.index
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))          # (what torch.cuda.current_stream(dev).cuda_stream holds, without the object: 0.1 against 1.9 us)
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != 0:
+        _lib.check(name, rc)
+
+
+def _query(name: str, *args) -> int:
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = _lib.bound(name)
+    return fn(*args)
 
 
 def _mat(x: torch.Tensor, what: str, cols: Optional[int] = None, rows: Optional[int] = None, dtype: Optional[torch.dtype] = None,
-         dev: Optional[torch.device] = None) -> torch.Tensor:
-    """x as [rows, cols] with unit column stride and rows that do not overlap"""
+         dev: Optional[torch.device] = None) -> Tuple[torch.Tensor, int, int, int]:
+    """(x, rows, cols, row stride) of x as a matrix with unit column stride and rows that do not overlap"""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"rows8: {what} must be a tensor")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"rows8: {what} requires grad, and these calls record nothing for autograd: detach it (forward and backward are explicit calls)")
     if not x.is_cuda or (dev is not None and x.device != dev):
         raise ValueError(f"rows8: {what} is on {x.device}; every tensor of a call must be on one HIP device")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"rows8: {what} has shape {tuple(x.shape)}; a last dimension of at least 1 is needed")
-    if cols is not None and x.shape[-1] != cols:
-        raise ValueError(f"rows8: {what} has {x.shape[-1]} columns, {cols} expected")
+    shape = x.shape
+    C = shape[-1] if shape else 0
+    if C == 0:
+        raise ValueError(f"rows8: {what} has shape {tuple(shape)}; a last dimension of at least 1 is needed")
+    if cols is not None and C != cols:
+        raise ValueError(f"rows8: {what} has {C} columns, {cols} expected")
     if dtype is not None and x.dtype is not dtype:
         raise TypeError(f"rows8: {what} is {x.dtype}, {dtype} expected")
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    if rows is not None and x.shape[0] != rows:
-        raise ValueError(f"rows8: {what} has {x.shape[0]} rows, {rows} expected")
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    return x
+    if x.is_contiguous():
+        M, ld = x.numel() // C, C
+    else:
+        if len(shape) != 2:
+            x = x.reshape(-1, C)
+        M = x.shape[0]
+        if (C > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < C):
+            x = x.contiguous()
+        ld = x.stride(0) if M > 1 else C
+    if rows is not None and M != rows:
+        raise ValueError(f"rows8: {what} has {M} rows, {rows} expected")
+    return x, M, C, ld
 
 
-def _ld(x: torch.Tensor) -> int:
-    return max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
+def _vec(x: torch.Tensor, what: str, n: int, dev: torch.device) -> torch.Tensor:
+    x, M, C, ld = _mat(x, what, dtype=_F32, dev=dev)
+    if M * C != n:
+        raise ValueError(f"rows8: {what} has {M * C} elements, {n} expected")
+    return x if M == 1 or ld == C else x.contiguous()
 
 
-def _vec(x: Optional[torch.Tensor], what: str, n: int, dev: torch.device) -> Optional[torch.Tensor]:
-    if x is None:
-        return None
-    return _mat(x.reshape(1, -1) if isinstance(x, torch.Tensor) else x, what, cols=n, rows=1, dtype=torch.float32, dev=dev)
-
-
-def _target(x: torch.Tensor, what: str, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
-    """a tensor that the call writes: never copied"""
-    if not isinstance(x, torch.Tensor) or tuple(x.shape) != shape or x.dtype is not dtype or x.device != dev:
-        raise ValueError(f"rows8: {what} must be a {dtype} tensor of shape {shape} on {dev}")
+def _target(x: torch.Tensor, what: str, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> int:
+    """row stride of a tensor that the call writes: never copied"""
+    if not isinstance(x, torch.Tensor) or tuple(x.shape) != tuple(shape) or x.dtype is not dtype or x.device != dev:
+        raise ValueError(f"rows8: {what} must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"rows8: {what} requires grad and would be written in place")
-    if (x.shape[-1] > 1 and x.stride(-1) != 1) or (x.dim() == 2 and x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        raise ValueError(f"rows8: {what} needs unit column stride and rows that do not overlap")
-    return x
+    if x.is_contiguous():
+        return shape[-1]
+    if x.dim() != 2 or (shape[1] > 1 and x.stride(1) != 1) or (shape[0] > 1 and x.stride(0) < shape[1]):
+        raise ValueError(f"rows8: {what} needs unit column stride and rows that do not overlap (more than two dimensions: contiguous)")
+    return x.stride(0) if shape[0] > 1 else shape[1]
 
 
 # ------------------------------------------------------------------------------------------------ int8 linear layer
 def quantize_rows(x: torch.Tensor) -> RowCodes:
     """Row codes of x: the tokens of an activation, or the output channels of a weight [N, K]."""
-    m = _mat(x, "x")
-    M, C = m.shape
+    m, M, C, ld = _mat(x, "x")
     code = _code(m.dtype)
-    q = torch.empty((M, _up(C, 128)), dtype=torch.int8, device=m.device)
-    s = torch.empty((M,), dtype=torch.float32, device=m.device)
-    _launch(m.device, "climb_rows8_quant", m, _ld(m), code, q, q.shape[1], s, M, C)
-    return RowCodes(q, s, C, tuple(x.shape[:-1]))
+    r = RowCodes(M, C, tuple(x.shape[:-1]), m.device)
+    p = r.buf.data_ptr()
+    _launch(m.device, "climb_rows8_quant", m.data_ptr(), ld, code, p, r.ld, p + M * r.ld, M, C)
+    return r
 
 
 def linear_i8(x: Union[torch.Tensor, RowCodes], w: RowCodes, bias: Optional[torch.Tensor] = None, epi: str = "none", resid: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = epi(x8 w8^T + bias): x quantised by token here (or handed over as RowCodes, which several products can share), w by output channel.
     epi: "none", "gelu" (erf form) or "resid" (+ resid, fp32; `out` may be `resid` itself).  The products' sum is exact, the rest is fp32, y is rounded once
-    to out_dtype (default: x's)."""
-    if epi not in _EPI:
+    to out_dtype (default: x's; fp32 for RowCodes).  `out` must not overlap x, w or bias."""
+    e = _EPI.get(epi)
+    if e is None:
         raise ValueError(f"rows8: unknown epilogue {epi!r} (one of {sorted(_EPI)})")
-    if (resid is not None) != (epi == "resid"):
+    if (resid is not None) != (e == 2):
         raise ValueError('rows8: `resid` goes with epi="resid"')
     if not isinstance(w, RowCodes):
         raise TypeError("rows8: w must be RowCodes (quantize_rows(weight))")
-    dev, N, K = w.q.device, w.rows, w.cols
-    if isinstance(x, RowCodes):
-        if x.q.device != dev:
-            raise ValueError(f"rows8: x is on {x.q.device}, w on {dev}")
-        if x.cols != K:
-            raise ValueError(f"rows8: x has {x.cols} columns, {K} expected")
-        xq, lead, dt = x, x.lead, torch.float32
-    else:
-        _mat(x, "x", cols=K, dev=dev)
-        xq, lead, dt = quantize_rows(x), tuple(x.shape[:-1]), x.dtype
+    dev, N, K = w.device, w.rows, w.cols
     if N == 0:
         raise ValueError("rows8: w has no rows")
-    M = xq.rows
-    if out is not None:
-        y = _target(out, "out", (*lead, N), out_dtype or out.dtype, dev)
-        if y.dim() != 2 and not y.is_contiguous():
-            raise ValueError("rows8: out with more than two dimensions must be contiguous")
-        y2 = y.view(-1, N) if y.dim() != 2 else y
+    codes = isinstance(x, RowCodes)
+    if codes:
+        if x.device != dev:
+            raise ValueError(f"rows8: x is on {x.device}, w on {dev}")
+        if x.cols != K:
+            raise ValueError(f"rows8: x has {x.cols} columns, {K} expected")
+        M, lead, dt = x.rows, x.lead, _F32
     else:
-        y = torch.empty((*lead, N), dtype=out_dtype or dt, device=dev)
-        y2 = y.view(M, N)
-    code = _code(y.dtype)
-    b = _vec(bias, "bias", N, dev)
-    r = _mat(resid, "resid", cols=N, rows=M, dtype=torch.float32, dev=dev) if resid is not None else None
-    _launch(dev, "climb_gemm_i8_nt", xq.q, xq.q.shape[1], xq.scale, w.q, w.q.shape[1], w.scale, y2, _ld(y2), code, M, N, K, b, _EPI[epi], r, _ld(r) if r is not None else 0)
+        m, M, _, ldx = _mat(x, "x", cols=K, dev=dev)
+        lead, dt = x.shape[:-1], m.dtype
+        xcode = _code(dt)
+    if out is None:
+        dt = out_dtype or dt
+        ycode = _code(dt)
+        y, ldy = torch.empty((*lead, N), dtype=dt, device=dev), N
+    else:
+        y, dt = out, out_dtype or out.dtype
+        ycode, ldy = _code(dt), _target(out, "out", (*lead, N), dt, dev)
+    b = 0
+    if bias is not None:
+        bias = _vec(bias, "bias", N, dev)
+        b = bias.data_ptr()
+    r = ldr = 0
+    if resid is not None:
+        resid, _, _, ldr = _mat(resid, "resid", cols=N, rows=M, dtype=_F32, dev=dev)
+        r = resid.data_ptr()
+    wp = w.buf.data_ptr()
+    if codes:
+        xp = x.buf.data_ptr()
+        _launch(dev, "climb_gemm_i8_nt", xp, x.ld, xp + M * x.ld, wp, w.ld, wp + N * w.ld, y.data_ptr(), ldy, ycode, M, N, K, b, e, r, ldr)
+    else:
+        nb = _query("climb_linear_i8_workspace", M, K)
+        ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb > 0 else None
+        _launch(dev, "climb_linear_i8", m.data_ptr(), ldx, xcode, wp, w.ld, wp + N * w.ld, y.data_ptr(), ldy, ycode, M, N, K, b, e, r, ldr,
+                ws.data_ptr() if nb > 0 else 0, nb)
     return y
 
 
 # ------------------------------------------------------------------------------------------------ checkpoints
 def checkpoint_save(x: torch.Tensor) -> Checkpoint:
     """Keep x in 8 bits."""
-    m = _mat(x, "x")
-    M, C = m.shape
+    m, M, C, ld = _mat(x, "x")
     code = _code(m.dtype)
     ck = Checkpoint(M, C, tuple(x.shape[:-1]), m.dtype, m.device)
-    _launch(m.device, "climb_act8_save", m, _ld(m), code, ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], M, C)
+    _launch(m.device, "climb_act8_save", m.data_ptr(), ld, code, *ck._args(), M, C)
     return ck
 
 
@@ -201,82 +274,94 @@ def weight_grad(dy: torch.Tensor, ck: Checkpoint, dw: Optional[torch.Tensor] = N
                 bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw [N, K], dbias [N]) of y = x w^T + b from dy (16 bit) and the checkpoint of x.  Given `dw` / `dbias` are added to (fp32, in place); `bias` False:
     no bias gradient."""
-    dev, K = ck.q.device, ck.cols
-    d = _mat(dy, "dy", rows=ck.rows, dtype=_lib.torch_h16(), dev=dev)
-    M, N = d.shape
+    dev, K = ck.device, ck.cols
+    d, M, N, ld = _mat(dy, "dy", rows=ck.rows, dtype=_h16_type(), dev=dev)
     if dbias is not None and not bias:
         raise ValueError("rows8: dbias given, bias=False")
     beta = 0.0 if dw is None and dbias is None else 1.0
     new = torch.empty if beta == 0.0 else torch.zeros
-    dw = new((N, K), dtype=torch.float32, device=dev) if dw is None else _target(dw, "dw", (N, K), torch.float32, dev)
-    if bias:
-        dbias = new((N,), dtype=torch.float32, device=dev) if dbias is None else _target(dbias, "dbias", (N,), torch.float32, dev)
-    nb = _lib.query_arg("climb_act8_weight_grad_workspace", M, N, K)
+    if dw is None:
+        dw, ldw = new((N, K), dtype=_F32, device=dev), K
+    else:
+        ldw = _target(dw, "dw", (N, K), _F32, dev)
+    if dbias is not None:
+        _target(dbias, "dbias", (N,), _F32, dev)
+    elif bias:
+        dbias = new((N,), dtype=_F32, device=dev)
+    nb = _query("climb_act8_weight_grad_workspace", M, N, K)
     ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb > 0 else None
-    _launch(dev, "climb_act8_weight_grad", d, _ld(d), ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], dw, _ld(dw), dbias, M, N, K, beta, ws, max(nb, 0))
+    _launch(dev, "climb_act8_weight_grad", d.data_ptr(), ld, *ck._args(), dw.data_ptr(), ldw, dbias.data_ptr() if dbias is not None else 0, M, N, K, beta,
+            ws.data_ptr() if nb > 0 else 0, nb)
     return dw, dbias
 
 
 def layernorm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float, out_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, Checkpoint]:
     """y = LayerNorm(x) (x fp32, at most 1536 columns; y in out_dtype, default fp32) and the checkpoint of x with its row statistics."""
-    m = _mat(x, "x", dtype=torch.float32)
-    M, C = m.shape
+    m, M, C, ld = _mat(x, "x", dtype=_F32)
     if C > 1536:
         raise ValueError(f"rows8: LayerNorm of {C} columns; this build holds rows of at most 1536 in registers")
-    dev = m.device
-    y = torch.empty(x.shape, dtype=out_dtype or torch.float32, device=dev)
-    code = _code(y.dtype)
+    dev, dt = m.device, out_dtype or _F32
+    code = _code(dt)
     g, b = _vec(gamma, "gamma", C, dev), _vec(beta, "beta", C, dev)
-    ck = Checkpoint(M, C, tuple(x.shape[:-1]), torch.float32, dev)
-    st = torch.empty((2, M), dtype=torch.float32, device=dev)
-    ck.mean, ck.rstd = st[0], st[1]
-    _launch(dev, "climb_act8_layernorm_fwd", m, _ld(m), g, b, float(eps), y, C, code, ck.mean, ck.rstd, ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], M, C)
+    y = torch.empty(x.shape, dtype=dt, device=dev)
+    ck = Checkpoint(M, C, tuple(x.shape[:-1]), _F32, dev, stats=True)
+    q, ldq, e, lde = ck._args()
+    st = q + ck._stats
+    _launch(dev, "climb_act8_layernorm_fwd", m.data_ptr(), ld, g.data_ptr(), b.data_ptr(), eps, y.data_ptr(), C, code, st, st + 4 * M, q, ldq, e, lde, M, C)
     return y, ck
 
 
 def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: Optional[torch.Tensor] = None, dgamma: Optional[torch.Tensor] = None,
                   dbeta: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dgamma, dbeta), dx = dres + d(LayerNorm)/dx^T dy in fp32; given `dgamma` / `dbeta` are added to."""
-    if ck.mean is None:
+    if not ck._stats:
         raise ValueError("rows8: this checkpoint holds no row statistics (layernorm_fwd makes one that does)")
-    dev, M, C = ck.q.device, ck.rows, ck.cols
-    d = _mat(dy, "dy", cols=C, rows=M, dev=dev)
+    dev, M, C = ck.device, ck.rows, ck.cols
+    d, _, _, ld = _mat(dy, "dy", cols=C, rows=M, dev=dev)
     code = _code(d.dtype)
     g = _vec(gamma, "gamma", C, dev)
-    r = _mat(dres, "dres", cols=C, rows=M, dtype=torch.float32, dev=dev) if dres is not None else None
+    r = ldr = 0
+    if dres is not None:
+        dres, _, _, ldr = _mat(dres, "dres", cols=C, rows=M, dtype=_F32, dev=dev)
+        r = dres.data_ptr()
     acc = dgamma is not None or dbeta is not None
     new = torch.zeros if acc or M == 0 else torch.empty
-    dgamma = new((C,), dtype=torch.float32, device=dev) if dgamma is None else _target(dgamma, "dgamma", (C,), torch.float32, dev)
-    dbeta = new((C,), dtype=torch.float32, device=dev) if dbeta is None else _target(dbeta, "dbeta", (C,), torch.float32, dev)
-    dx = torch.empty((*ck.lead, C), dtype=torch.float32, device=dev)
+    if dgamma is None:
+        dgamma = new((C,), dtype=_F32, device=dev)
+    else:
+        _target(dgamma, "dgamma", (C,), _F32, dev)
+    if dbeta is None:
+        dbeta = new((C,), dtype=_F32, device=dev)
+    else:
+        _target(dbeta, "dbeta", (C,), _F32, dev)
+    dx = torch.empty((*ck.lead, C), dtype=_F32, device=dev)
     if M == 0:
         return dx, dgamma, dbeta
-    rpb = _lib.query("climb_act8_layernorm_bwd_rows_per_block")
-    nblk = -(-M // rpb)
-    part = torch.empty((nblk, 3, C), dtype=torch.float32, device=dev)
-    _launch(dev, "climb_act8_layernorm_bwd", d, _ld(d), code, ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], ck.mean, ck.rstd, g, r, _ld(r) if r is not None else 0,
-            dx, C, None, 0, part, M, C)
-    _launch(dev, "climb_colreduce3", part, 3 * C, nblk, dgamma, dbeta, None, C, 1.0 if acc else 0.0)
+    nblk = _query("climb_act8_layernorm_bwd_blocks", M)
+    part = torch.empty((nblk * 3 * C,), dtype=_F32, device=dev)
+    q, ldq, e, lde = ck._args()
+    st = q + ck._stats
+    _launch(dev, "climb_act8_layernorm_bwd", d.data_ptr(), ld, code, q, ldq, e, lde, st, st + 4 * M, g.data_ptr(), r, ldr, dx.data_ptr(), C, 0, 0, part.data_ptr(), M, C)
+    _launch(dev, "climb_colreduce3", part.data_ptr(), 3 * C, nblk, dgamma.data_ptr(), dbeta.data_ptr(), 0, C, 1.0 if acc else 0.0)
     return dx, dgamma, dbeta
 
 
 def gelu_fwd(u: torch.Tensor) -> Tuple[torch.Tensor, Checkpoint]:
     """a = gelu(u) (erf form) in u's dtype, and the checkpoint of u."""
-    m = _mat(u, "u")
-    M, C = m.shape
+    m, M, C, ld = _mat(u, "u")
     code = _code(m.dtype)
     a = torch.empty(u.shape, dtype=m.dtype, device=m.device)
     ck = Checkpoint(M, C, tuple(u.shape[:-1]), m.dtype, m.device)
-    _launch(m.device, "climb_act8_gelu_fwd", m, _ld(m), code, a, C, ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], M, C)
+    _launch(m.device, "climb_act8_gelu_fwd", m.data_ptr(), ld, code, a.data_ptr(), C, *ck._args(), M, C)
     return a, ck
 
 
 def gelu_bwd(da: torch.Tensor, ck: Checkpoint, recompute: bool = False):
     """du = da gelu'(u) in da's dtype; recompute: (du, gelu(u)) -- the activation itself, which the next layer's weight gradient reads, is not kept."""
-    dev, M, C = ck.q.device, ck.rows, ck.cols
-    d = _mat(da, "da", cols=C, rows=M, dev=dev)
+    dev, M, C = ck.device, ck.rows, ck.cols
+    d, _, _, ld = _mat(da, "da", cols=C, rows=M, dev=dev)
     code = _code(d.dtype)
     du = torch.empty((*ck.lead, C), dtype=d.dtype, device=dev)
     a = torch.empty_like(du) if recompute else None
-    _launch(dev, "climb_act8_gelu_bwd", d, _ld(d), code, ck.q, ck.q.shape[1], ck.exps, ck.exps.shape[1], du, C, a, C, M, C)
+    _launch(dev, "climb_act8_gelu_bwd", d.data_ptr(), ld, code, *ck._args(), du.data_ptr(), C, a.data_ptr() if recompute else 0, C, M, C)
     return (du, a) if recompute else du

@@ -266,15 +266,20 @@ int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, flo
 /* C[m,n] (c_dtype) = epi(sum_k A[m,k] B[n,k] sa[m] sb[n] + bias[n]); A / B row codes of the tokens and of the weight's rows (one scale an output channel), the
  * sum exact in int32 (K <= 2^17).  epi: 0 none, 1 GELU (erf form; no aux_out), 2 + aux (fp32 [M,N], may be C).  bias may be NULL. */
 int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const void* B, long ldb, const float* sb, void* C, long ldc, int c_dtype, int M, int N, int K, const float* bias, int epi, const float* aux, long ldaux, void* stream);
+/* the same from tokens that are not quantised yet: y[m,n] (y_dtype) = epi(row codes of x (dtype) times W ...).  One launch for few tokens, else climb_rows8_quant
+ * into `workspace` (16-byte aligned, at least climb_linear_i8_workspace(M, K) bytes, 0: none needed; scratch of this call alone) and climb_gemm_i8_nt; the
+ * results are the same bits either way */
+long climb_linear_i8_workspace(int M, int K);
+int climb_linear_i8(const void* x, long ldx, int dtype, const void* W, long ldw, const float* sw, void* y, long ldy, int y_dtype, int M, int N, int K, const float* bias, int epi, const float* aux, long ldaux, void* workspace, long workspace_bytes, void* stream);
 /* checkpoints: write one, read one back (dtype 0 / 1).  climb_act8_group() = 64, the columns that share a scale */
 int climb_act8_group(void);
 int climb_act8_save(const void* x, long ldx, int dtype, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
 int climb_act8_load(const void* q, long ldq, const void* e, long lde, void* y, long ldy, int dtype, int M, int C, void* stream);
 /* climb_layernorm_fwd that also keeps its input as a checkpoint (C <= 1536), and climb_layernorm_bwd's contract with the checkpoint in place of x: dtype = that of dy
- * and dcast; dx fp32 (may be dres_in); part[ceil(M / R)][3][C] = { dgamma, dbeta, colsum(dx) } partials, R = climb_act8_layernorm_bwd_rows_per_block(),
- * reduced by climb_colreduce3 */
+ * and dcast; dx fp32 (may be dres_in); part[climb_act8_layernorm_bwd_blocks(M)][3][C] = { dgamma, dbeta, colsum(dx) } partials, reduced by
+ * climb_colreduce3 */
 int climb_act8_layernorm_fwd(const float* x, long ldx, const float* gamma, const float* beta, float eps, void* y, long ldy, int y_dtype, float* mean, float* rstd, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
-int climb_act8_layernorm_bwd_rows_per_block(void);
+int climb_act8_layernorm_bwd_blocks(int M);
 int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd, const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, int M, int C, void* stream);
 /* a = gelu(u) (erf form) and the checkpoint of u; du = da gelu'(checkpoint) and, if a != NULL, a = gelu(checkpoint) (the operand of the next layer's weight
  * gradient).  dtype = that of every matrix */

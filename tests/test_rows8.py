@@ -41,6 +41,22 @@ def test_int8_product_refuses(mem, change, rc):
     aux = p if a["aux"] else None
     assert _rc("climb_gemm_i8_nt", A, a["lda"], a["sa"], a["B"], a["ldb"], a["sb"], a["C"], a["ldc"], a["c_dtype"], a["M"], a["N"], a["K"], None, a["epi"], aux, a["ldaux"],
                None) == rc
+    # ... and so does the call that quantises its tokens (A as a 16-bit matrix), with few tokens and with many
+    if "lda" in change and "K" not in change or "aoff" in change or "sa" in change:
+        return
+    for M in (a["M"], a["M"] * 100):
+        assert _rc("climb_linear_i8", A, max(a["K"], 1), 1, a["B"], a["ldb"], a["sb"], a["C"], a["ldc"], a["c_dtype"], M, a["N"], a["K"], None, a["epi"], aux, a["ldaux"], p, 1 << 30,
+                   None) == rc
+
+
+def test_linear_asks_for_its_workspace(mem):
+    p = mem[0]
+    assert _rc("climb_linear_i8_workspace", 1, 768) == 0 and _rc("climb_linear_i8_workspace", 64, 100) == 64 * 132 and _rc("climb_linear_i8_workspace", -1, 8) == EINVAL
+    need = 64 * 132
+    for ws, nb in ((None, need), (p + 4, need), (p, need - 1)):
+        assert _rc("climb_linear_i8", p, 100, 0, p, 128, p, p, 32, 0, 64, 32, 100, None, 0, None, 0, ws, nb, None) == EINVAL
+    for dtype, ldx in ((2, 100), (0, 99)):
+        assert _rc("climb_linear_i8", p, ldx, dtype, p, 128, p, p, 32, 0, 64, 32, 100, None, 0, None, 0, p, need, None) == EINVAL
 
 
 @pytest.mark.parametrize("change", [dict(M=-1), dict(C=0), dict(ldq=96), dict(ldq=104), dict(lde=1), dict(dtype=2), dict(x=None), dict(q=None), dict(e=None), dict(ldx=99)])
@@ -100,7 +116,8 @@ def test_tensor_calls_refuse():
         rows8.checkpoint_save([1.0])
     with pytest.raises(RuntimeError, match="autograd"):
         rows8.gelu_fwd(torch.zeros(4, 8, requires_grad=True))
-    w = rows8.RowCodes(torch.zeros(3, 128, dtype=torch.int8), torch.ones(3), 8, (3,))
+    w = rows8.RowCodes(3, 8, (3,), torch.device("cpu"))
+    assert w.q.shape == (3, 128) and w.scale.shape == (3,)
     with pytest.raises(ValueError, match="epilogue"):
         rows8.linear_i8(x, w, epi="tanh")
     with pytest.raises(ValueError, match="resid"):
@@ -110,4 +127,7 @@ def test_tensor_calls_refuse():
     ck = rows8.Checkpoint(4, 8, (4,), torch.float32, torch.device("cpu"))
     with pytest.raises(ValueError, match="row statistics"):
         rows8.layernorm_bwd(x, ck, torch.ones(8))
-    assert ck.nbytes == 4 * 16 + 4 and rows8.GROUP == _lib.query("climb_act8_group")
+    assert ck.nbytes == 4 * 16 + 4 * 4 and ck.q.shape == (4, 16) and ck.exps.shape == (4, 1) and ck.mean is None
+    ck = rows8.Checkpoint(3, 70, (3,), torch.float32, torch.device("cpu"), stats=True)
+    assert ck.nbytes == 3 * 84 + 4 + 24 and ck.mean.shape == ck.rstd.shape == (3,)
+    assert rows8.GROUP == _lib.query("climb_act8_group")
