@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
 // The same sum on 256 (n) x 256 (k) tiles, one workgroup of 8 waves a CU (4 x 2 waves of 64 x 128): a code is expanded once for 256 channels (the 128-tile
 // kernel is bound by that VALU work).  Everything comes to LDS by DMA: a ring of 5 stages { gradients [32 tokens][256] , codes [32][256], exponents }, and two
 // images of expanded codes.  The step that multiplies token tile t (two groups of 8 MFMAs)
-//   - expands the codes of tile t + 1 between the MFMAs of its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
+//   - expands the codes of tile t + 1 in its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
 //   - meets the workgroup in the second group; behind the barrier the ring slot of tile t takes the DMA of tile t + 5, and the first fragments of tile t + 1
 //     are read under the rest of the group.
 // As in gemm_i8.hip fragments are read behind the first MFMA of the group before, and no load goes to registers: hipcc would wait for all DMA with it.
@@ -365,13 +365,6 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (i || j) acc[i][j] = CLIMB_MFMA_H16(fa[ms][i], fb[ms][j], acc[i][j], 0, 0, 0);
-      if (ms == 0) {          // the expansion's ~50 VALU operations between the 7 MFMAs
-#pragma unroll
-        for (int i = 0; i < 7; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);
-        }
-      }
       __builtin_amdgcn_sched_barrier(0);
       if (bias_tile) {          // (a fragment holds 8 tokens of one channel; the tiles are dealt to the workgroups that share the channels)
 #pragma unroll

@@ -251,7 +251,7 @@ extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const 
 // dependent trips to memory and the launch.
 #define FEW_M 16
 #define FEW_STEPS 12          // 64-byte steps of a wave: K <= 4 * 12 * 64
-template <typename T>
+template <typename T, int MODE>
 __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict__ x, long ldx, const signed char* __restrict__ W, long ldw, const float* __restrict__ sw,
                                                             void* __restrict__ y, long ldy, int y_dtype, int M, int N, int K, int Kp, const float* __restrict__ bias,
                                                             int epi, const float* aux, long ldaux) {
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
     float v[4];
 #pragma unroll 3
     for (int c = lane * 4; c < K; c += 256) {
-      row_ld<false, 4>(xr + c, K - c, v);
+      row_ld<MODE, 4>(xr, c, K, v);
 #pragma unroll
       for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[j]));
     }
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
     if (lane == 0) sc[r] = s;
 #pragma unroll 3
     for (int c = lane * 4; c < Kp; c += 256) {
-      row_ld<false, 4>(xr + c, K - c, v);
+      row_ld<MODE, 4>(xr, c, K, v);
       *reinterpret_cast<unsigned*>(smem + r * pitch + c) = rowq4(v, s, rs, mx >= 0x7f800000u);
     }
   }
@@ -328,11 +328,11 @@ extern "C" int climb_linear_i8(const void* x, long ldx, int dtype, const void* W
     const int lds = FEW_M * (Kp + 16) + (4 * 16 * 17 + 16) * 4;
     const dim3 grid((N + 15) / 16), blk(256);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == CLIMB_DT_F32)
-      hipLaunchKernelGGL((linear_i8_few_kernel<float>), grid, blk, lds, st, (const float*)x, ldx, (const signed char*)W, ldw, sw, y, ldy, y_dtype, M, N, K, Kp, bias, epi, aux, ldaux);
-    else
-      hipLaunchKernelGGL((linear_i8_few_kernel<bf16_t>), grid, blk, lds, st, (const bf16_t*)x, ldx, (const signed char*)W, ldw, sw, y, ldy, y_dtype, M, N, K, Kp, bias, epi, aux,
-                         ldaux);
+#define FEW(T_, MODE_) \
+  hipLaunchKernelGGL((linear_i8_few_kernel<T_, MODE_>), grid, blk, lds, st, (const T_*)x, ldx, (const signed char*)W, ldw, sw, y, ldy, y_dtype, M, N, K, Kp, bias, epi, aux, ldaux)
+    if (dtype == CLIMB_DT_F32) { if (K < 4) FEW(float, 2); else FEW(float, 0); }
+    else { if (K < 4) FEW(bf16_t, 2); else FEW(bf16_t, 0); }
+#undef FEW
     LAUNCH_CHECK();
     return CLIMB_OK;
   }

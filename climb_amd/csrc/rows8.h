@@ -102,41 +102,49 @@ __device__ __forceinline__ float gelu_phi_pair(float x, float& d) {
   return fmaf(-z, q, fmaxf(x, 0.f));
 }
 
-// N consecutive elements of a row (N = 4 or 8), `left` = columns that exist from p on.  VEC: whole rows of 16-byte pieces (the launcher's condition).
-template <bool VEC, int N, typename T>
-__device__ __forceinline__ void row_ld(const T* __restrict__ p, int left, float (&v)[N]) {
-  if constexpr (VEC) {
-    if (left > 0) {
-      if constexpr (N == 8 && sizeof(T) == 2) {
-        const uint4 r = *reinterpret_cast<const uint4*>(p);
-        v[0] = h16lo_to_f32(r.x); v[1] = h16hi_to_f32(r.x); v[2] = h16lo_to_f32(r.y); v[3] = h16hi_to_f32(r.y);
-        v[4] = h16lo_to_f32(r.z); v[5] = h16hi_to_f32(r.z); v[6] = h16lo_to_f32(r.w); v[7] = h16hi_to_f32(r.w);
-      } else {
+// Columns c .. c + N - 1 of a row of C (N = 4 or 8), zeros past its end.  MODE (row_mode): 1 whole rows of aligned pieces, C % N == 0; 0 any address and
+// C >= N: the hardware reads unaligned words, and hipcc makes wide loads of the copy; 2 shorter rows.  The load itself is UNCONDITIONAL -- a piece at or past the end is
+// read as the row's last N columns and shifted down -- because a load under a condition is waited for inside it: the pieces of a row would come one
+// latency after the other.
+template <int MODE, int N, typename T>
+__device__ __forceinline__ void row_ld(const T* __restrict__ row, int c, int C, float (&v)[N]) {
+  if constexpr (MODE == 2) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          const float4 r = ld4(p + i);
-          v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
-        }
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-  } else {
-    if (left >= N) {          // rows at any address: the hardware reads unaligned words, hipcc makes wide loads of the copy
-      T r[N];
-      __builtin_memcpy(r, p, sizeof(r));
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = Act<T>::ld(r + i);
+    for (int i = 0; i < N; ++i) v[i] = c + i < C ? Act<T>::ld(row + c + i) : 0.f;
+    return;
+  }
+  const int sh = max(c - (C - N), 0);
+  const T* p = row + (sh ? C - N : c);
+  if constexpr (MODE == 1) {
+    if constexpr (N == 8 && sizeof(T) == 2) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      v[0] = h16lo_to_f32(r.x); v[1] = h16hi_to_f32(r.x); v[2] = h16lo_to_f32(r.y); v[3] = h16hi_to_f32(r.y);
+      v[4] = h16lo_to_f32(r.z); v[5] = h16hi_to_f32(r.z); v[6] = h16lo_to_f32(r.w); v[7] = h16hi_to_f32(r.w);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = i < left ? Act<T>::ld(p + i) : 0.f;
+      for (int i = 0; i < N; i += 4) {
+        const float4 r = ld4(p + i);
+        v[i] = r.x; v[i + 1] = r.y; v[i + 2] = r.z; v[i + 3] = r.w;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sh ? 0.f : v[i];
+  } else {
+    T r[N];
+    __builtin_memcpy(r, p, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<T>::ld(r + i);
+#pragma unroll
+    for (int b = 1; b < N; b *= 2)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (sh & b) ? (i + b < N ? v[i + b] : 0.f) : v[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sh >= N ? 0.f : v[i];
   }
 }
-template <bool VEC, int N, typename T>
+template <int MODE, int N, typename T>
 __device__ __forceinline__ void row_st(T* __restrict__ p, int left, const float (&v)[N]) {
-  if constexpr (VEC) {
+  if constexpr (MODE == 1) {
     if (left > 0) {
       if constexpr (N == 8 && sizeof(T) == 2) {
         *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
@@ -158,29 +166,46 @@ __device__ __forceinline__ void row_st(T* __restrict__ p, int left, const float 
     }
   }
 }
-// largest absolute value (as bits) over the W lanes that hold a group
-template <int W>
-__device__ __forceinline__ unsigned lanes_umax(unsigned m) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    const unsigned t = __shfl_xor(m, o, 64);
-    m = t > m ? t : m;
+static inline int row_mode(bool aligned, int C, int N) { return C < N ? 2 : (aligned && C % N == 0 ? 1 : 0); }
+
+// Reductions over W = 8, 16 or 64 neighbouring lanes without a trip through LDS: quad permutes, mirrors of 8 and 16 lanes (DPP), and the row / half swaps of
+// gfx950 for 32 and 64.  Every lane ends with the result; the order of a sum is fixed.
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned x) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true); }
+template <int W, typename F>
+__device__ __forceinline__ unsigned lanes_reduce(unsigned x, F f) {
+  x = f(x, dpp<0xB1>(x));          // quad_perm [1, 0, 3, 2]
+  x = f(x, dpp<0x4E>(x));          // quad_perm [2, 3, 0, 1]
+  x = f(x, dpp<0x141>(x));         // mirror within 8 lanes
+  if constexpr (W >= 16) x = f(x, dpp<0x140>(x));          // mirror within 16 lanes
+  if constexpr (W == 64) {
+    auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(r[0], r[1]);
+    auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = f(h[0], h[1]);
   }
-  return m;
+  return x;
+}
+// largest absolute value (as bits)
+template <int W> __device__ __forceinline__ unsigned lanes_umax(unsigned m) {
+  return lanes_reduce<W>(m, [](unsigned a, unsigned b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+  return __uint_as_float(lanes_reduce<64>(__float_as_uint(v), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 
-// true-quotient rounding: k = rint(x / s) from a reciprocal may miss a tie by its rounding; the remainder x - k s is exact in one fma and settles it
-__device__ __forceinline__ int rowq(float x, float s, float rs) {
-  const float k = rintf(x * rs), r = fmaf(-k, s, x), a = 2.f * fabsf(r);
-  int q = (int)k;
-  if (a > s || (a == s && (q & 1))) q += r > 0.f ? 1 : -1;
-  return q;
+// True-quotient rounding.  x * (1 / s) is rounded to the nearest integer k by adding 1.5 * 2^23 in the same fma (k in the low bits), which may miss next to a
+// half; the remainder r = x - k s is exact in one fma and settles it: k moves towards r's sign if 2 |r| > s, or 2 |r| = s and k is odd.  The sign and zero of
+// 2 |r| - s are those of its bits as an integer (an exact zero is +0), so "bits + (k & 1) > 0" is both conditions at once.
+__device__ __forceinline__ unsigned rowq(float x, float s, float rs) {
+  const float magic = 12582912.f, u = fmaf(x, rs, magic), r = fmaf(magic - u, s, x), a = fmaf(2.f, fabsf(r), -s);
+  const unsigned k = __float_as_uint(u);
+  const int away = (__float_as_int(r) >> 31) | 1;
+  return k + ((int)(__float_as_uint(a) + (k & 1u)) > 0 ? away : 0);
 }
 __device__ __forceinline__ float row_scale(unsigned mx) {
   return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
 }
 __device__ __forceinline__ unsigned rowq4(const float (&v)[4], float s, float rs, bool bad) {
-  const unsigned w = ((unsigned)rowq(v[0], s, rs) & 255u) | (((unsigned)rowq(v[1], s, rs) & 255u) << 8) | (((unsigned)rowq(v[2], s, rs) & 255u) << 16) |
-                     (((unsigned)rowq(v[3], s, rs) & 255u) << 24);
+  const unsigned w = __builtin_amdgcn_perm(rowq(v[1], s, rs), rowq(v[0], s, rs), 0x0c0c0400u) | __builtin_amdgcn_perm(rowq(v[3], s, rs), rowq(v[2], s, rs), 0x04000c0cu);
   return bad ? 0u : w;
 }

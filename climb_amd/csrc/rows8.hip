@@ -2,12 +2,14 @@
 // their forward and read it in their backward.  All are bound by HBM; each input is read once and each output written once.
 #include "rows8.h"
 
+// the launcher of a row_mode
+#define BY_MODE(mode, F, ...) ((mode) == 1 ? F(1, __VA_ARGS__) : (mode) == 0 ? F(0, __VA_ARGS__) : F(2, __VA_ARGS__))
 static inline bool al(const void* p, long ld, int elems_per_16b) { return !((uintptr_t)p & 15) && ld % elems_per_16b == 0; }
 
 // ------------------------------------------------------------------------------------------------ row codes
 // One wave owns a row of C <= 256 NV and keeps it in registers; columns [C, Kp) of the code row are written as zeros (the product runs over whole
 // 128-byte pieces).
-template <typename T, bool VEC, int NV>
+template <typename T, int MODE, int NV>
 __global__ __launch_bounds__(256) void rows8_quant_kernel(const T* __restrict__ x, long ldx, signed char* __restrict__ q, long ldq, float* __restrict__ s,
                                                           int M, int C, int Kp) {
   const int lane = threadIdx.x & 63;
@@ -18,7 +20,7 @@ __global__ __launch_bounds__(256) void rows8_quant_kernel(const T* __restrict__ 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * 64 + lane) * 4;
-    row_ld<VEC, 4>(x + row * ldx + c, C - c, v[i]);
+    row_ld<MODE, 4>(x + row * ldx, c, C, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -34,7 +36,7 @@ __global__ __launch_bounds__(256) void rows8_quant_kernel(const T* __restrict__ 
   }
 }
 // rows too long for one wave's registers: a workgroup a row, read twice (the second time from the caches)
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __global__ __launch_bounds__(256) void rows8_quant_long_kernel(const T* __restrict__ x, long ldx, signed char* __restrict__ q, long ldq, float* __restrict__ s,
                                                                int C, int Kp) {
   __shared__ unsigned red[4];
@@ -42,7 +44,7 @@ __global__ __launch_bounds__(256) void rows8_quant_long_kernel(const T* __restri
   unsigned mx = 0;
   float v[4];
   for (int c = threadIdx.x * 4; c < C; c += 1024) {
-    row_ld<VEC, 4>(x + row * ldx + c, C - c, v);
+    row_ld<MODE, 4>(x + row * ldx, c, C, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) mx = max(mx, abs_bits(v[j]));
   }
@@ -53,20 +55,21 @@ __global__ __launch_bounds__(256) void rows8_quant_long_kernel(const T* __restri
   const float sc = row_scale(mx), rs = 1.f / sc;
   if (threadIdx.x == 0) s[row] = sc;
   for (int c = threadIdx.x * 4; c < Kp; c += 1024) {
-    row_ld<VEC, 4>(x + row * ldx + c, C - c, v);
+    row_ld<MODE, 4>(x + row * ldx, c, C, v);
     *reinterpret_cast<unsigned*>(q + row * ldq + c) = rowq4(v, sc, rs, mx >= 0x7f800000u);
   }
 }
-template <typename T, bool VEC>
+template <typename T, int MODE>
 static int rows8_quant_launch(const T* x, long ldx, signed char* q, long ldq, float* s, int M, int C, hipStream_t st) {
   const int Kp = (C + 127) / 128 * 128;
   const dim3 grid((M + 3) / 4), blk(256);
-#define RQ(NV_) hipLaunchKernelGGL((rows8_quant_kernel<T, VEC, NV_>), grid, blk, 0, st, x, ldx, q, ldq, s, M, C, Kp)
-  if (Kp <= 256) RQ(1);
+#define RQ(NV_) hipLaunchKernelGGL((rows8_quant_kernel<T, MODE, NV_>), grid, blk, 0, st, x, ldx, q, ldq, s, M, C, Kp)
+  if constexpr (MODE == 2) RQ(1);
+  else if (Kp <= 256) RQ(1);
   else if (Kp <= 768) RQ(3);
   else if (Kp <= 1536) RQ(6);
   else if (Kp <= 12 * 256) RQ(12);
-  else hipLaunchKernelGGL((rows8_quant_long_kernel<T, VEC>), dim3(M), blk, 0, st, x, ldx, q, ldq, s, C, Kp);
+  else hipLaunchKernelGGL((rows8_quant_long_kernel<T, MODE>), dim3(M), blk, 0, st, x, ldx, q, ldq, s, C, Kp);
 #undef RQ
   LAUNCH_CHECK();
   return CLIMB_OK;
@@ -77,12 +80,11 @@ extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, lo
   if (!x || !q || !s) return CLIMB_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   signed char* qc = (signed char*)q;
-  if (dtype == CLIMB_DT_F32)
-    return (C % 4 == 0 && al(x, ldx, 4)) ? rows8_quant_launch<float, true>((const float*)x, ldx, qc, ldq, s, M, C, st)
-                                         : rows8_quant_launch<float, false>((const float*)x, ldx, qc, ldq, s, M, C, st);
-  if (dtype == CLIMB_DT_BF16)
-    return (C % 4 == 0 && al(x, ldx, 4)) ? rows8_quant_launch<bf16_t, true>((const bf16_t*)x, ldx, qc, ldq, s, M, C, st)
-                                         : rows8_quant_launch<bf16_t, false>((const bf16_t*)x, ldx, qc, ldq, s, M, C, st);
+  const int mode = row_mode(al(x, ldx, 4), C, 4);
+#define RQL(MODE_, T_) rows8_quant_launch<T_, MODE_>((const T_*)x, ldx, qc, ldq, s, M, C, st)
+  if (dtype == CLIMB_DT_F32) return BY_MODE(mode, RQL, float);
+  if (dtype == CLIMB_DT_BF16) return BY_MODE(mode, RQL, bf16_t);
+#undef RQL
   return CLIMB_EINVAL;
 }
 
@@ -90,7 +92,7 @@ extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, lo
 // Eight lanes hold a group of 64 columns (8 each: 16-byte loads in 16 bits); a thread's unit is (row, group).
 //   OP 0  codes <- x                    OP 1  codes <- x, y = gelu(x)
 //   OP 2  y <- codes                    OP 3  y = x gelu'(codes), y2 = gelu(codes) if y2
-template <typename T, bool VEC, int OP>
+template <typename T, int MODE, int OP>
 __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long ldx, T* __restrict__ y, long ldy, T* __restrict__ y2, long ldy2,
                                                    signed char* __restrict__ q, long ldq, unsigned char* __restrict__ e, long lde, unsigned units, int C, unsigned G) {
   constexpr int DEG = GeluDeg<T>::v;
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long
   const int c = (int)(g * ACT8_GROUP + (threadIdx.x & 7) * 8), left = u < units ? C - c : 0;
   float v[8], o[8];
   if constexpr (OP == 0 || OP == 1) {
-    row_ld<VEC, 8>(x + row * ldx + c, left, v);
+    row_ld<MODE, 8>(x + row * ldx, c, C, v);
     unsigned mx = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) mx = max(mx, abs_bits(v[i]));
@@ -112,17 +114,17 @@ __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long
     if constexpr (OP == 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = gelu_phi<T>(v[i]);
-      row_st<VEC, 8>(y + row * ldy + c, left, o);
+      row_st<MODE, 8>(y + row * ldy + c, left, o);
     }
   } else {
-    uint2 w = make_uint2(0u, 0u);
-    if (left > 0) w = *reinterpret_cast<const uint2*>(q + row * ldq + c);
+    if (left <= 0) return;          // (so that every load below is unconditional)
+    const uint2 w = *reinterpret_cast<const uint2*>(q + row * ldq + c);
     const float step = act8_step(e[row * lde + g]);
-    if constexpr (OP == 3) row_ld<VEC, 8>(x + row * ldx + c, left, v);
+    if constexpr (OP == 3) row_ld<MODE, 8>(x + row * ldx, c, C, v);
     const float4 a = act8_unpack4(w.x, step), b = act8_unpack4(w.y, step);
     const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     if constexpr (OP == 2) {
-      row_st<VEC, 8>(y + row * ldy + c, left, d);
+      row_st<MODE, 8>(y + row * ldy + c, left, d);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -130,8 +132,8 @@ __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long
         o[i] = gelu_phi_pair<DEG>(d[i], dg);
         v[i] *= dg;
       }
-      row_st<VEC, 8>(y + row * ldy + c, left, v);
-      if (y2) row_st<VEC, 8>(y2 + row * ldy2 + c, left, o);
+      row_st<MODE, 8>(y + row * ldy + c, left, v);
+      if (y2) row_st<MODE, 8>(y2 + row * ldy2 + c, left, o);
     }
   }
 }
@@ -148,14 +150,15 @@ static int act8_launch(const void* x, long ldx, int dtype, void* y, long ldy, vo
   const long units = (long)M * G;
   if (units >= (1L << 31)) return CLIMB_EUNSUPPORTED;      // 32-bit unit numbers (137 G elements)
   const int pe = dtype == CLIMB_DT_F32 ? 4 : 8;
-  const bool vec = C % 8 == 0 && (OP == 2 || al(x, ldx, pe)) && (OP == 0 || al(y, ldy, pe)) && (!y2 || al(y2, ldy2, pe));
+  const bool aligned = (OP == 2 || al(x, ldx, pe)) && (OP == 0 || al(y, ldy, pe)) && (!y2 || al(y2, ldy2, pe));
   const dim3 grid((unsigned)((units + 31) / 32)), blk(256);
   hipStream_t st = (hipStream_t)stream;
-#define AL_(T_, V_)                                                                                                                                              \
-  hipLaunchKernelGGL((act8_kernel<T_, V_, OP>), grid, blk, 0, st, (const T_*)x, ldx, (T_*)y, ldy, (T_*)y2, ldy2, (signed char*)q, ldq, (unsigned char*)e, lde, \
+  const int mode = row_mode(aligned, C, 8);
+#define AL_(MODE_, T_)                                                                                                                                              \
+  hipLaunchKernelGGL((act8_kernel<T_, MODE_, OP>), grid, blk, 0, st, (const T_*)x, ldx, (T_*)y, ldy, (T_*)y2, ldy2, (signed char*)q, ldq, (unsigned char*)e, lde, \
                      (unsigned)units, C, G)
-  if (dtype == CLIMB_DT_F32) { if (vec) AL_(float, true); else AL_(float, false); }
-  else { if (vec) AL_(bf16_t, true); else AL_(bf16_t, false); }
+  if (dtype == CLIMB_DT_F32) { if (mode == 1) AL_(1, float); else if (mode == 0) AL_(0, float); else AL_(2, float); }
+  else { if (mode == 1) AL_(1, bf16_t); else if (mode == 0) AL_(0, bf16_t); else AL_(2, bf16_t); }
 #undef AL_
   LAUNCH_CHECK();
   return CLIMB_OK;
@@ -177,7 +180,7 @@ extern "C" int climb_act8_gelu_bwd(const void* da, long ldda, int dtype, const v
 
 // ------------------------------------------------------------------------------------------------ LayerNorm
 // One wave owns a row (4 columns a lane, 256 a step); 16 lanes hold a checkpoint group.
-template <typename TO, bool VEC, int NV>
+template <typename TO, int MODE, int NV>
 __global__ __launch_bounds__(256) void act8_ln_fwd_kernel(const float* __restrict__ x, long ldx, const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           float eps, TO* __restrict__ y, long ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                                           signed char* __restrict__ q, long ldq, unsigned char* __restrict__ e, long lde, int M, int C) {
@@ -188,12 +191,18 @@ __global__ __launch_bounds__(256) void act8_ln_fwd_kernel(const float* __restric
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * 64 + lane) * 4;
-    row_ld<VEC, 4>(x + row * ldx + c, C - c, v[i]);
+    row_ld<MODE, 4>(x + row * ldx, c, C, v[i]);
+  }
+  float g[NV][4], b[NV][4];          // (fetched under the row's statistics)
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, g[i]);
+    row_ld<MODE, 4>(beta, (i * 64 + lane) * 4, C, b[i]);
   }
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) s += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
-  const float mean = wave_sum(s) / (float)C;
+  const float mean = lanes_sum(s) / (float)C;
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -204,11 +213,15 @@ __global__ __launch_bounds__(256) void act8_ln_fwd_kernel(const float* __restric
       if (j < left) ss += d * d;
     }
   }
-  const float rstd = rsqrtf(wave_sum(ss) / (float)C + eps);
+  const float rstd = rsqrtf(lanes_sum(ss) / (float)C + eps);
   if (lane == 0) {
     mean_out[row] = mean;
     rstd_out[row] = rstd;
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(g[i][j]), "+v"(b[i][j]));          // (hipcc would move the loads to their use)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * 64 + lane) * 4, left = C - c;
@@ -219,21 +232,20 @@ __global__ __launch_bounds__(256) void act8_ln_fwd_kernel(const float* __restric
     if (left > 0) {
       *reinterpret_cast<unsigned*>(q + row * ldq + c) = act8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], ex);
       if ((lane & 15) == 0) e[row * lde + i * 4 + (lane >> 4)] = (unsigned char)ex;
-      float g[4], b[4], o[4];
-      row_ld<VEC, 4>(gamma + c, left, g);
-      row_ld<VEC, 4>(beta + c, left, b);
+      float o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[j], b[j]);
-      row_st<VEC, 4>(y + row * ldy + c, left, o);
+      for (int j = 0; j < 4; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[i][j], b[i][j]);
+      row_st<MODE, 4>(y + row * ldy + c, left, o);
     }
   }
 }
-template <typename TO, bool VEC>
+template <typename TO, int MODE>
 static int act8_ln_fwd_launch(const float* x, long ldx, const float* gamma, const float* beta, float eps, TO* y, long ldy, float* mean, float* rstd, signed char* q, long ldq,
                               unsigned char* e, long lde, int M, int C, hipStream_t st) {
   const dim3 grid((M + 3) / 4), blk(256);
-#define LF(NV_) hipLaunchKernelGGL((act8_ln_fwd_kernel<TO, VEC, NV_>), grid, blk, 0, st, x, ldx, gamma, beta, eps, y, ldy, mean, rstd, q, ldq, e, lde, M, C)
-  if (C <= 256) LF(1);
+#define LF(NV_) hipLaunchKernelGGL((act8_ln_fwd_kernel<TO, MODE, NV_>), grid, blk, 0, st, x, ldx, gamma, beta, eps, y, ldy, mean, rstd, q, ldq, e, lde, M, C)
+  if constexpr (MODE == 2) LF(1);
+  else if (C <= 256) LF(1);
   else if (C <= 768) LF(3);
   else LF(6);
 #undef LF
@@ -247,15 +259,13 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
   if (M == 0) return CLIMB_OK;
   if (!x || !gamma || !beta || !y || !mean || !rstd) return CLIMB_EINVAL;
   // 4 elements a lane: 16-byte pieces of fp32, 8-byte pieces of the 16-bit type
-  const bool vec = C % 4 == 0 && al(x, ldx, 4) && al(y, ldy, 4) && al(gamma, 0, 4) && al(beta, 0, 4);
+  const int mode = row_mode(al(x, ldx, 4) && al(y, ldy, 4) && al(gamma, 0, 4) && al(beta, 0, 4), C, 4);
   hipStream_t st = (hipStream_t)stream;
   signed char* qc = (signed char*)q;
   unsigned char* ec = (unsigned char*)e;
-  if (y_dtype == CLIMB_DT_F32)
-    return vec ? act8_ln_fwd_launch<float, true>(x, ldx, gamma, beta, eps, (float*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st)
-               : act8_ln_fwd_launch<float, false>(x, ldx, gamma, beta, eps, (float*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st);
-  return vec ? act8_ln_fwd_launch<bf16_t, true>(x, ldx, gamma, beta, eps, (bf16_t*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st)
-             : act8_ln_fwd_launch<bf16_t, false>(x, ldx, gamma, beta, eps, (bf16_t*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st);
+#define LFL(MODE_, TO_) act8_ln_fwd_launch<TO_, MODE_>(x, ldx, gamma, beta, eps, (TO_*)y, ldy, mean, rstd, qc, ldq, ec, lde, M, C, st)
+  return y_dtype == CLIMB_DT_F32 ? BY_MODE(mode, LFL, float) : BY_MODE(mode, LFL, bf16_t);
+#undef LFL
 }
 
 // dx = dres + rstd (g - mean_c(g) - xh mean_c(g xh)),  g = dy gamma,  xh = (codes - mean) rstd;  partial column sums {dgamma, dbeta, colsum(dx)} of the
@@ -263,7 +273,7 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
 #define A8LN_WAVES 8
 // rows a wave: three where that still leaves two workgroups a CU (12288 rows: 512), else one -- fewer partial rows against more waves on a short launch
 static inline int a8ln_rpw(int M) { return M >= 8192 ? 3 : 1; }
-template <typename T, bool VEC, int NV>
+template <typename T, int MODE, int NV, bool RES>
 __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* __restrict__ dy, long lddy, const signed char* __restrict__ q, long ldq,
                                                                       const unsigned char* __restrict__ e, long lde, const float* __restrict__ mean,
                                                                       const float* __restrict__ rstd, const float* __restrict__ gamma, const float* dres, long ldr,
@@ -274,55 +284,77 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * 64 + lane) * 4;
-    row_ld<VEC, 4>(gamma + c, C - c, gm[i]);
+    row_ld<MODE, 4>(gamma, c, C, gm[i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) ag[i][j] = ab[i][j] = as[i][j] = 0.f;
   }
-  for (int rr = 0; rr < rpw; ++rr) {
-    const long row = ((long)blockIdx.x * rpw + rr) * A8LN_WAVES + wid;
-    if (row >= M) break;
-    const float mu = mean[row], rs = rstd[row];
-    float d[NV][4], rin[NV][4], xh[NV][4];
-    unsigned w[NV], ex[NV];
+  struct Row { float d[NV][4], r[NV][4], mu, rs; unsigned w[NV], ex[NV]; };
+  auto load = [&](Row& R, long row) {
+    R.mu = mean[row];
+    R.rs = rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * 64 + lane) * 4, left = C - c;
-      row_ld<VEC, 4>(dy + row * lddy + c, left, d[i]);
-      w[i] = left > 0 ? *reinterpret_cast<const unsigned*>(q + row * ldq + c) : 0u;
-      ex[i] = left > 0 ? e[row * lde + i * 4 + (lane >> 4)] : 1u;
-      if (dres) row_ld<VEC, 4>(dres + row * ldr + c, left, rin[i]);
+      row_ld<MODE, 4>(dy + row * lddy, c, C, R.d[i]);
+      R.w[i] = *reinterpret_cast<const unsigned*>(q + row * ldq + (left > 0 ? c : 0));          // (unconditional, as row_ld)
+      R.ex[i] = e[row * lde + (left > 0 ? i * 4 + (lane >> 4) : 0)];
+      if constexpr (RES) row_ld<MODE, 4>(dres + row * ldr, c, C, R.r[i]);
       else
 #pragma unroll
-        for (int j = 0; j < 4; ++j) rin[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) R.r[i][j] = 0.f;
     }
-    float s1 = 0.f, s2 = 0.f;
+  };
+  auto finish = [&](const Row& R, long row) {
+    float s1 = 0.f, s2 = 0.f, xh[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float4 xv = act8_unpack4(w[i], act8_step(ex[i]));
+      const bool in = (i * 64 + lane) * 4 < C;
+      const float4 xv = act8_unpack4(in ? R.w[i] : 0u, in ? act8_step(R.ex[i]) : 0.f);
       const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {          // (columns past C have d = gamma = 0: no contribution)
-        xh[i][j] = (xx[j] - mu) * rs;
-        const float g = d[i][j] * gm[i][j];
+        xh[i][j] = (xx[j] - R.mu) * R.rs;
+        const float g = R.d[i][j] * gm[i][j];
         s1 += g;
         s2 += g * xh[i][j];
       }
     }
-    const float m1 = wave_sum(s1) / (float)C, m2 = wave_sum(s2) / (float)C;
+    const float m1 = lanes_sum(s1) / (float)C, m2 = lanes_sum(s2) / (float)C;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * 64 + lane) * 4, left = C - c;
       float o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[j] = rin[i][j] + rs * (d[i][j] * gm[i][j] - m1 - xh[i][j] * m2);
-        ag[i][j] += d[i][j] * xh[i][j];
-        ab[i][j] += d[i][j];
+        o[j] = R.r[i][j] + R.rs * (R.d[i][j] * gm[i][j] - m1 - xh[i][j] * m2);
+        ag[i][j] += R.d[i][j] * xh[i][j];
+        ab[i][j] += R.d[i][j];
         as[i][j] += o[j];
       }
-      row_st<VEC, 4>(dx + row * ldo + c, left, o);
-      if (dcast) row_st<VEC, 4>(dcast + row * ldc + c, left, o);
+      row_st<MODE, 4>(dx + row * ldo + c, left, o);
+      if (dcast) row_st<MODE, 4>(dcast + row * ldc + c, left, o);
     }
+  };
+  // a row's loads go out before the row in front of it is finished (dx may be dres: rows are disjoint, and a wave reads its row before it writes it); rows of
+  // more than 768 columns would need more registers than two waves a SIMD have
+  const long row0 = (long)blockIdx.x * rpw * A8LN_WAVES + wid;
+  if constexpr (NV > 3) {
+    for (int rr = 0; rr < rpw && row0 + rr * A8LN_WAVES < M; ++rr) {
+      Row A;
+      load(A, row0 + rr * A8LN_WAVES);
+      finish(A, row0 + rr * A8LN_WAVES);
+    }
+  } else if (row0 < M) {
+    Row A;
+    load(A, row0);
+    int rr = 1;
+    for (; rr < rpw && row0 + rr * A8LN_WAVES < M; ++rr) {
+      Row B;
+      load(B, row0 + rr * A8LN_WAVES);
+      finish(A, row0 + (rr - 1) * A8LN_WAVES);
+      A = B;
+    }
+    finish(A, row0 + (rr - 1) * A8LN_WAVES);
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
@@ -342,17 +374,20 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
     }
   }
 }
-template <typename T, bool VEC>
+template <typename T, int MODE>
 static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long ldq, const unsigned char* e, long lde, const float* mean, const float* rstd,
                               const float* gamma, const float* dres, long ldr, float* dx, long ldo, T* dcast, long ldc, float* part, int M, int C, hipStream_t st) {
   const int rpw = a8ln_rpw(M);
   const dim3 grid((M + A8LN_WAVES * rpw - 1) / (A8LN_WAVES * rpw)), blk(64 * A8LN_WAVES);
-#define LB(NV_) \
-  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, VEC, NV_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C, rpw)
-  if (C <= 256) LB(1);
+#define LBK(NV_, RES_) \
+  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, MODE, NV_, RES_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C, rpw)
+#define LB(NV_) do { if (dres) LBK(NV_, true); else LBK(NV_, false); } while (0)
+  if constexpr (MODE == 2) LB(1);
+  else if (C <= 256) LB(1);
   else if (C <= 768) LB(3);
   else LB(6);
 #undef LB
+#undef LBK
   LAUNCH_CHECK();
   return CLIMB_OK;
 }
@@ -365,12 +400,11 @@ extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, co
   if (C > 1536) return CLIMB_EUNSUPPORTED;
   if (M == 0) return CLIMB_OK;
   if (!dy || !mean || !rstd || !gamma || !dx || !part) return CLIMB_EINVAL;
-  const bool vec = C % 4 == 0 && al(dy, lddy, 4) && al(dx, ldo, 4) && al(gamma, 0, 4) && (!dres_in || al(dres_in, ldr, 4)) && (!dcast || al(dcast, ldc, 4));
+  const int mode = row_mode(al(dy, lddy, 4) && al(dx, ldo, 4) && al(gamma, 0, 4) && (!dres_in || al(dres_in, ldr, 4)) && (!dcast || al(dcast, ldc, 4)), C, 4);
   hipStream_t st = (hipStream_t)stream;
-#define LBT(T_, V_)                                                                                                                                                   \
-  act8_ln_bwd_launch<T_, V_>((const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc, \
-                             part, M, C, st)
-  if (dtype == CLIMB_DT_F32) return vec ? LBT(float, true) : LBT(float, false);
-  return vec ? LBT(bf16_t, true) : LBT(bf16_t, false);
-#undef LBT
+#define LBL(MODE_, T_)                                                                                                                                                   \
+  act8_ln_bwd_launch<T_, MODE_>((const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc, \
+                                part, M, C, st)
+  return dtype == CLIMB_DT_F32 ? BY_MODE(mode, LBL, float) : BY_MODE(mode, LBL, bf16_t);
+#undef LBL
 }

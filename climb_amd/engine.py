@@ -129,14 +129,29 @@ class Workspace:
         self.tmean, self.trstd = buf((B * T,)), buf((B * T,))
         self.a_patch = buf((B * self.NP, cfg["channels"] * cfg["patch"] ** 2), adt)
         self.proj = buf((B * self.NP, H))
-        self.x = [buf((M, H)) for _ in range(L + 1)]          # residual stream at every layer boundary (fp32)
-        self.h1 = [buf((M, H)) for _ in range(L)]
-        self.xn = [opbuf(M, H) for _ in range(L)]
-        self.hn = [opbuf(M, H) for _ in range(L)]
+        def per_layer(make, n, shared=1):
+            """n buffers; under act8 `shared` of them in turn (a layer's checkpoint is what the backward reads, the tensor itself is scratch)"""
+            if not eng.act8:
+                return [make() for _ in range(n)]
+            few = [make() for _ in range(min(shared, n))]
+            return [few[i % len(few)] for i in range(n)]
+        self.x = per_layer(lambda: buf((M, H)), L + 1, 2)          # residual stream at every layer boundary (fp32)
+        self.h1 = per_layer(lambda: buf((M, H)), L)
+        self.xn = per_layer(lambda: opbuf(M, H), L)
+        self.hn = per_layer(lambda: opbuf(M, H), L)
         self.qkv = [buf((M, 3 * H), adt) for _ in range(L)]
         self.ctx = [buf((M, H), adt) for _ in range(L)]
-        self.u = [buf((M, Fd), adt) for _ in range(L)]
-        self.a = [opbuf(M, Fd) for _ in range(L)]
+        self.u = per_layer(lambda: buf((M, Fd), adt), L)
+        self.a = per_layer(lambda: opbuf(M, Fd), L)
+        self.i8 = None               # scratch of the int8 products (eval_i8), allocated by the first forward that runs them
+        if eng.act8:
+            from .rows8 import Checkpoint
+            self.ck = [{n: Checkpoint(M, c, (M,), adt, dev) for n, c in (("x", H), ("h1", H), ("xn", H), ("hn", H), ("u", Fd))} for _ in range(L)]
+            self.du_a = buf((M, Fd), adt)          # d(gelu output) before x gelu'(checkpoint)
+            self.nln8 = _lib.query_arg("climb_act8_layernorm_bwd_blocks", M)
+            self.part8 = buf((self.nln8 * 3 * H,))
+            self.wg8_bytes = max(_lib.query_arg("climb_act8_weight_grad_workspace", M, n, H) for n in (3 * H, Fd))
+            self.wg8 = torch.empty((max(self.wg8_bytes, 16),), dtype=torch.uint8, device=dev)
         if sp:      # split twins of the fp32 tensors that something besides a GEMM reads too (attention output / gradient, im2col, d(projection))
             self.a_patch_s = opbuf(B * self.NP, cfg["channels"] * cfg["patch"] ** 2)
             self.ctx_s = [opbuf(M, H) for _ in range(L)]
@@ -286,6 +301,19 @@ class ViltEngine:
         # LayerNorm, forward and backward.  Same loss, same gradients (tests/test_gpu_parity.py compares the two steps); off by default so that
         # the default step executes every FLOP of the reference's (bench.py times both).
         self.cls_only_last = os.environ.get("CLIMB_AMD_CLS_ONLY_LAST", "0") != "0" and not self.split      # (the opt-in row pruning has no split path)
+        # OPT-IN, 16-bit modes (climb_amd/rows8.py's formats, csrc/rows8.h):
+        #   eval_i8 (CLIMB_AMD_EVAL_I8=1): a forward that saves nothing (evaluation under no_grad) runs the encoder layers' linear products in int8, tokens
+        #     quantised by row, weights by output channel once per parameter version; everything else of the forward as it is
+        #   act8 (CLIMB_AMD_ACT8=1): a training forward keeps the LayerNorms' and the GELU's inputs and the inputs of the QKV and up-projections as 8-bit
+        #     checkpoints instead of 16 / 32-bit tensors (36 -> 16 bytes a token, layer and channel); the backward reads those
+        self.eval_i8 = os.environ.get("CLIMB_AMD_EVAL_I8", "0") != "0" and precision == "bf16"
+        self.act8 = os.environ.get("CLIMB_AMD_ACT8", "0") != "0" and precision == "bf16"
+        if self.act8 and (layout.adapters or self.cls_only_last):
+            raise NotImplementedError("CLIMB_AMD_ACT8: no 8-bit checkpoints with adapters or CLIMB_AMD_CLS_ONLY_LAST")
+        self._i8_pass = False          # inside a forward that eval_i8 covers
+        self._i8_weights: Dict[str, object] = {}          # weight name -> rows8.RowCodes
+        self._i8_version = None
+        self._param_epoch = 0          # parameter updates that bump no version counter (FusedAdamW writes through the C ABI)
 
     # ------------------------------------------------------------------ buffers
     def allocate(self):
@@ -399,7 +427,7 @@ class ViltEngine:
 
     def workspace(self, B: int, T: int, gh: int = None, gw: int = None, nseq: int = None, tag: str = None) -> Workspace:
         g0 = self.cfg["image"] // self.cfg["patch"]
-        key = (B, T, gh or g0, gw or g0, nseq, tag)
+        key = (B, T, gh or g0, gw or g0, nseq, tag, self.act8)
         ws = self._ws.get(key)
         if ws is None:
             if len(self._ws) >= 3:      # bound HBM use when batch shapes vary (last partial batch, replay batches, canvases)
@@ -438,7 +466,32 @@ class ViltEngine:
         """dst (split [2][M][C]) = f(src fp32 [M, C]): 0 copy, 1 gelu, 2 src * gelu'(aux)"""
         _lib.call("climb_split_f32", src, C, dst, C, M * C, M, C, mode, aux, C, _stream())
 
+    def _i8_weight(self, wname, N, K):
+        """row codes of the fp32 master weight, one scale an output channel; laid out once per parameter version"""
+        ver = (self.flat.data_ptr(), self.flat._version, self._param_epoch)
+        if ver != self._i8_version:
+            self._i8_weights.clear()
+            self._i8_version = ver
+        w = self._i8_weights.get(wname)
+        if w is None:
+            from . import rows8
+            o = self.layout.offset[wname]
+            with torch.no_grad():
+                w = self._i8_weights[wname] = rows8.quantize_rows(self.flat[o:o + N * K].view(N, K).detach())
+        return w
+
+    def _i8_fwd(self, ws, X, wname, bname, Y, M, N, K, epi, aux, out_f32):
+        w = self._i8_weight(wname, N, K)
+        nb = _lib.query_arg("climb_linear_i8_workspace", M, K)
+        if ws.i8 is None or ws.i8.numel() < nb:
+            ws.i8 = torch.empty((nb,), dtype=torch.uint8, device=self.device)
+        p = w.buf.data_ptr()
+        self._timed_call("linear_i8", 2.0 * M * N * K, "climb_linear_i8", X, K, BF16, p, w.ld, p + N * w.ld, Y, N, F32 if out_f32 else BF16, M, N, K,
+                         self.p(bname) if bname else None, epi, aux, N, ws.i8, nb, _stream())
+
     def linear_fwd(self, X, wname, bname, Y, M, N, K, epi=EPI_NONE, aux=None, aux_out=None, aux2=None, out_f32=False):
+        if self._i8_pass and epi in (EPI_NONE, self.epi_gelu) and aux2 is None:
+            return self._i8_fwd(self._i8_pass, X, wname, bname, Y, M, N, K, EPI_GELU if epi == self.epi_gelu else EPI_NONE, None, out_f32)
         if self.split and not self._force_f32:
             if epi not in (EPI_NONE, EPI_RESID):
                 raise NotImplementedError("bf16x3: fused activation epilogues are not built for split operands")
@@ -475,6 +528,28 @@ class ViltEngine:
             self._gemm_f32(dY, 1, N, X, 1, K, self.g(wname), K, N, K, M, beta=1.0)
         else:
             self._bf16_dw(dY, X, wname, M, N, K, self.g(bname) if want_b else None)
+
+    # ---- 8-bit activation checkpoints (act8)
+    def ln_fwd_act8(self, x, ln, y, mean, rstd, ck, ckn, M, H):
+        """y = LayerNorm(x); x kept in `ck`, y -- the next product's input, which its weight gradient reads -- in `ckn`"""
+        st = _stream()
+        _lib.call("climb_act8_layernorm_fwd", x, H, self.p(ln + ".weight"), self.p(ln + ".bias"), self.cfg["ln_eps"], y, H, self.adt, mean, rstd, *ck._args(), M, H, st)
+        _lib.call("climb_act8_save", y, H, self.adt, *ckn._args(), M, H, st)
+
+    def ln_bwd_act8(self, ws, dy, ck, mean, rstd, ln, bias_name, M, H):
+        """climb_layernorm_bwd + reduce3 on a checkpoint: the residual gradient ws.dres in place, its 16-bit copy in ws.dres_c"""
+        _lib.call("climb_act8_layernorm_bwd", dy, H, self.adt, *ck._args(), mean, rstd, self.p(ln + ".weight"), ws.dres, H, ws.dres, H, ws.dres_c, H, ws.part8, M, H, _stream())
+        self.reduce3(ws.part8, ws.nln8, H, ln + ".weight", ln + ".bias", bias_name)
+
+    def dw_act8(self, ws, dY, ck, wname, bname, M, N, K):
+        """grad(W)[N, K] += dY^T x, grad(b)[N] += column sums of dY, x from its checkpoint"""
+        want_b = self.requires_grad[bname]
+        if not self.requires_grad[wname]:
+            if want_b:
+                self.bias_grad(dY, self.adt, bname, M, N, ws)
+            return
+        self._timed_call("act8_weight_grad", 2.0 * M * N * K, "climb_act8_weight_grad", dY, N, *ck._args(), self.g(wname), K, self.g(bname) if want_b else None, M, N, K, 1.0,
+                         ws.wg8, ws.wg8_bytes, _stream())
 
     # the same three products on a row-STRIDED subset (the last layer's [CLS] rows: row b of an operand is row b * S_pad of a saved [M, .] one)
     def _lin_fwd_ld(self, X, ldx, wname, bname, Y, ldy, M, N, K, epi=EPI_NONE, aux=None, ldaux=0, aux_out=None, ldauxo=0, out_f32=False):
@@ -665,6 +740,7 @@ class ViltEngine:
     def params_updated(self, shadow_fresh: bool = False, t_fresh=None, updated=None):
         """`updated` (names, optional): everything the optimizer changed this step -- anything else keeps its transposed shadow.  Two updates without a
         refresh in between (nobody ran a forward) accumulate."""
+        self._param_epoch += 1
         prev_pending = self._shadow_stale == "transpose-only"
         prev_upd = getattr(self, "_t_updated", None)
         self._shadow_stale = "transpose-only" if (shadow_fresh and self._shadow_stale in (False, "transpose-only")) else True
@@ -793,11 +869,18 @@ class ViltEngine:
         r = self.layout.adapters[ad] if ad is not None else 0
         prune = self.cls_only_last and ad is None
         odt = self.odt
+        act8 = self.act8 and save
+        if act8 and (ad is not None or prune):
+            raise NotImplementedError("8-bit activation checkpoints (act8) with an active adapter or cls_only_last")
+        self._i8_pass = ws if (self.eval_i8 and not save and not prune) else False
         for i in range(cfg["layers"]):
             l = f"{ENC}encoder.layer.{i}."
             x = ws.x[i]
-            _lib.call("climb_layernorm_fwd", x, H, self.p(l + "layernorm_before.weight"), self.p(l + "layernorm_before.bias"), cfg["ln_eps"],
-                      ws.xn[i], H, odt, ws.mean1[i], ws.rstd1[i], M, H, st)
+            if act8:
+                self.ln_fwd_act8(x, l + "layernorm_before", ws.xn[i], ws.mean1[i], ws.rstd1[i], ws.ck[i]["x"], ws.ck[i]["xn"], M, H)
+            else:
+                _lib.call("climb_layernorm_fwd", x, H, self.p(l + "layernorm_before.weight"), self.p(l + "layernorm_before.bias"), cfg["ln_eps"],
+                          ws.xn[i], H, odt, ws.mean1[i], ws.rstd1[i], M, H, st)
             # fused QKV projection: q/k/v weights are adjacent in the flat buffer (HF:325-327 as one [2304,768] GEMM)
             self.linear_fwd(ws.xn[i], l + "attention.attention.query.weight", l + "attention.attention.query.bias", ws.qkv[i], M, 3 * H, H)
             if self.split:          # three-product bf16 MFMAs on planes formed inside the kernel; ctx as fp32 (the backward's softmax row term) AND as the out-projection's operand
@@ -827,6 +910,12 @@ class ViltEngine:
                 a_ = f"{l}attention.output.adapters.{ad}."
                 self.linear_fwd(ws.ctx[i], l + "attention.output.dense.weight", l + "attention.output.dense.bias", ws.ya[i], M, H, H)
                 self.adapter_fwd(a_, ws.ya[i], x, ws.za[i], ws.sa[i], ws.h1[i], M, H, r)
+            if act8:
+                self.ln_fwd_act8(ws.h1[i], l + "layernorm_after", ws.hn[i], ws.mean2[i], ws.rstd2[i], ws.ck[i]["h1"], ws.ck[i]["hn"], M, H)
+                self.linear_fwd(ws.hn[i], l + "intermediate.dense.weight", l + "intermediate.dense.bias", ws.u[i], M, Fd, H)
+                _lib.call("climb_act8_gelu_fwd", ws.u[i], Fd, adt, ws.a[i], Fd, *ws.ck[i]["u"]._args(), M, Fd, st)
+                self.linear_fwd_resid(ws.a[i], l + "output.dense.weight", l + "output.dense.bias", ws.x[i + 1], M, H, Fd, ws.h1[i])
+                continue
             _lib.call("climb_layernorm_fwd", ws.h1[i], H, self.p(l + "layernorm_after.weight"), self.p(l + "layernorm_after.bias"), cfg["ln_eps"],
                       ws.hn[i], H, odt, ws.mean2[i], ws.rstd2[i], M, H, st)
             if self.split and SPLIT_FUSED_ACT and _lib.query_arg("climb_gemm_split_nt_takes_act", M, Fd, H):
@@ -844,6 +933,7 @@ class ViltEngine:
                 a_ = f"{l}output.adapters.{ad}."
                 self.linear_fwd(ws.a[i], l + "output.dense.weight", l + "output.dense.bias", ws.yo[i], M, H, Fd)
                 self.adapter_fwd(a_, ws.yo[i], ws.h1[i], ws.zo[i], ws.so[i], ws.x[i + 1], M, H, r)
+        self._i8_pass = False
         xL, ldxL = (ws.xLc, H) if prune else (ws.x[cfg["layers"]], ws.S_pad * H)
         # final LayerNorm only on the row the pooler consumes (token 0 = text [CLS]); `last_hidden_state` is never
         # used by CLiMB (REF/modeling/vilt.py:123-124), so the other S-1 rows are dead work we skip
@@ -862,7 +952,7 @@ class ViltEngine:
             self._generation = getattr(self, "_generation", 0) + 1
             # ViLT-BERT: `inputs_embeds` is BertParams' reusable output buffer, which the next BERT forward of this shape overwrites -- the
             # embedding backward reads it, so the saved copy is its own tensor (7.9 MB at bs = 64)
-            self.saved = dict(ws=ws, input_ids=input_ids, token_type_ids=token_type_ids, adapter=ad, var=var, generation=self._generation, cls_only=prune,
+            self.saved = dict(ws=ws, act8=act8, input_ids=input_ids, token_type_ids=token_type_ids, adapter=ad, var=var, generation=self._generation, cls_only=prune,
                               inputs_embeds=inputs_embeds.clone() if inputs_embeds is not None else None)
             self.last_ws = ws
         return ws.pooled
@@ -874,6 +964,8 @@ class ViltEngine:
             self._bf16_fwd(X, wname, bname, Y, M, N, K, EPI_NONE, None, None, out_f32=True)
 
     def linear_fwd_resid(self, X, wname, bname, Y, M, N, K, resid):
+        if self._i8_pass:
+            return self._i8_fwd(self._i8_pass, X, wname, bname, Y, M, N, K, EPI_RESID, resid, True)
         if self.precision == "fp32":          # (and split)
             self.linear_fwd(X, wname, bname, Y, M, N, K, EPI_RESID, resid)
         else:
@@ -898,7 +990,7 @@ class ViltEngine:
     # ------------------------------------------------------------------ deferred, grouped weight gradients
     def _dw_group_size(self, ws: Workspace, ad) -> int:
         """Layers per grouped weight-gradient launch for this backward; 0 = the immediate per-GEMM path."""
-        if (self.precision != "bf16" and not self.split) or (ws.M % 128) or self.overlap_dw:
+        if (self.precision != "bf16" and not self.split) or (ws.M % 128) or self.overlap_dw or self.act8:          # (act8: weight gradients are taken layer by layer, from scratch tensors)
             return 0
         if ad is not None:
             # under an active adapter the base is normally frozen (train_adapter); the backward then keeps one d(y) scratch for all layers,
@@ -1199,6 +1291,14 @@ class ViltEngine:
             dxc(nL).view(B, ws.S_pad, H)[:, 0].copy_(ws.dres.view(B, ws.S_pad, H)[:, 0])
         for i in range(cfg["layers"] - 1, first_layer - 1, -1):
             l = f"{ENC}encoder.layer.{i}."
+            if sv["act8"]:
+                self._layer_backward_act8(ws, l, i, M, H, Fd, need_dx=i > first_layer or embeddings,
+                                          below=f"{ENC}encoder.layer.{i - 1}.output.dense.bias" if i > first_layer else None)
+                group.append(i)
+                if len(group) >= rgroup or i == first_layer:
+                    self._ready(lay.layer_range[min(group)][0], lay.layer_range[max(group)][1])
+                    group = []
+                continue
             if prune and i == nL - 1:
                 self._last_layer_backward_cls(ws, l, i)     # MLP, LayerNorm and out-projection on the B [CLS] rows; leaves d(ctx) in ws.dctx
             else:
@@ -1278,6 +1378,27 @@ class ViltEngine:
             self._ready(*lay.embed_range)
         self.saved = None          # the activations are consumed: a later no-grad forward may use this workspace again
 
+    def _layer_backward_act8(self, ws: Workspace, l: str, i: int, M, H, Fd, need_dx: bool, below: Optional[str]):
+        """One layer's backward from its 8-bit checkpoints.  In and out: d(x_{i+1}) -> d(x_i) in ws.dres (fp32) and ws.dres_c (16 bit); `below` = the output bias
+        of the layer below, whose gradient is the column sums of d(x_i)."""
+        st = _stream()
+        ck = ws.ck[i]
+        # MLP: x_{i+1} = h1 + W2 gelu(u) + b2,  u = W1 hn + b1
+        self.linear_dx(ws.dres_c, l + "output.dense.weight", ws.du_a, M, H, Fd)
+        _lib.call("climb_act8_gelu_bwd", ws.du_a, Fd, self.adt, *ck["u"]._args(), ws.du, Fd, ws.a[i], Fd, M, Fd, st)
+        self.linear_dw(ws.dres_c, ws.a[i], l + "output.dense.weight", M, H, Fd)
+        self.dw_act8(ws, ws.du, ck["hn"], l + "intermediate.dense.weight", l + "intermediate.dense.bias", M, Fd, H)
+        self.linear_dx(ws.du, l + "intermediate.dense.weight", ws.dhn, M, Fd, H)
+        self.ln_bwd_act8(ws, ws.dhn, ck["h1"], ws.mean2[i], ws.rstd2[i], l + "layernorm_after", l + "attention.output.dense.bias", M, H)
+        # attention: h1 = x + Wo ctx + bo
+        self.linear_dw(ws.dres_c, ws.ctx[i], l + "attention.output.dense.weight", M, H, H)
+        self.linear_dx(ws.dres_c, l + "attention.output.dense.weight", ws.dctx, M, H, H)
+        self.attn_bwd(ws.qkv[i], ws.key_bias, ws.dctx, ws.ctx[i], ws.lse[i], ws.delta, ws.dqkv, ws.B, ws.S_pad)
+        self.dw_act8(ws, ws.dqkv, ck["xn"], l + "attention.attention.query.weight", l + "attention.attention.query.bias", M, 3 * H, H)
+        if need_dx:
+            self.linear_dx(ws.dqkv, l + "attention.attention.query.weight", ws.dxn, M, 3 * H, H)
+            self.ln_bwd_act8(ws, ws.dxn, ck["x"], ws.mean1[i], ws.rstd1[i], l + "layernorm_before", below, M, H)
+
     def _last_layer_backward_cls(self, ws: Workspace, l: str, i: int):
         """Backward of the last layer's MLP, `layernorm_after` and attention out-projection on the B [CLS] rows (`cls_only_last`): d(x_L) is
         zero everywhere else, so every product below is the dense one with its all-zero rows left out.  In: d(x_L) in the [CLS] rows of
@@ -1316,6 +1437,13 @@ class ViltEngine:
             finally:
                 self._force_f32 = False
             return
+        i8, self._i8_pass = self._i8_pass, False          # (the bottleneck's skinny products stay in 16 bits)
+        try:
+            self._adapter_fwd_h16(a_, y, resid, z_pre, s_act, out, M, H, r)
+        finally:
+            self._i8_pass = i8
+
+    def _adapter_fwd_h16(self, a_: str, y, resid, z_pre, s_act, out, M, H, r):
         if self.precision != "fp32" and H % 128 == 0 and r % 16 == 0 and r <= 64 and _FUSED_ADAPTER:
             _lib.call("climb_adapter_fwd_bf16", y, H, resid, H, self.sp(a_ + "adapter_down.0.weight"), self.p(a_ + "adapter_down.0.bias"),
                       self.sp(a_ + "adapter_up.weight"), self.p(a_ + "adapter_up.bias"), z_pre, s_act, r, out, H, M, H, r, _stream())

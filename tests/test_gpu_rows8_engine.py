@@ -1,0 +1,229 @@
+"""The two opt-in uses of 8-bit rows in the engine: training with 8-bit activation checkpoints (CLIMB_AMD_ACT8=1, ViltEngine.act8) and evaluation with int8
+linear products (CLIMB_AMD_EVAL_I8=1, ViltEngine.eval_i8), against the same model without them."""
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import vilt_oracle as vo
+from tests.test_gpu_parity import enc_to_inputs, grads_of, make_model
+
+pytestmark = pytest.mark.gpu
+H16 = os.environ.get("CLIMB_AMD_H16", "bf16")
+
+
+def _model(**flags):
+    model, _ = make_model(["vqa"], 42, precision=H16)
+    eng = model._host.engine()
+    for k, v in flags.items():
+        setattr(eng, k, v)
+    return model, eng
+
+
+def _batch(B, seed):
+    enc = vo.synthetic_encodings(B, seed=seed, ragged_text=True)
+    return (*enc_to_inputs(enc), vo.synthetic_vqa_targets(B, seed=seed))
+
+
+def _rel(a, b):
+    return float((a.double() - b.double()).norm() / (b.double().norm() + 1e-30))
+
+
+def _tensors(o, seen, depth=0):
+    if isinstance(o, torch.Tensor):
+        seen[o.untyped_storage().data_ptr()] = o.untyped_storage().nbytes()
+    elif isinstance(o, (list, tuple)):
+        for v in o:
+            _tensors(v, seen, depth + 1)
+    elif isinstance(o, dict):
+        for v in o.values():
+            _tensors(v, seen, depth + 1)
+    elif hasattr(o, "buf"):
+        _tensors(o.buf, seen, depth + 1)
+    return seen
+
+
+@pytest.fixture(scope="module")
+def steps():
+    """one training step of the same model and batch: plain 16-bit, with checkpoints, and the fp32 mode"""
+    images, texts, target = _batch(5, 3)
+    out = {}
+    for name in ("plain", "act8", "fp32"):
+        if name == "fp32":
+            if H16 == "fp16":
+                continue          # (one process, one 16-bit type; the fp32 mode needs neither)
+            model, _ = make_model(["vqa"], 42, precision="fp32")
+        else:
+            model, eng = _model(act8=name == "act8")
+        model.train()
+        loss, (pooled, logits), _, _ = model.fused_forward_backward("vqa", images, texts, target)
+        out[name] = (float(loss), pooled.cpu(), logits.cpu(), grads_of(model))
+        if name != "fp32":
+            ws = vars(eng.last_ws)
+            kept = ("ck", "qkv", "ctx") if name == "act8" else ("x", "h1", "xn", "hn", "u", "a", "qkv", "ctx")
+            out[name + "_bytes"] = sum(_tensors([ws[k] for k in kept], {}).values())
+    return out
+
+
+def test_checkpointed_step_has_the_plain_steps_gradients(steps):
+    """The forward differs from the plain one in one rounding (the GELU reads its input in 16 bits), so loss and outputs agree to the 16-bit mode's own noise.
+    The backward reads activations whose codes err by at most half a step of max / 63.5 of 64 values (normal data: 2.5 sigma / 63.5 / sqrt 12 = 1.1 % r.m.s.): a
+    weight gradient inherits that once, a layer's input gradient through LayerNorm and GELU' about as much again, and 12 layers add independent errors to a
+    residual stream that carries most of the gradient past them: 1.1 % (1 + sqrt(12) / 2) = 3 % expected, 8 % allowed; a checkpoint read with a wrong scale,
+    layout, layer or statistic is off by far more."""
+    loss, pooled, logits, G = steps["act8"]
+    l0, p0, o0, G0 = steps["plain"]
+    assert abs(loss - l0) < 2e-3 * abs(l0) and _rel(pooled, p0) < 0.03 and _rel(logits, o0) < 0.03
+    assert set(G) == set(G0)
+    worst = ("", 0.0)
+    for n in G0:
+        if n.endswith("attention.key.bias"):          # identically zero up to rounding
+            continue
+        r = _rel(G[n], G0[n])
+        worst = max(worst, (n, r), key=lambda t: t[1])
+        assert r < 0.08, (n, r)
+    print("worst gradient:", worst)
+    if "fp32" in steps:          # ... and is hardly further from the fp32 mode than the plain 16-bit step
+        Gf = steps["fp32"][3]
+        a = float(np.median([_rel(G[n], Gf[n]) for n in Gf if not n.endswith("key.bias")]))
+        b = float(np.median([_rel(G0[n], Gf[n]) for n in Gf if not n.endswith("key.bias")]))
+        print("median error against fp32: checkpoints %.4f, plain %.4f" % (a, b))
+        assert a < b + 0.03
+
+
+def test_checkpoints_take_less_than_half_of_the_saved_activations(steps):
+    """a layer keeps 6 H (q, k, v) + 2 H (attention output) + 8 H (codes; 1 / 64 more of exponents) bytes a token instead of 36 H"""
+    print("bytes kept:", steps["plain_bytes"], "->", steps["act8_bytes"])
+    M, H = 5 * 192, 768
+    assert steps["plain_bytes"] >= 12 * M * H * 36 and steps["act8_bytes"] < 0.47 * steps["plain_bytes"]
+
+
+def test_checkpointed_step_beside_other_work():
+    """a forward without gradients between a training forward and its backward; two backwards into one gradient; the captured step.  Two runs of one step are not
+    the same bits (the heads' products split their sums with atomics), and a last bit that moves there moves 16-bit roundings below it by a step, 2^-7 of
+    single elements: 2 % of a gradient's norm is allowed.  Another batch's activations, a stale checkpoint or a sum taken twice is of order 1."""
+    same = 0.02
+    model, eng = _model(act8=True)
+    images, texts, target = _batch(3, 7)
+    other = _batch(3, 8)
+    model.train()
+    crit = torch.nn.BCEWithLogitsLoss(reduction="mean")
+
+    def backward(between):
+        model.zero_grad(set_to_none=True)
+        _, logits = model("vqa", images, texts)
+        if between:
+            with torch.no_grad():
+                model("vqa", other[0], other[1])
+        (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+        return grads_of(model)
+    a, b = backward(False), backward(True)
+    for n in a:
+        assert _rel(b[n], a[n]) < same or n.endswith("key.bias"), n
+    model.zero_grad(set_to_none=True)
+    model.fused_forward_backward("vqa", images, texts, target)
+    one = grads_of(model)
+    model.fused_forward_backward("vqa", images, texts, target)
+    two = grads_of(model)
+    for n in one:
+        assert _rel(two[n], 2 * one[n]) < same or n.endswith("key.bias"), n
+    model.zero_grad(set_to_none=True)
+    for seed in (7, 9, 7):
+        im, tx, tg = _batch(3, seed)
+        model.zero_grad(set_to_none=True)
+        want = model.fused_forward_backward("vqa", im, tx, tg)[0]
+        gw = grads_of(model)
+        model.zero_grad(set_to_none=True)
+        got = model.graphed_forward_backward("vqa", im, tx, tg)[0]
+        gg = grads_of(model)
+        assert abs(float(got) - float(want)) <= 1e-5 * abs(float(want))
+        for n in gw:
+            assert _rel(gg[n], gw[n]) < same or n.endswith("key.bias"), n
+
+
+def test_frozen_layers_and_optimizer_with_checkpoints():
+    model, eng = _model(act8=True)
+    for n, p in model.named_parameters():
+        if ".embeddings." in n or any(f"encoder.layer.{i}." in n for i in range(9)):
+            p.requires_grad = False
+    images, texts, target = _batch(2, 11)
+    model.train()
+    opt = model.create_optimizer(dict(lr=1e-4, weight_decay=1e-2, adam_epsilon=1e-8)) if False else None
+    model.fused_forward_backward("vqa", images, texts, target)
+    G = grads_of(model)
+    assert not any("encoder.layer.8." in n for n in G) and any("encoder.layer.9." in n for n in G)
+    ref, _ = _model()
+    for n, p in ref.named_parameters():
+        p.requires_grad = not (".embeddings." in n or any(f"encoder.layer.{i}." in n for i in range(9)))
+    ref.train()
+    ref.fused_forward_backward("vqa", images, texts, target)
+    R = grads_of(ref)
+    assert set(R) == set(G)
+    for n in R:
+        if not n.endswith("key.bias"):
+            assert _rel(G[n], R[n]) < 0.08, n
+
+
+def test_act8_refuses_what_it_does_not_cover():
+    model, eng = _model(act8=True)
+    eng.cls_only_last = True
+    images, texts, target = _batch(2, 1)
+    with pytest.raises(NotImplementedError, match="act8"):
+        model.fused_forward_backward("vqa", images, texts, target)
+
+
+def _evaluate(model, images, texts):
+    model.eval()
+    with torch.no_grad():
+        pooled, logits = model("vqa", images, texts)
+    return pooled.cpu(), logits.cpu()
+
+
+def test_int8_evaluation():
+    """tokens and weights in int8: 0.7 % r.m.s. an operand (3 sigma / 127 / sqrt 12), 1 % a product, 48 products of which each adds to a residual stream: a few
+    per cent of the outputs; 10 % allowed"""
+    images, texts, _ = _batch(6, 5)
+    plain, _ = _model()
+    model, eng = _model(eval_i8=True)
+    p0, o0 = _evaluate(plain, images, texts)
+    eng.prof = {"kernel": "linear_i8", "events": []}
+    p1, o1 = _evaluate(model, images, texts)
+    assert len(eng.prof["events"]) == 48          # four products a layer went through the int8 kernels
+    eng.prof = None
+    print("int8 evaluation: pooled %.4f logits %.4f" % (_rel(p1, p0), _rel(o1, o0)))
+    assert 0 < _rel(p1, p0) < 0.1 and _rel(o1, o0) < 0.1
+    # training forwards are untouched, and the codes follow the parameters
+    target = vo.synthetic_vqa_targets(6, seed=5)
+    for m in (plain, model):
+        m.train()
+        m.zero_grad(set_to_none=True)
+    a = plain.fused_forward_backward("vqa", images, texts, target)
+    b = model.fused_forward_backward("vqa", images, texts, target)
+    assert abs(float(a[0]) - float(b[0])) < 1e-5 * abs(float(a[0]))
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if n.endswith("output.dense.weight") or n.endswith("query.weight"):
+                p.mul_(1.5)
+    p2, _ = _evaluate(model, images, texts)
+    fresh, _ = _model(eval_i8=True)
+    fresh.load_state_dict(model.state_dict())
+    p3, _ = _evaluate(fresh, images, texts)
+    assert _rel(p2, p1) > 0.05 and _rel(p2, p3) < 1e-5
+
+
+def test_int8_evaluation_after_an_optimizer_step():
+    """FusedAdamW writes the parameters through the C ABI: the next evaluation multiplies by the new ones"""
+    images, texts, target = _batch(4, 6)
+    model, eng = _model(eval_i8=True)
+    opt = model.create_optimizer({"lr": 1e-2, "weight_decay": 0.0, "adam_epsilon": 1e-8})
+    before, _ = _evaluate(model, images, texts)
+    model.train()
+    model.fused_forward_backward("vqa", images, texts, target)
+    opt.step()
+    opt.zero_grad()
+    after, _ = _evaluate(model, images, texts)
+    fresh, _ = _model(eval_i8=True)
+    fresh.load_state_dict(model.state_dict())
+    want, _ = _evaluate(fresh, images, texts)
+    assert _rel(after, want) < 1e-5 and _rel(after, before) > 1e-3
