@@ -2,6 +2,7 @@
 //   C[m,n] = epi( (sum_k qa[m,k] qb[n,k]) sa[m] sb[n] + bias[n] ),   the sum in int32 (exact: K <= 2^17), everything after it in fp32, rounded once.
 // v_mfma_i32_32x32x32_i8 (twice the 16-bit MFMA rate).  The weights are the MFMA's A operand and the tokens its B operand, so a lane of the accumulator
 // owns ONE token and groups of 4 consecutive channels.
+#include <type_traits>
 #include "rows8.h"
 #include "gemm_bf16_nt.h"
 
@@ -57,8 +58,8 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
                                                                long ldc, int M, int N, int nk, const float* __restrict__ bias, const float* __restrict__ aux,
                                                                long ldaux, int vec) {
   constexpr int NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * BK, LPT = I8Src<BN, NT, BK>::CNT + I8Src<BM, NT, BK>::CNT;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // S stages, then BM token scales
-  float* sas = reinterpret_cast<float*>(smem + S * STAGE);
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // S stages, then the tile's token scales, channel scales and biases
+  float *sas = reinterpret_cast<float*>(smem + S * STAGE), *sbs = sas + BM, *bs = sbs + BN;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wid % WN, wm = wid / WN, half = lane >> 5, l31 = lane & 31;
   int tm, tn;
   const int nbm = (M + BM - 1) / BM, nbn = (N + BN - 1) / BN;
@@ -70,7 +71,14 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   srcA.init(m0, M, lda);
   const signed char* Bp = B + (long)n0 * ldb;
   const signed char* Ap = A + (long)m0 * lda;
-  for (int i = threadIdx.x; i < BM; i += NT) sas[i] = sa[min(m0 + i, M - 1)];
+  // by DMA too, and first: they have landed when the first stage has, and no wait of the epilogue begins with them
+  auto row_dma = [&](const float* __restrict__ src, int i0, int last, float* dst, int n) {
+    for (int c = wid * 64; c < n; c += NT)
+      __builtin_amdgcn_global_load_lds((gbl_void_t*)(src + min(i0 + c + lane, last)), (lds_void_t*)(dst + c), 4, 0, 0);
+  };
+  row_dma(sa, m0, M - 1, sas, BM);
+  row_dma(sb, n0, N - 1, sbs, BN);
+  if (bias) row_dma(bias, n0, N - 1, bs, BN);
 #pragma unroll
   for (int s = 0; s < S; ++s)
     if (s < nk) {
@@ -118,7 +126,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       acc[0][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks & 1][0], fa[ks & 1][0], acc[0][0], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);          // (one MFMA is under way; nothing is out of LDS now, see below)
+      __builtin_amdgcn_sched_barrier(0);          // (one MFMA is under way; nothing is out of LDS now, see above)
       if (ks + 1 < KS) frags(fb[(ks + 1) & 1], fa[(ks + 1) & 1], lbase + cur * STAGE, co[ks + 1]);
       else if (kt + 1 < nk) {
         arrive(min(nk - kt - 2, S - 2));
@@ -148,52 +156,58 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   float sbv[PERIOD][4], bv[PERIOD][4];
 #pragma unroll
   for (int p = 0; p < PERIOD; ++p) {
-    const int n = nw + ((p * 64 + lane) % CPR) * 4;
-    i8_load4(sb + n, sbv[p], N - n, vec);
-    if (bias) i8_load4(bias + n, bv[p], N - n, vec);
-    else
+    const int n = wn * NI * 32 + ((p * 64 + lane) % CPR) * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bv[p][i] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      sbv[p][i] = sbs[n + i];
+      bv[p][i] = bias ? bs[n + i] : 0.f;
+    }
   }
+  // `full`: the whole tile exists and is made of whole pieces, so nothing is tested on the way (tests cut the block into pieces that hipcc does not interleave)
+  auto drain = [&](auto full_) {
+    constexpr bool FULL = decltype(full_)::value;
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) {
+    for (int j = 0; j < MJ; ++j) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<i32x4*>(stage + l31 * PITCH + ((i * 8 + ((2 * g + half) ^ (l31 & 7))) << 4)) =
-            (i32x4){acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-    float rv[EPI == EPI_RESID ? NI * 4 : 1][4];
-    if constexpr (EPI == EPI_RESID) {
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<i32x4*>(stage + l31 * PITCH + ((i * 8 + ((2 * g + half) ^ (l31 & 7))) << 4)) =
+              (i32x4){acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      float rv[EPI == EPI_RESID ? NI * 4 : 1][4];
+      if constexpr (EPI == EPI_RESID) {
+#pragma unroll
+        for (int p = 0; p < NI * 4; ++p) {
+          const int q = p * 64 + lane, m = mw + j * 32 + q / CPR, n = nw + (q % CPR) * 4;
+          i8_load4(aux + (long)m * ldaux + n, rv[p], FULL ? 4 : (m < M ? N - n : 0), FULL || vec);
+        }
+      }
 #pragma unroll
       for (int p = 0; p < NI * 4; ++p) {
-        const int q = p * 64 + lane, m = mw + j * 32 + q / CPR, n = nw + (q % CPR) * 4;
-        i8_load4(aux + (long)m * ldaux + n, rv[p], m < M ? N - n : 0, vec);
+        const int q = p * 64 + lane, r = q / CPR, c = q % CPR, m = mw + j * 32 + r, n = nw + c * 4;
+        const i32x4 a = *reinterpret_cast<const i32x4*>(stage + r * PITCH + (((c & ~7) | ((c ^ r) & 7)) << 4));
+        if (!FULL && (m >= M || n >= N)) continue;
+        const float s = sas[m - m0];
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = fmaf((float)a[i], s * sbv[p % PERIOD][i], bv[p % PERIOD][i]);
+          if (EPI == EPI_GELU) v[i] = gelu_phi<TO>(v[i]);
+          if (EPI == EPI_RESID) v[i] += rv[EPI == EPI_RESID ? p : 0][i];
+        }
+        i8_store4(C + (long)m * ldc + n, v, FULL ? 4 : N - n, FULL || vec);
       }
     }
-#pragma unroll
-    for (int p = 0; p < NI * 4; ++p) {
-      const int q = p * 64 + lane, r = q / CPR, c = q % CPR, m = mw + j * 32 + r, n = nw + c * 4;
-      const i32x4 a = *reinterpret_cast<const i32x4*>(stage + r * PITCH + (((c & ~7) | ((c ^ r) & 7)) << 4));
-      if (m >= M || n >= N) continue;
-      const float s = sas[m - m0];
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = fmaf((float)a[i], s * sbv[p % PERIOD][i], bv[p % PERIOD][i]);
-        if (EPI == EPI_GELU) v[i] = gelu_phi<TO>(v[i]);
-        if (EPI == EPI_RESID) v[i] += rv[EPI == EPI_RESID ? p : 0][i];
-      }
-      i8_store4(C + (long)m * ldc + n, v, N - n, vec);
-    }
-  }
+  };
+  if (vec && m0 + BM <= M && n0 + BN <= N) drain(std::true_type{});
+  else drain(std::false_type{});
 }
 
 template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
 static int i8_launch(const signed char* A, long lda, const float* sa, const signed char* B, long ldb, const float* sb, TO* C, long ldc, int M, int N, int Kp,
                      const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
-  constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + BM * 4;
-  static_assert(LDS * OCC <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * BK, "LDS");
+  constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + (BM + 2 * BN) * 4;
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && LDS * OCC <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * BK, "LDS");
   const long tiles = (long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles >= (1L << 31)) return CLIMB_EUNSUPPORTED;
   auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, BK, S, OCC>;
@@ -210,8 +224,9 @@ static int i8_pick(const signed char* A, long lda, const float* sa, const signed
                    const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
   auto tiles = [&](int bm, int bn) { return (long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
 #define I8_GO(NI_, MJ_, WN_, WM_, BK_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, BK_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
-  if (Kp >= 1536 && tiles(192, 192) >= 192) I8_GO(3, 1, 2, 6, 128, 3, 1);
-  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 64, 3, 2);
+  const long t192 = tiles(192, 192);
+  if (t192 >= 192 && (t192 <= 256 || Kp >= 1536)) I8_GO(3, 1, 2, 6, 128, 3, 1);
+  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 128, 2, 2);
   I8_GO(1, 1, 2, 2, 128, 3, 3);
 #undef I8_GO
 }
@@ -308,6 +323,7 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
   if (y_dtype == CLIMB_DT_F32) static_cast<float*>(y)[(long)m * ldy + n] = v;
   else static_cast<bf16_t*>(y)[(long)m * ldy + n] = f32_to_bf16(v);
 }
+
 static bool i8_few(int M, int K) { return M <= FEW_M && (K + I8_BK - 1) / I8_BK * I8_BK <= 4 * FEW_STEPS * 64; }
 
 extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);

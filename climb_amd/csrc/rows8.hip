@@ -269,7 +269,7 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
 }
 
 // dx = dres + rstd (g - mean_c(g) - xh mean_c(g xh)),  g = dy gamma,  xh = (codes - mean) rstd;  partial column sums {dgamma, dbeta, colsum(dx)} of the
-// workgroup's rows in part[workgroup][3][C], summed by climb_colreduce3 in a fixed order.
+// workgroup's rows in part[workgroup][3][C], summed in a fixed order by the column reduction that follows.
 #define A8LN_WAVES 8
 // rows a wave: three where that still leaves two workgroups a CU (12288 rows: 512), else one -- fewer partial rows against more waves on a short launch
 static inline int a8ln_rpw(int M) { return M >= 8192 ? 3 : 1; }
@@ -280,11 +280,11 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
                                                                       float* dx, long ldo, T* __restrict__ dcast, long ldc, float* __restrict__ part, int M, int C, int rpw) {
   __shared__ __attribute__((aligned(16))) float red[A8LN_WAVES][NV * 256];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  float ag[NV][4], ab[NV][4], as[NV][4], gm[NV][4];
+  constexpr bool KEEP = NV <= 3;          // gamma stays in registers; longer rows (24 columns a lane) have none left and read it twice a row, from L1
+  float ag[NV][4], ab[NV][4], as[NV][4], gm[KEEP ? NV : 1][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * 64 + lane) * 4;
-    row_ld<MODE, 4>(gamma, c, C, gm[i]);
+    if constexpr (KEEP) row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, gm[i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) ag[i][j] = ab[i][j] = as[i][j] = 0.f;
   }
@@ -311,10 +311,11 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
       const bool in = (i * 64 + lane) * 4 < C;
       const float4 xv = act8_unpack4(in ? R.w[i] : 0u, in ? act8_step(R.ex[i]) : 0.f);
       const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
+      if constexpr (!KEEP) row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, gm[0]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {          // (columns past C have d = gamma = 0: no contribution)
         xh[i][j] = (xx[j] - R.mu) * R.rs;
-        const float g = R.d[i][j] * gm[i][j];
+        const float g = R.d[i][j] * gm[KEEP ? i : 0][j];
         s1 += g;
         s2 += g * xh[i][j];
       }
@@ -324,9 +325,10 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
     for (int i = 0; i < NV; ++i) {
       const int c = (i * 64 + lane) * 4, left = C - c;
       float o[4];
+      if constexpr (!KEEP) row_ld<MODE, 4>(gamma, c, C, gm[0]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[j] = R.r[i][j] + R.rs * (R.d[i][j] * gm[i][j] - m1 - xh[i][j] * m2);
+        o[j] = R.r[i][j] + R.rs * (R.d[i][j] * gm[KEEP ? i : 0][j] - m1 - xh[i][j] * m2);
         ag[i][j] += R.d[i][j] * xh[i][j];
         ab[i][j] += R.d[i][j];
         as[i][j] += o[j];
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
   // a row's loads go out before the row in front of it is finished (dx may be dres: rows are disjoint, and a wave reads its row before it writes it); rows of
   // more than 768 columns would need more registers than two waves a SIMD have
   const long row0 = (long)blockIdx.x * rpw * A8LN_WAVES + wid;
-  if constexpr (NV > 3) {
+  if constexpr (!KEEP) {
     for (int rr = 0; rr < rpw && row0 + rr * A8LN_WAVES < M; ++rr) {
       Row A;
       load(A, row0 + rr * A8LN_WAVES);
@@ -391,10 +393,11 @@ static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long
   LAUNCH_CHECK();
   return CLIMB_OK;
 }
+extern "C" int climb_colreduce3(const float* part, long stride, int nblk, float* out0, float* out1, float* out2, int ncols, float beta, void* stream);      // rowwise.hip
 extern "C" int climb_act8_layernorm_bwd_blocks(int M) { return M <= 0 ? 0 : (int)(((long)M + A8LN_WAVES * a8ln_rpw(M) - 1) / (A8LN_WAVES * a8ln_rpw(M))); }
 extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd,
-                                        const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, int M, int C,
-                                        void* stream) {
+                                        const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, float* dgamma, float* dbeta,
+                                        float* colsum, float beta, int M, int C, void* stream) {
   if ((dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) || !ck_ok(q, ldq, e, lde, M, C) || lddy < C || ldo < C || (dres_in && ldr < C) || (dcast && ldc < C))
     return CLIMB_EINVAL;
   if (C > 1536) return CLIMB_EUNSUPPORTED;
@@ -405,6 +408,7 @@ extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, co
 #define LBL(MODE_, T_)                                                                                                                                                   \
   act8_ln_bwd_launch<T_, MODE_>((const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc, \
                                 part, M, C, st)
-  return dtype == CLIMB_DT_F32 ? BY_MODE(mode, LBL, float) : BY_MODE(mode, LBL, bf16_t);
+  const int rc = dtype == CLIMB_DT_F32 ? BY_MODE(mode, LBL, float) : BY_MODE(mode, LBL, bf16_t);
 #undef LBL
+  return rc != CLIMB_OK ? rc : climb_colreduce3(part, 3L * C, climb_act8_layernorm_bwd_blocks(M), dgamma, dbeta, colsum, C, beta, stream);
 }

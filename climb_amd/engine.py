@@ -148,8 +148,7 @@ class Workspace:
             from .rows8 import Checkpoint
             self.ck = [{n: Checkpoint(M, c, (M,), adt, dev) for n, c in (("x", H), ("h1", H), ("xn", H), ("hn", H), ("u", Fd))} for _ in range(L)]
             self.du_a = buf((M, Fd), adt)          # d(gelu output) before x gelu'(checkpoint)
-            self.nln8 = _lib.query_arg("climb_act8_layernorm_bwd_blocks", M)
-            self.part8 = buf((self.nln8 * 3 * H,))
+            self.part8 = buf((_lib.query_arg("climb_act8_layernorm_bwd_blocks", M) * 3 * H,))
             self.wg8_bytes = max(_lib.query_arg("climb_act8_weight_grad_workspace", M, n, H) for n in (3 * H, Fd))
             self.wg8 = torch.empty((max(self.wg8_bytes, 16),), dtype=torch.uint8, device=dev)
         if sp:      # split twins of the fp32 tensors that something besides a GEMM reads too (attention output / gradient, im2col, d(projection))
@@ -538,8 +537,9 @@ class ViltEngine:
 
     def ln_bwd_act8(self, ws, dy, ck, mean, rstd, ln, bias_name, M, H):
         """climb_layernorm_bwd + reduce3 on a checkpoint: the residual gradient ws.dres in place, its 16-bit copy in ws.dres_c"""
-        _lib.call("climb_act8_layernorm_bwd", dy, H, self.adt, *ck._args(), mean, rstd, self.p(ln + ".weight"), ws.dres, H, ws.dres, H, ws.dres_c, H, ws.part8, M, H, _stream())
-        self.reduce3(ws.part8, ws.nln8, H, ln + ".weight", ln + ".bias", bias_name)
+        grads = [self.g(n) if (n is not None and self.requires_grad[n]) else None for n in (ln + ".weight", ln + ".bias", bias_name)]
+        _lib.call("climb_act8_layernorm_bwd", dy, H, self.adt, *ck._args(), mean, rstd, self.p(ln + ".weight"), ws.dres, H, ws.dres, H, ws.dres_c, H, ws.part8, *grads, 1.0, M, H,
+                  _stream())
 
     def dw_act8(self, ws, dY, ck, wname, bname, M, N, K):
         """grad(W)[N, K] += dY^T x, grad(b)[N] += column sums of dY, x from its checkpoint"""

@@ -325,24 +325,24 @@ def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: O
         dres, _, _, ldr = _mat(dres, "dres", cols=C, rows=M, dtype=_F32, dev=dev)
         r = dres.data_ptr()
     acc = dgamma is not None or dbeta is not None
-    new = torch.zeros if acc or M == 0 else torch.empty
+    new = g.new_zeros if acc or M == 0 else g.new_empty
     if dgamma is None:
-        dgamma = new((C,), dtype=_F32, device=dev)
+        dgamma = new(C)
     else:
         _target(dgamma, "dgamma", (C,), _F32, dev)
     if dbeta is None:
-        dbeta = new((C,), dtype=_F32, device=dev)
+        dbeta = new(C)
     else:
         _target(dbeta, "dbeta", (C,), _F32, dev)
-    dx = torch.empty((*ck.lead, C), dtype=_F32, device=dev)
+    dx = g.new_empty((*ck.lead, C))
     if M == 0:
         return dx, dgamma, dbeta
     nblk = _query("climb_act8_layernorm_bwd_blocks", M)
-    part = torch.empty((nblk * 3 * C,), dtype=_F32, device=dev)
+    part = g.new_empty(nblk * 3 * C)
     q, ldq, e, lde = ck._args()
     st = q + ck._stats
-    _launch(dev, "climb_act8_layernorm_bwd", d.data_ptr(), ld, code, q, ldq, e, lde, st, st + 4 * M, g.data_ptr(), r, ldr, dx.data_ptr(), C, 0, 0, part.data_ptr(), M, C)
-    _launch(dev, "climb_colreduce3", part.data_ptr(), 3 * C, nblk, dgamma.data_ptr(), dbeta.data_ptr(), 0, C, 1.0 if acc else 0.0)
+    _launch(dev, "climb_act8_layernorm_bwd", d.data_ptr(), ld, code, q, ldq, e, lde, st, st + 4 * M, g.data_ptr(), r, ldr, dx.data_ptr(), C, 0, 0, part.data_ptr(),
+            dgamma.data_ptr(), dbeta.data_ptr(), 0, 1.0 if acc else 0.0, M, C)
     return dx, dgamma, dbeta
 
 

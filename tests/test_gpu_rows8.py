@@ -197,7 +197,7 @@ def _check_linear(x, w, bias, resid, epi, out_dt, y, s=None):
     assert worst <= 1.0, worst
 
 
-LINEAR = [(1, 768, 768), (1, 16, 17), (2, 100, 33), (15, 768, 96), (16, 2000, 40), (17, 129, 65), (40, 128, 128), (64, 1536, 3129), (185, 768, 768), (200, 77, 130),
+LINEAR = [(1, 768, 768), (7, 5000, 33), (33, 1500, 50), (49, 3200, 17), (64, 4, 5), (12288, 200, 192), (1, 16, 17), (2, 100, 33), (15, 768, 96), (16, 2000, 40), (17, 129, 65), (40, 128, 128), (64, 1536, 3129), (185, 768, 768), (200, 77, 130),
           (333, 640, 1001), (1000, 256, 1100), (2500, 384, 1200)]
 
 

@@ -71,13 +71,13 @@ def test_checkpoint_calls_refuse(mem, change):
     assert _rc("climb_act8_gelu_fwd", a["x"], a["ldx"], a["dtype"], p, 100, *ck, *mc) == EINVAL
     assert _rc("climb_act8_gelu_bwd", a["x"], a["ldx"], a["dtype"], *ck, p, 100, None, 0, *mc) == EINVAL
     assert _rc("climb_act8_layernorm_fwd", p, 100, p, p, 1e-5, a["x"], a["ldx"], a["dtype"], p, p, *ck, *mc) == EINVAL
-    assert _rc("climb_act8_layernorm_bwd", a["x"], a["ldx"], a["dtype"], *ck, p, p, p, None, 0, p, 100, None, 0, p, *mc) == EINVAL
+    assert _rc("climb_act8_layernorm_bwd", a["x"], a["ldx"], a["dtype"], *ck, p, p, p, None, 0, p, 100, None, 0, p, p, p, None, 0.0, *mc) == EINVAL
 
 
 def test_layernorm_refuses_rows_it_cannot_hold(mem):
     p = mem[0]
     assert _rc("climb_act8_layernorm_fwd", p, 1540, p, p, 1e-5, p, 1540, 0, p, p, p, 1552, p, 25, 4, 1540, None) == EUNSUPPORTED
-    assert _rc("climb_act8_layernorm_bwd", p, 1540, 0, p, 1552, p, 25, p, p, p, None, 0, p, 1540, None, 0, p, 4, 1540, None) == EUNSUPPORTED
+    assert _rc("climb_act8_layernorm_bwd", p, 1540, 0, p, 1552, p, 25, p, p, p, None, 0, p, 1540, None, 0, p, p, p, None, 0.0, 4, 1540, None) == EUNSUPPORTED
 
 
 def test_weight_gradient_refuses_and_asks_for_its_workspace(mem):
