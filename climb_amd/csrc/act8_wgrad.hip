@@ -177,12 +177,14 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
     float s[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      float v[V];
-      __builtin_memcpy(v, part + (long)k * NK + i, sizeof(v));
+    for (int k0 = 0; k0 < splits; k0 += 8) {          // eight planes' loads on their way at once; planes past the last are it again, not added
+      float v[8][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[j] += v[j];
+      for (int k = 0; k < 8; ++k) __builtin_memcpy(v[k], part + (long)min(k0 + k, splits - 1) * NK + i, sizeof(v[k]));
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] += k0 + k < splits ? v[k][j] : 0.f;
     }
     const long n = i / K;          // (V divides K: one row)
     float* o = C + n * ldc + (i - n * K);
@@ -204,6 +206,9 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
 //   - expands the codes of tile t + 1 in its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
 //   - meets the workgroup in the second group; behind the barrier the ring slot of tile t takes the DMA of tile t + 5, and the first fragments of tile t + 1
 //     are read under the rest of the group.
+// Measured, 3072 x 768 over 12288 tokens: 72 us (0.81 PFLOP/s) + 14 us of reduction, against 125 + 9 for the 128-tile kernel and 118 us for the vendor library's
+// 16-bit product of the same shape.  Bounded by the loop: its LDS reads (taken out: - 16 us), its MFMAs (33 us at the clock the chip sustains), the expansion (- 8 us)
+// and the final stores (- 7 us) overlap between the two waves of a SIMD only.
 // As in gemm_i8.hip fragments are read behind the first MFMA of the group before, and no load goes to registers: hipcc would wait for all DMA with it.
 #define WB_T 256
 #define WB_BR 32
@@ -404,15 +409,17 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
 
 // The plan of a problem: which kernel, and into how many token ranges the reduction is cut.
 //   small: 128 x 128 tiles, two workgroups a CU, no range below 256 tokens (below that the second launch costs more)
-//   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, and enough tokens for every
-//          CU to have 512 of them
+//   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, tiles for at least 24 CUs, and tokens enough that
+//          every range has 512.  Its partial sums are 256 KB a workgroup whatever the problem, twice what the small tiles write: with fewer tiles (more ranges) that
+//          outweighs the faster loop.  Both kernels with the reduction, us, big / small, N x K over M tokens: 3072 x 768 over 12288 86 / 128, over 4096 47 / 51, over
+//          2048 38 / 34; 2304 x 768 over 12288 70 / 92; 768 x 768 over 12288 52 / 40; 512 x 512 over 12288 43 / 35.
 struct WgPlan { bool big; int splits, rows; long ws; };
 static_assert(WB_LDS <= 160 * 1024, "LDS");
 static WgPlan wgrad_plan(int M, int N, int K, bool aligned) {
   WgPlan p;
   const long bt = (long)((N + WB_T - 1) / WB_T) * ((K + WB_T - 1) / WB_T), st = (long)((N + 127) / 128) * ((K + 127) / 128);
   const long mtiles = ((long)M + WG_BR - 1) / WG_BR, bs = bt <= 256 ? 256 / bt : 1;
-  p.big = aligned && N % 8 == 0 && N >= 256 && K >= 256 && bt <= 256 && bs * bt >= 192 && mtiles >= 8 * bs;
+  p.big = aligned && N % 8 == 0 && bt >= 24 && bt <= 256 && bs * bt >= 192 && mtiles >= 8 * bs;
   long s = 512 / st, most = M / 256;
   s = p.big ? bs : (s < most ? s : most);
   if (s < 1) s = 1;
@@ -435,7 +442,7 @@ extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, 
   if (((uintptr_t)dY & 1) || ((uintptr_t)C & 3) || ((uintptr_t)dbias & 3)) return CLIMB_EINVAL;
   const WgPlan p = wgrad_plan(M, N, K, lddy % 8 == 0 && !((uintptr_t)dY & 15) && lde % 4 == 0 && !((uintptr_t)e & 3) && lddy < (1L << 24) && ldq < (1L << 24));
   const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
-  if (tiles * p.splits >= (1L << 31)) return CLIMB_EUNSUPPORTED;
+  if (tiles * p.splits >= (1L << 24)) return CLIMB_EUNSUPPORTED;          // (a launch holds less than 2^32 threads)
   hipStream_t st = (hipStream_t)stream;
   const bf16_t* dy = (const bf16_t*)dY;
   const signed char* qc = (const signed char*)q;

@@ -1,6 +1,8 @@
 // int8 product with a scale for each token and each output channel:
 //   C[m,n] = epi( (sum_k qa[m,k] qb[n,k]) sa[m] sb[n] + bias[n] ),   the sum in int32 (exact: K <= 2^17), everything after it in fp32, rounded once.
-// v_mfma_i32_32x32x32_i8 (twice the 16-bit MFMA rate).  The weights are the MFMA's A operand and the tokens its B operand, so a lane of the accumulator
+// v_mfma_i32_32x32x32_i8 (twice the 16-bit MFMA rate).  Measured: 12288 x 768 -> 3072 with GELU to 16 bits 53 us (1.09 PFLOP/s; the matrix unit is busy 12 us of it at
+// its peak clock, the epilogue's VALU ~20 us, 85 MB leave and enter HBM in ~15), 12288 x 3072 -> 768 + fp32 residual 40 us (1.45 PFLOP/s).  What bounds it is that these
+// phases of a tile overlap only across the workgroups of a CU, at the 1.9 GHz the chip sustains under MFMA load.  The weights are the MFMA's A operand and the tokens its B operand, so a lane of the accumulator
 // owns ONE token and groups of 4 consecutive channels.
 #include <type_traits>
 #include "rows8.h"
@@ -35,14 +37,14 @@ struct I8Src {
 };
 
 template <typename TO>
-__device__ __forceinline__ void i8_store4(TO* __restrict__ p, const float (&v)[4], int left, bool vec) {
+__device__ __forceinline__ void i8_store4(TO* p, const float (&v)[4], int left, bool vec) {
   if (vec && left >= 4) st4(p, make_float4(v[0], v[1], v[2], v[3]));
   else
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < left) Act<TO>::st(p + i, v[i]);
 }
-__device__ __forceinline__ void i8_load4(const float* __restrict__ p, float (&v)[4], int left, bool vec) {
+__device__ __forceinline__ void i8_load4(const float* p, float (&v)[4], int left, bool vec) {
   if (vec && left >= 4) {
     const float4 r = ld4(p);
     v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
@@ -54,8 +56,8 @@ __device__ __forceinline__ void i8_load4(const float* __restrict__ p, float (&v)
 // WN x WM waves of (32 NI channels) x (32 MJ tokens); S stages in LDS.
 template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
 __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed char* __restrict__ A, long lda, const float* __restrict__ sa,
-                                                               const signed char* __restrict__ B, long ldb, const float* __restrict__ sb, TO* __restrict__ C,
-                                                               long ldc, int M, int N, int nk, const float* __restrict__ bias, const float* __restrict__ aux,
+                                                               const signed char* __restrict__ B, long ldb, const float* __restrict__ sb, TO* C,
+                                                               long ldc, int M, int N, int nk, const float* __restrict__ bias, const float* aux,
                                                                long ldaux, int vec) {
   constexpr int NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * BK, LPT = I8Src<BN, NT, BK>::CNT + I8Src<BM, NT, BK>::CNT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // S stages, then the tile's token scales, channel scales and biases
@@ -209,7 +211,7 @@ static int i8_launch(const signed char* A, long lda, const float* sa, const sign
   constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + (BM + 2 * BN) * 4;
   static_assert(BM % 64 == 0 && BN % 64 == 0 && LDS * OCC <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * BK, "LDS");
   const long tiles = (long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  if (tiles >= (1L << 31)) return CLIMB_EUNSUPPORTED;
+  if (tiles * (64 * WN * WM) >= (1L << 32)) return CLIMB_EUNSUPPORTED;          // (a launch holds less than 2^32 threads)
   auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, BK, S, OCC>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -224,6 +226,9 @@ static int i8_pick(const signed char* A, long lda, const float* sa, const signed
                    const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
   auto tiles = [&](int bm, int bn) { return (long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
 #define I8_GO(NI_, MJ_, WN_, WM_, BK_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, BK_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
+  // 192 x 192 tiles (twelve waves of 32 x 96, one workgroup a CU) where they fill one round of the chip or K is long: 12288 x 3072 -> 768 + residual 40 us (128 x 128:
+  // 49), 12288 x 768 -> 768 + residual 20.5 (23).  128 x 128, two workgroups a CU, one's epilogue beside the other's products: 12288 x 768 -> 3072 45 us (192: 51), with
+  // GELU 54 (63), -> 2304 36 (39).  64 x 64, three a CU, where the larger tiles leave CUs idle: 1024 x 768 -> 768 6.0 us (128: 9.1), 185 x 768 -> 3072 5.9 (9.2).
   const long t192 = tiles(192, 192);
   if (t192 >= 192 && (t192 <= 256 || Kp >= 1536)) I8_GO(3, 1, 2, 6, 128, 3, 1);
   if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 128, 2, 2);
@@ -244,7 +249,7 @@ static int i8_epi(const signed char* A, long lda, const float* sa, const signed 
 extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const void* B, long ldb, const float* sb, void* C, long ldc, int c_dtype, int M, int N, int K,
                                 const float* bias, int epi, const float* aux, long ldaux, void* stream) {
   const int Kp = (K + I8_BK - 1) / I8_BK * I8_BK;
-  if (M < 0 || N <= 0 || K <= 0 || lda < Kp || ldb < Kp || lda % 16 || ldb % 16 || ldc < N || ((uintptr_t)A & 15) || ((uintptr_t)B & 15)) return CLIMB_EINVAL;
+  if (M < 0 || N <= 0 || K <= 0 || M > (1 << 30) || N > (1 << 30) || lda < Kp || ldb < Kp || lda % 16 || ldb % 16 || ldc < N || ((uintptr_t)A & 15) || ((uintptr_t)B & 15)) return CLIMB_EINVAL;
   if (epi != EPI_NONE && epi != EPI_GELU && epi != EPI_RESID) return CLIMB_EINVAL;
   if (epi == EPI_RESID && ldaux < N) return CLIMB_EINVAL;
   if (K > (1 << 17) || lda >= (1L << 22) || ldb >= (1L << 22)) return CLIMB_EUNSUPPORTED;          // int32 sums: 127^2 K < 2^31; 32-bit offsets inside a tile
@@ -261,18 +266,20 @@ extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const 
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
-// y = epi(rows8(x) W^T + bias) for M <= 16 tokens in ONE launch: a workgroup owns 16 channels, quantises the tokens itself (its weights are already on their
+// y = epi(rows8(x) W^T + bias) for M <= 8 tokens in ONE launch: a workgroup owns 16 channels, quantises the tokens itself (its weights are already on their
 // way by then), its four waves share the reduction in 64-byte steps of v_mfma_i32_16x16x64_i8 and add their int32 sums through LDS.  Bound by latency: two
 // dependent trips to memory and the launch.
-#define FEW_M 16
-#define FEW_STEPS 12          // 64-byte steps of a wave: K <= 4 * 12 * 64
+// Against quantising in a launch of its own (768 channels, one / two launches): K = 768: 1 token 3.7 / 6.4 us, 4: 4.1 / 6.6, 8: 5.5 / 6.6, 16: 8.4 / 6.9; K = 3072:
+// 7.3 / 12.7, 8.5 / 13.0, 13.3 / 13.1, 22.6 / 13.2 -- every workgroup quantises every token, so eight is where it stops paying.
+#define FEW_M 8
+#define FEW_STEPS 12          // 64-byte steps of a wave, held in registers: K <= 4 * 12 * 64
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict__ x, long ldx, const signed char* __restrict__ W, long ldw, const float* __restrict__ sw,
-                                                            void* __restrict__ y, long ldy, int y_dtype, int M, int N, int K, int Kp, const float* __restrict__ bias,
+                                                            void* y, long ldy, int y_dtype, int M, int N, int K, int Kp, const float* __restrict__ bias,
                                                             int epi, const float* aux, long ldaux) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // codes [16][Kp + 16], sums [4][16][17], scales [16]
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // codes [16][Kp + 16] (8 rows written), sums [4][16][17], scales [16]
   const int pitch = Kp + 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, n0 = blockIdx.x * 16;
-  int* red = reinterpret_cast<int*>(smem + FEW_M * pitch);
+  int* red = reinterpret_cast<int*>(smem + 16 * pitch);
   float* sc = reinterpret_cast<float*>(red + 4 * 16 * 17);
   const int steps = Kp / 64;
   i32x4 wf[FEW_STEPS];
@@ -305,14 +312,14 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
   i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < FEW_STEPS; ++i)
-    if (wave + 4 * i < steps) {          // (rows M .. 15 of the image are whatever LDS held: their columns of the result are not read)
+    if (wave + 4 * i < steps) {          // (rows M .. 15 of the image are whatever LDS held: integers all the same, and their columns of the result are not read)
       const i32x4 tf = *reinterpret_cast<const i32x4*>(smem + l15 * pitch + (wave + 4 * i) * 64 + (lane >> 4) * 16);
       acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], tf, acc, 0, 0, 0);
     }
 #pragma unroll
   for (int i = 0; i < 4; ++i) red[(wave * 16 + (lane >> 4) * 4 + i) * 17 + l15] = acc[i];
   __syncthreads();
-  const int m = threadIdx.x >> 4, n = n0 + l15;
+  const int m = threadIdx.x >> 4, n = n0 + l15;          // (16 x 16 results, rows M .. 15 are not there)
   if (m >= M || n >= N) return;
   int sum = 0;
 #pragma unroll
@@ -328,12 +335,12 @@ static bool i8_few(int M, int K) { return M <= FEW_M && (K + I8_BK - 1) / I8_BK 
 
 extern "C" int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);
 extern "C" long climb_linear_i8_workspace(int M, int K) {
-  if (M < 0 || K <= 0) return CLIMB_EINVAL;
+  if (M < 0 || M > (1 << 30) || K <= 0 || K > (1 << 17)) return CLIMB_EINVAL;
   return i8_few(M, K) ? 0 : (long)M * ((K + I8_BK - 1) / I8_BK * I8_BK + 4);
 }
 extern "C" int climb_linear_i8(const void* x, long ldx, int dtype, const void* W, long ldw, const float* sw, void* y, long ldy, int y_dtype, int M, int N, int K,
                                const float* bias, int epi, const float* aux, long ldaux, void* workspace, long workspace_bytes, void* stream) {
-  if (M < 0 || N <= 0 || K <= 0 || K > (1 << 17) || ldx < K || (dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) || (y_dtype != CLIMB_DT_F32 && y_dtype != CLIMB_DT_BF16))
+  if (M < 0 || N <= 0 || K <= 0 || M > (1 << 30) || N > (1 << 27) || K > (1 << 17) || ldx < K || (dtype != CLIMB_DT_F32 && dtype != CLIMB_DT_BF16) || (y_dtype != CLIMB_DT_F32 && y_dtype != CLIMB_DT_BF16))
     return K > (1 << 17) ? CLIMB_EUNSUPPORTED : CLIMB_EINVAL;
   const int Kp = (K + I8_BK - 1) / I8_BK * I8_BK;
   if (ldw < Kp || ldw % 16 || ((uintptr_t)W & 15) || ldy < N || (epi != EPI_NONE && epi != EPI_GELU && epi != EPI_RESID) || (epi == EPI_RESID && ldaux < N)) return CLIMB_EINVAL;
@@ -341,7 +348,7 @@ extern "C" int climb_linear_i8(const void* x, long ldx, int dtype, const void* W
   if (M == 0) return CLIMB_OK;
   if (!x || !W || !sw || !y || (epi == EPI_RESID && !aux)) return CLIMB_EINVAL;
   if (i8_few(M, K)) {
-    const int lds = FEW_M * (Kp + 16) + (4 * 16 * 17 + 16) * 4;
+    const int lds = 16 * (Kp + 16) + (4 * 16 * 17 + 16) * 4;
     const dim3 grid((N + 15) / 16), blk(256);
     hipStream_t st = (hipStream_t)stream;
 #define FEW(T_, MODE_) \

@@ -226,7 +226,7 @@ def test_linear_leading_dims_codes_out_and_residual_in_place(dev):
     _check_linear(x, w, None, None, "none", torch.float32, y.view(42, 50))
     codes = rows8.quantize_rows(d3)
     assert torch.equal(rows8.linear_i8(codes, w8), y)                       # shared codes: the same bits ...
-    assert torch.equal(rows8.linear_i8(d[:9], w8), y.view(42, 50)[:9])      # ... and few tokens in their one launch
+    assert torch.equal(rows8.linear_i8(d[:8], w8), y.view(42, 50)[:8])      # ... and few tokens in their one launch
     wide = torch.full((42, 60), 5.0, device="cuda")
     res = torch.randn(42, 50, generator=torch.Generator().manual_seed(3))
     wide[:, 4:54] = res.cuda()
@@ -268,7 +268,7 @@ def test_tensor_call_refusals_on_the_gpu(dev):
 
 # ------------------------------------------------------------------------------------------------ weight gradient
 WGRAD = [(1, 1, 1), (1, 768, 40), (3, 17, 130), (63, 64, 64), (64, 1536, 3129), (65, 129, 127), (185, 768, 768), (511, 100, 200), (512, 33, 77), (700, 384, 260), (3000, 200, 90),
-         (12288, 130, 140), (8195, 1000, 1288), (4097, 768, 2304), (12290, 1536, 768)]
+         (12288, 130, 140), (8195, 1000, 1288), (4097, 768, 2304), (12290, 1536, 768), (4609, 768, 2304), (12290, 1536, 1024)]
 
 
 @pytest.mark.parametrize("M,K,N", WGRAD)
@@ -435,6 +435,23 @@ def test_gradients_against_differences(dev):
         num = (((xd @ (w + p).t()) - (xd @ (w - p).t())) * h.double()).sum() / 2e-3
         assert abs(float(num) - float(dw[n, k])) < 1e-4
     assert (dw.cpu().double() - h.double().t() @ xd).abs().max() < 1e-4
+
+
+def test_broadcast_gradients(dev):
+    """a gradient that is a broadcast view (all rows, or all columns, one number in memory) gives what its copy gives"""
+    from climb_amd import rows8
+    M, C, N = 40, 96, 64
+    _, x = _make(M, C, torch.float32, 1)
+    g, b = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    _, ck = rows8.layernorm_fwd(x, g, b, 1e-5)
+    _, uk = rows8.gelu_fwd(x)
+    for view in (torch.randn(1, C, device="cuda").expand(M, C), torch.randn(M, 1, device="cuda").expand(M, C), torch.randn((), device="cuda").expand(M, C)):
+        for got, want in zip(rows8.layernorm_bwd(view, ck, g, dres=view), rows8.layernorm_bwd(view.contiguous(), ck, g, dres=view.contiguous())):
+            assert torch.equal(got, want)
+        assert torch.equal(rows8.gelu_bwd(view, uk), rows8.gelu_bwd(view.contiguous(), uk))
+    dy = torch.randn(1, N, device="cuda").to(_h16()).expand(M, N)
+    for got, want in zip(rows8.weight_grad(dy, uk), rows8.weight_grad(dy.contiguous(), uk)):
+        assert torch.equal(got, want)
 
 
 # ------------------------------------------------------------------------------------------------ as they are used together

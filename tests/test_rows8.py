@@ -97,6 +97,18 @@ def test_weight_gradient_refuses_and_asks_for_its_workspace(mem):
     assert call(nbytes=need - 1) == EINVAL
 
 
+def test_sizes_beyond_a_launch_are_refused(mem):
+    p = mem[0]
+    big = (1 << 30) + 1
+    assert _rc("climb_rows8_quant", p, 64, 0, p, 128, p, big, 64, None) == EINVAL
+    assert _rc("climb_rows8_quant", p, 64, 0, p, 128, p, 1 << 28, 64, None) == EUNSUPPORTED
+    assert _rc("climb_act8_save", p, 64, 0, p, 64, p, 1, 1 << 29, 64, None) == EUNSUPPORTED
+    assert _rc("climb_act8_gelu_fwd", p, 64, 0, p, 64, p, 64, p, 1, 1 << 29, 64, None) == EUNSUPPORTED
+    assert _rc("climb_act8_layernorm_fwd", p, 64, p, p, 1e-5, p, 64, 0, p, p, p, 64, p, 1, 1 << 26, 64, None) == EUNSUPPORTED
+    assert _rc("climb_gemm_i8_nt", p, 128, p, p, 128, p, p, 1 << 20, 0, 1 << 24, 1 << 20, 64, None, 0, None, 0, None) == EUNSUPPORTED
+    assert _rc("climb_act8_weight_grad", p, 1 << 20, p, 1 << 20, p, 1 << 14, p, 1 << 20, None, 64, 1 << 20, 1 << 20, 0.0, p, 1 << 60, None) == EUNSUPPORTED
+
+
 def test_nothing_is_launched_for_no_rows():
     z = (0, 64, None)
     assert _rc("climb_rows8_quant", None, 64, 0, None, 128, None, *z) == 0

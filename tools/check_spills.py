@@ -7,7 +7,11 @@ import re
 import subprocess
 import sys
 
-CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "climb_amd", "csrc")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from climb_amd.build import FLAGS          # what the library is built with: other flags allocate other registers
+
+CSRC = os.path.join(ROOT, "climb_amd", "csrc")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # kernels whose spills are a measured trade (see their comments): attention backward phase 1 (168-VGPR cap keeps 3 workgroups per CU),
 # the 192x192 GEMM with the fp32 residual / adapter dual-residual operand prefetched (a few dwords, outside the k-loop),
@@ -16,14 +20,15 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # epilogue itself no longer spills: r03, the lane id is recomputed per tile instead of kept across the k-loop);
 # the grouped weight-gradient launch with the optimizer in its epilogue (r04): 13 dwords of per-lane constants (fragment offsets, lane ids) stored once
 # before the item loop and reloaded once per TILE (192 k-tiles each), none inside the k-loop;
+# the four-wave NT GEMM with the gelu' epilogue that only CLIMB_AMD_GELU_SAVE=pre selects (seven dwords since packed fp32 arithmetic is off);
 # bench.py's pipe-only diagnostic (16 accumulator tiles = all 256 AGPRs + 256 VGPRs at one wave per SIMD: one dword outside its MFMA loop)
 KNOWN = ("gemm_bf16_ntsk_kernelIfLi2E", "attn_bwd_bf16_kernelILi1E", "attn_bwd_bf16_fused_kernel", "gemm_bf16_nt192_kernelIfLi2E", "gemm_bf16_nt192_kernelItLi2E", "gemm_bf16_nt192_kernelIfLi7E",
          "gemm_bf16_nt192_kernelItLi7E", "gemm_f32_kernelILi128ELi128ELb1E",
-         "gemm_bf16_nt2_kernelIfLi2E", "gemm_bf16_nt2_kernelItLi2E", "mfma_sustained_kernel", "gemm_bf16_tn_grouped_kernelILb0ELb1E")
+         "gemm_bf16_nt2_kernelIfLi2E", "gemm_bf16_nt2_kernelItLi2E", "gemm_bf16_nt4_kernelItLi3E", "mfma_sustained_kernel", "gemm_bf16_tn_grouped_kernelILb0ELb1E")
 
 
 def report(path):
-    cmd = [HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Rpass-analysis=kernel-resource-usage", "-c", path, "-o", os.devnull]
+    cmd = [HIPCC] + FLAGS + ["-Rpass-analysis=kernel-resource-usage", "-c", path, "-o", os.devnull]
     err = subprocess.run(cmd, capture_output=True, text=True).stderr
     out = []
     name = vgpr = None
