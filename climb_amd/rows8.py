@@ -37,7 +37,7 @@ class RowCodes:
 
     def __init__(self, rows: int, cols: int, lead: Tuple[int, ...], device: torch.device):
         self.rows, self.cols, self.ld, self.lead, self.device = rows, cols, _up(cols, 128), lead, device
-        self.buf = torch.empty((rows * (self.ld + 4),), dtype=torch.int8, device=device)
+        self.buf = torch.empty(rows * (self.ld + 4), dtype=torch.int8, device=device)
 
     @property
     def q(self) -> torch.Tensor:
@@ -62,7 +62,7 @@ class Checkpoint:
         self.lead, self.dtype, self.device = lead, dtype, device
         n = rows * (self.ld + self.groups)
         self._stats = _up(n, 16) if stats else 0          # byte offset of mean [rows], rstd [rows]
-        self.buf = torch.empty((self._stats + 8 * rows if stats else n,), dtype=torch.uint8, device=device)
+        self.buf = torch.empty(self._stats + 8 * rows if stats else n, dtype=torch.uint8, device=device)
 
     @property
     def q(self) -> torch.Tensor:
@@ -176,6 +176,11 @@ def _mat(x: torch.Tensor, what: str, cols: Optional[int] = None, rows: Optional[
     return x, M, C, ld
 
 
+def _like(x: torch.Tensor, shape) -> torch.Tensor:
+    """an empty contiguous tensor of x's dtype (empty_like is the cheapest of torch's allocations)"""
+    return torch.empty_like(x) if x.shape == shape and x.is_contiguous() else x.new_empty(shape)
+
+
 def _vec(x: torch.Tensor, what: str, n: int, dev: torch.device) -> torch.Tensor:
     x, M, C, ld = _mat(x, what, dtype=_F32, dev=dev)
     if M * C != n:
@@ -236,7 +241,7 @@ def linear_i8(x: Union[torch.Tensor, RowCodes], w: RowCodes, bias: Optional[torc
     if out is None:
         dt = out_dtype or dt
         ycode = _code(dt)
-        y, ldy = torch.empty((*lead, N), dtype=dt, device=dev), N
+        y, ldy = (m.new_empty((*lead, N)) if not codes and dt is m.dtype else torch.empty((*lead, N), dtype=dt, device=dev)), N
     else:
         y, dt = out, out_dtype or out.dtype
         ycode, ldy = _code(dt), _target(out, "out", (*lead, N), dt, dev)
@@ -254,7 +259,7 @@ def linear_i8(x: Union[torch.Tensor, RowCodes], w: RowCodes, bias: Optional[torc
         _launch(dev, "climb_gemm_i8_nt", xp, x.ld, xp + M * x.ld, wp, w.ld, wp + N * w.ld, y.data_ptr(), ldy, ycode, M, N, K, b, e, r, ldr)
     else:
         nb = _query("climb_linear_i8_workspace", M, K)
-        ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb > 0 else None
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
         _launch(dev, "climb_linear_i8", m.data_ptr(), ldx, xcode, wp, w.ld, wp + N * w.ld, y.data_ptr(), ldy, ycode, M, N, K, b, e, r, ldr,
                 ws.data_ptr() if nb > 0 else 0, nb)
     return y
@@ -289,7 +294,7 @@ def weight_grad(dy: torch.Tensor, ck: Checkpoint, dw: Optional[torch.Tensor] = N
     elif bias:
         dbias = new((N,), dtype=_F32, device=dev)
     nb = _query("climb_act8_weight_grad_workspace", M, N, K)
-    ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb > 0 else None
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
     _launch(dev, "climb_act8_weight_grad", d.data_ptr(), ld, *ck._args(), dw.data_ptr(), ldw, dbias.data_ptr() if dbias is not None else 0, M, N, K, beta,
             ws.data_ptr() if nb > 0 else 0, nb)
     return dw, dbias
@@ -303,7 +308,7 @@ def layernorm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps:
     dev, dt = m.device, out_dtype or _F32
     code = _code(dt)
     g, b = _vec(gamma, "gamma", C, dev), _vec(beta, "beta", C, dev)
-    y = torch.empty(x.shape, dtype=dt, device=dev)
+    y = _like(x, x.shape) if dt is _F32 else torch.empty(x.shape, dtype=dt, device=dev)
     ck = Checkpoint(M, C, tuple(x.shape[:-1]), _F32, dev, stats=True)
     q, ldq, e, lde = ck._args()
     st = q + ck._stats
@@ -334,7 +339,7 @@ def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: O
         dbeta = new(C)
     else:
         _target(dbeta, "dbeta", (C,), _F32, dev)
-    dx = g.new_empty((*ck.lead, C))
+    dx = _like(g if dres is None else dres, (*ck.lead, C))
     if M == 0:
         return dx, dgamma, dbeta
     nblk = _query("climb_act8_layernorm_bwd_blocks", M)
@@ -350,7 +355,7 @@ def gelu_fwd(u: torch.Tensor) -> Tuple[torch.Tensor, Checkpoint]:
     """a = gelu(u) (erf form) in u's dtype, and the checkpoint of u."""
     m, M, C, ld = _mat(u, "u")
     code = _code(m.dtype)
-    a = torch.empty(u.shape, dtype=m.dtype, device=m.device)
+    a = _like(u, u.shape)
     ck = Checkpoint(M, C, tuple(u.shape[:-1]), m.dtype, m.device)
     _launch(m.device, "climb_act8_gelu_fwd", m.data_ptr(), ld, code, a.data_ptr(), C, *ck._args(), M, C)
     return a, ck
@@ -361,7 +366,7 @@ def gelu_bwd(da: torch.Tensor, ck: Checkpoint, recompute: bool = False):
     dev, M, C = ck.device, ck.rows, ck.cols
     d, _, _, ld = _mat(da, "da", cols=C, rows=M, dev=dev)
     code = _code(d.dtype)
-    du = torch.empty((*ck.lead, C), dtype=d.dtype, device=dev)
+    du = _like(d, (*ck.lead, C))
     a = torch.empty_like(du) if recompute else None
     _launch(dev, "climb_act8_gelu_bwd", d.data_ptr(), ld, code, *ck._args(), du.data_ptr(), C, a.data_ptr() if recompute else 0, C, M, C)
     return (du, a) if recompute else du
