@@ -226,18 +226,16 @@ __device__ __forceinline__ bf16x8 wb_frag(const unsigned char* __restrict__ p) {
   c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * WB_PITCH));
   return c.b;
 }
-// 16 codes -> 16 numbers of the operand type.  Offset binary: byte ^ 128 is code + 128 in 0 .. 255, one conversion, and one fma takes the offset out (exact)
+// 16 codes -> 16 numbers of the operand type (a signed byte is one conversion, its multiple of the step one exact product)
 __device__ __forceinline__ void wb_expand(u32x4 q, unsigned e4, bool live, unsigned char* __restrict__ Bs) {
   const int row = threadIdx.x >> 4, c16 = threadIdx.x & 15;
-  const float step = live ? act8_step((e4 >> ((c16 >> 2) * 8)) & 255u) : 0.f, off = -128.f * step;
+  const float step = live ? act8_step((e4 >> ((c16 >> 2) * 8)) & 255u) : 0.f;
   unsigned h[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned w = q[i] ^ 0x80808080u;
-    const float a = fmaf((float)(w & 255u), step, off), b = fmaf((float)((w >> 8) & 255u), step, off);
-    const float c = fmaf((float)((w >> 16) & 255u), step, off), d = fmaf((float)(w >> 24), step, off);
-    h[2 * i] = pack_bf16x2(a, b);
-    h[2 * i + 1] = pack_bf16x2(c, d);
+    const float4 v = act8_unpack4(q[i], step);
+    h[2 * i] = pack_bf16x2(v.x, v.y);
+    h[2 * i + 1] = pack_bf16x2(v.z, v.w);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -430,17 +428,17 @@ static WgPlan wgrad_plan(int M, int N, int K, bool aligned) {
   return p;
 }
 extern "C" long climb_act8_weight_grad_workspace(int M, int N, int K) {
-  if (M < 0 || M > (1 << 30) || N <= 0 || K <= 0) return CLIMB_EINVAL;
+  if (M < 0 || M > (1 << 30) || N <= 0 || N > (1 << 30) || K <= 0 || K > (1 << 30)) return CLIMB_EINVAL;
   const long a = wgrad_plan(M, N, K, true).ws, b = wgrad_plan(M, N, K, false).ws;          // (alignments are not known here)
   return a > b ? a : b;
 }
 extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, long ldq, const void* e, long lde, float* C, long ldc, float* dbias, int M, int N, int K,
                                       float beta, void* workspace, long workspace_bytes, void* stream) {
-  if (M < 0 || M > (1 << 30) || N <= 0 || K <= 0 || lddy < N || ldc < K || ldq < K || ldq % 16 || ((uintptr_t)q & 15) || lde < (K + ACT8_GROUP - 1) / ACT8_GROUP || !C)
+  if (M < 0 || M > (1 << 30) || N <= 0 || N > (1 << 30) || K <= 0 || K > (1 << 30) || lddy < N || ldc < K || ldq < K || ldq % 16 || ((uintptr_t)q & 15) || lde < (K + ACT8_GROUP - 1) / ACT8_GROUP || !C)
     return CLIMB_EINVAL;
   if (M > 0 && (!dY || !q || !e)) return CLIMB_EINVAL;
   if (((uintptr_t)dY & 1) || ((uintptr_t)C & 3) || ((uintptr_t)dbias & 3)) return CLIMB_EINVAL;
-  const WgPlan p = wgrad_plan(M, N, K, lddy % 8 == 0 && !((uintptr_t)dY & 15) && lde % 4 == 0 && !((uintptr_t)e & 3) && lddy < (1L << 24) && ldq < (1L << 24));
+  const WgPlan p = wgrad_plan(M, N, K, lddy % 8 == 0 && !((uintptr_t)dY & 15) && lde % 4 == 0 && !((uintptr_t)e & 3) && lddy < (1L << 24) && ldq < (1L << 24) && lde < (1L << 24));
   const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
   if (tiles * p.splits >= (1L << 24)) return CLIMB_EUNSUPPORTED;          // (a launch holds less than 2^32 threads)
   hipStream_t st = (hipStream_t)stream;

@@ -215,6 +215,21 @@ def test_linear(dev, M, K, N, xn, yn, epi):
     _check_linear(x, w, bias, resid, epi, _dt(yn), y)
 
 
+# every tile size of the product, whole and ragged: 256 tiles of 192 x 192 in one round; more of them with a long reduction; 128 x 128; 64 x 64
+@pytest.mark.parametrize("M,K,N", [(12288, 130, 768), (12101, 256, 581), (10000, 1600, 800), (10000, 200, 800), (1000, 260, 777)])
+@pytest.mark.parametrize("epi", ["none", "gelu", "resid"])
+def test_linear_tiles(dev, M, K, N, epi):
+    from climb_amd import rows8
+    g = torch.Generator().manual_seed(M + K)
+    x, w, bias = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g) * 0.05, torch.randn(N + 1, generator=g)[1:]
+    resid = torch.randn(M, N, generator=g) if epi == "resid" else None
+    out_dtype = torch.float32 if epi == "resid" else _h16()
+    b = torch.zeros(N + 1, device="cuda")[1:]          # (a base that is aligned to its element only)
+    b.copy_(bias)
+    y = rows8.linear_i8(x.cuda(), rows8.quantize_rows(w.cuda()), b, epi=epi, resid=resid.cuda() if resid is not None else None, out_dtype=out_dtype)
+    _check_linear(x, w, bias, resid, epi, out_dtype, y)
+
+
 def test_linear_leading_dims_codes_out_and_residual_in_place(dev):
     from climb_amd import rows8
     x, d = _make(6 * 7, 96, torch.float32, 1)
@@ -316,6 +331,26 @@ def test_weight_gradient_keeps_nan_in_its_columns(dev):
     dw, db = rows8.weight_grad(dd, rows8.checkpoint_save(d))
     nan = torch.isnan(dw).any(0)
     assert nan[64:128].all() and not nan[:64].any() and not nan[128:].any() and not torch.isnan(db).any()
+
+
+@pytest.mark.parametrize("M,K,N", [(100, 200, 50), (4609, 768, 2304)])
+def test_weight_gradient_of_the_largest_numbers(dev, M, K, N):
+    """groups whose step is 2^121 or 2^122 (fp32 numbers next to the top of the range): 128 steps are beyond fp32, the values are not"""
+    from climb_amd import rows8
+    x, _ = _make(M, K, torch.float32, 20)
+    x[5, 3], x[7, 3], x[9, 70], x[M - 1, K - 1] = 3.3e38, -1.6e38, -3.4e38, 2.0e38
+    x[11] = torch.linspace(-1.0, 1.0, K) * 3e38
+    dy = _make(M, N, _h16(), 21)[0]
+    dy[[5, 7, 9, 11, M - 1]] = 2.0 ** -14
+    _, _, v = ref_checkpoint(x, _h16() is torch.float16)
+    dw, _ = rows8.weight_grad(dy.cuda(), rows8.checkpoint_save(x.cuda()))
+    if _h16() is torch.float16:          # (numbers beyond 65504 are infinite operands: zero codes stay zeros, columns without such a number stay finite)
+        v = torch.where(v.abs() > 65504, torch.sign(v) * math.inf, v)
+        finite = torch.isfinite(v).all(0)
+        assert torch.isfinite(dw.cpu()[:, finite]).all() and not torch.isfinite(dw.cpu()[:, ~finite]).any()
+        return
+    ref, mag = dy.double().t() @ v, dy.double().abs().t() @ v.abs()
+    assert ((dw.cpu().double() - ref).abs() <= 2 * (M + 16) * U * mag + 1e-30).all()
 
 
 # ------------------------------------------------------------------------------------------------ LayerNorm and GELU
@@ -529,6 +564,93 @@ def test_captured_and_replayed_beside_eager_work(dev):
             torch.cuda.synchronize()
             for a, b in zip(outs, want):
                 assert torch.equal(a, b)
+
+
+def test_large_products_captured_without_a_run_before(dev):
+    """the kernels that ask for more than 64 KB of LDS, first called inside a capture; replayed three times beside eager work"""
+    from climb_amd import rows8
+    M, K, N = 12290, 768, 768
+    x, dy = torch.randn(M, K, device="cuda"), torch.randn(M, 3 * N, device="cuda").to(_h16())
+    w8, ck = rows8.quantize_rows(torch.randn(N, K, device="cuda")), rows8.checkpoint_save(x)
+    codes = rows8.quantize_rows(x)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = rows8.linear_i8(codes, w8)
+        dw, db = rows8.weight_grad(dy, ck)
+    for rep in range(3):
+        dy.copy_(torch.randn(M, 3 * N, device="cuda"))
+        want = (rows8.linear_i8(codes, w8), *rows8.weight_grad(dy, ck))
+        gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((y, dw, db), want):
+            assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(dev):
+    """matrices of more than 2^32 elements: the last rows come out as they do alone"""
+    from climb_amd import rows8
+    M, C, t = 5_600_000, 768, 40
+    assert M * C > 2 ** 32
+    tail = torch.randn(t, C, device="cuda")
+    h = torch.zeros(M, C, dtype=_h16(), device="cuda")
+    h[-t:] = tail.to(_h16())
+    last = h[-t:].clone()
+    codes, few = rows8.quantize_rows(h), rows8.quantize_rows(last)
+    assert torch.equal(codes.q[-t:], few.q) and torch.equal(codes.scale[-t:], few.scale)
+    w8 = rows8.quantize_rows(torch.randn(900, C, device="cuda"))
+    y = rows8.linear_i8(codes, w8, epi="gelu", out_dtype=_h16())          # [M, 900]
+    assert torch.equal(y[-t:], rows8.linear_i8(few, w8, epi="gelu", out_dtype=_h16()))
+    del codes, y
+    a, ck = rows8.gelu_fwd(h)
+    a1, ck1 = rows8.gelu_fwd(last)
+    assert torch.equal(a[-t:], a1) and torch.equal(ck.q[-t:], ck1.q) and torch.equal(ck.exps[-t:], ck1.exps)
+    assert torch.equal(ck.load()[-t:], ck1.load())
+    du, a2 = rows8.gelu_bwd(h, ck, recompute=True)
+    du1, a3 = rows8.gelu_bwd(last, ck1, recompute=True)
+    assert torch.equal(du[-t:], du1) and torch.equal(a2[-t:], a3)
+    del a, du, a2
+    for N in (64, 2304):          # both kernels of the weight gradient; rows of zeros add nothing
+        d = torch.zeros(M, N, dtype=_h16(), device="cuda")
+        d[-t:] = torch.randn(t, N, device="cuda").to(_h16())
+        dw, db = rows8.weight_grad(d, ck)
+        dw1, db1 = rows8.weight_grad(d[-t:], ck1)
+        mag = d[-t:].float().abs().t() @ ck1.load(torch.float32).abs()
+        assert ((dw - dw1).abs() <= 4 * (t + 16) * U * mag).all()          # two orders of at most t + 16 additions
+        assert ((db - db1).abs() <= 4 * (t + 16) * U * d[-t:].float().abs().sum(0)).all()
+        del d
+    del h, ck
+    x = torch.zeros(M, C, device="cuda")
+    x[-t:] = tail
+    g, b = torch.rand(C, device="cuda") + 0.5, torch.randn(C, device="cuda")
+    y, ck = rows8.layernorm_fwd(x, g, b, 1e-5, out_dtype=_h16())
+    y1, ck1 = rows8.layernorm_fwd(tail, g, b, 1e-5, out_dtype=_h16())
+    assert torch.equal(y[-t:], y1) and torch.equal(ck.q[-t:], ck1.q) and torch.equal(ck.rstd[-t:], ck1.rstd)
+    dx, _, _ = rows8.layernorm_bwd(y, ck, g, dres=x)
+    assert torch.equal(dx[-t:], rows8.layernorm_bwd(y1, ck1, g, dres=tail)[0])
+
+
+def test_rows_that_are_not_numbers_stay_in_their_rows(dev):
+    """LayerNorm and GELU of rows with a NaN or an infinity: those rows' gradients are NaN where their groups are, the other rows' bits stay as they were"""
+    from climb_amd import rows8
+    M, C = 50, 200
+    _, x = _make(M, C, torch.float32, 30)
+    _, dy = _make(M, C, torch.float32, 31)
+    g, b = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    clean_y, ck = rows8.layernorm_fwd(x, g, b, 1e-5)
+    clean_dx = rows8.layernorm_bwd(dy, ck, g)[0]
+    clean_du = rows8.gelu_bwd(dy, rows8.gelu_fwd(x)[1])
+    x[3, 70], x[44, 199] = float("nan"), float("inf")
+    keep = torch.ones(M, dtype=torch.bool, device="cuda")
+    keep[[3, 44]] = False
+    y, ck = rows8.layernorm_fwd(x, g, b, 1e-5)
+    dx, dg, _ = rows8.layernorm_bwd(dy, ck, g)
+    for got, want in ((y, clean_y), (dx, clean_dx)):
+        assert torch.equal(got[keep], want[keep]) and torch.isnan(got[~keep]).all()
+    assert torch.isnan(dg).all()
+    du = rows8.gelu_bwd(dy, rows8.gelu_fwd(x)[1])
+    bad = torch.zeros(M, C, dtype=torch.bool, device="cuda")
+    bad[3, 64:128] = bad[44, 192:] = True
+    assert torch.isnan(du[bad]).all() and torch.equal(du[~bad], clean_du[~bad])
 
 
 def test_two_streams_at_once(dev):

@@ -87,6 +87,7 @@ def test_weight_gradient_refuses_and_asks_for_its_workspace(mem):
     assert need > 0 and need % (4 * (96 * 100 + 96)) == 0
     assert _rc("climb_act8_weight_grad_workspace", 100, 96, 100) == 0          # one token range: straight into C
     assert _rc("climb_act8_weight_grad_workspace", -1, 96, 100) == EINVAL
+    assert _rc("climb_act8_weight_grad_workspace", 64, 2 ** 31 - 1, 100) == EINVAL and _rc("climb_act8_weight_grad_workspace", 64, 96, 2 ** 31 - 1) == EINVAL
 
     def call(nbytes=need, **change):
         a = dict(ok, **change)
