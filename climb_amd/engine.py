@@ -840,6 +840,7 @@ class ViltEngine:
             ws = self.workspace(B, T, gh, gw, nseq, tag="nograd")
         st = _stream()
         adt = self.adt
+        self._i8_pass = False          # (a forward that raised may have left it on)
         self.refresh_shadow()
         e = ENC + "embeddings."
         ws.img_type.copy_(img_type)
@@ -870,6 +871,8 @@ class ViltEngine:
         prune = self.cls_only_last and ad is None
         odt = self.odt
         act8 = self.act8 and save
+        if (act8 or self.eval_i8) and self.precision != "bf16":
+            raise NotImplementedError(f"act8 / eval_i8 in {'bf16x3' if self.split else 'fp32'}: 8-bit rows go with the 16-bit operand types")
         if act8 and (ad is not None or prune):
             raise NotImplementedError("8-bit activation checkpoints (act8) with an active adapter or cls_only_last")
         self._i8_pass = ws if (self.eval_i8 and not save and not prune) else False

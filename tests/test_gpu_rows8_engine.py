@@ -173,6 +173,39 @@ def test_act8_refuses_what_it_does_not_cover():
         model.fused_forward_backward("vqa", images, texts, target)
 
 
+def test_8_bit_rows_go_with_the_16_bit_types():
+    if H16 == "fp16":
+        pytest.skip("one process, one 16-bit type")
+    images, texts, target = _batch(2, 1)
+    for flag in ("act8", "eval_i8"):
+        model, _ = make_model(["vqa"], 42, precision="fp32")
+        setattr(model._host.engine(), flag, True)
+        with pytest.raises(NotImplementedError, match="16-bit"):
+            model.fused_forward_backward("vqa", images, texts, target)
+
+
+def test_a_forward_that_raised_leaves_no_trace(monkeypatch):
+    """an evaluation that ends in the middle of the encoder: the next training step is the plain one"""
+    images, texts, target = _batch(3, 2)
+    plain, _ = _model()
+    model, eng = _model(eval_i8=True)
+    attn = type(eng).attn_fwd
+    def fail(*a, **k):
+        raise KeyboardInterrupt
+    monkeypatch.setattr(type(eng), "attn_fwd", fail)
+    with pytest.raises(KeyboardInterrupt):
+        _evaluate(model, images, texts)
+    monkeypatch.setattr(type(eng), "attn_fwd", attn)
+    for m in (plain, model):
+        m.train()
+    a, b = (m.fused_forward_backward("vqa", images, texts, target) for m in (plain, model))
+    assert abs(float(a[0]) - float(b[0])) < 1e-5 * abs(float(a[0]))
+    p, _ = _evaluate(model, images, texts)
+    fresh, _ = _model(eval_i8=True)
+    want, _ = _evaluate(fresh, images, texts)
+    assert _rel(p, want) < 1e-5
+
+
 def _evaluate(model, images, texts):
     model.eval()
     with torch.no_grad():
