@@ -13,18 +13,18 @@ typedef __attribute__((ext_vector_type(16))) int i32x16;
 
 #define I8_BK 128          // the code rows are whole 128-byte pieces
 
-// LDS image of an operand tile: [rows][BK bytes], 16-byte chunk c of row r at position c ^ i8_swz(r): the 16 rows that a fragment read (16 bytes a lane, 32 rows
+// LDS image of an operand tile: [rows][128 bytes], 16-byte chunk c of row r at position c ^ i8_swz(r): the 16 rows that a fragment read (16 bytes a lane, 32 rows
 // of one chunk) takes in a cycle lie in 16 different 16-byte slots of the 256-byte bank line.  global_load_lds writes LDS linearly, so the swizzle is applied to the
 // SOURCE address.
-template <int BK> __device__ __forceinline__ int i8_swz(int row) { return BK == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
-template <int ROWS, int NT, int BK>
+__device__ __forceinline__ int i8_swz(int row) { return (row >> 1) & 7; }
+template <int ROWS, int NT>
 struct I8Src {
-  static constexpr int CPR = BK / 16, CNT = ROWS * CPR / NT;
+  static constexpr int CPR = I8_BK / 16, CNT = ROWS * CPR / NT;
   unsigned off[CNT];          // per lane: byte offsets from the tile's first row
   __device__ __forceinline__ void init(int row0, int R, long ld) {
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      const int slot = i * NT + threadIdx.x, row = slot / CPR, c = (slot % CPR) ^ i8_swz<BK>(row);
+      const int slot = i * NT + threadIdx.x, row = slot / CPR, c = (slot % CPR) ^ i8_swz(row);
       off[i] = (unsigned)(min(row, R - 1 - row0) * (unsigned)ld) + c * 16;          // rows past the end repeat the last one: their results are not stored
     }
   }
@@ -54,12 +54,12 @@ __device__ __forceinline__ void i8_load4(const float* p, float (&v)[4], int left
 }
 
 // WN x WM waves of (32 NI channels) x (32 MJ tokens); S stages in LDS.
-template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
+template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int S, int OCC>
 __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed char* __restrict__ A, long lda, const float* __restrict__ sa,
                                                                const signed char* __restrict__ B, long ldb, const float* __restrict__ sb, TO* C,
                                                                long ldc, int M, int N, int nk, const float* __restrict__ bias, const float* aux,
                                                                long ldaux, int vec) {
-  constexpr int NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * BK, LPT = I8Src<BN, NT, BK>::CNT + I8Src<BM, NT, BK>::CNT;
+  constexpr int BK = I8_BK, NT = 64 * WN * WM, BN = 32 * NI * WN, BM = 32 * MJ * WM, STAGE = (BN + BM) * BK, LPT = I8Src<BN, NT>::CNT + I8Src<BM, NT>::CNT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // S stages, then the tile's token scales, channel scales and biases
   float *sas = reinterpret_cast<float*>(smem + S * STAGE), *sbs = sas + BM, *bs = sbs + BN;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wid % WN, wm = wid / WN, half = lane >> 5, l31 = lane & 31;
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   const int nbm = (M + BM - 1) / BM, nbn = (N + BN - 1) / BN;
   nt_tile<8>(nbm, nbn, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  I8Src<BN, NT, BK> srcB;
-  I8Src<BM, NT, BK> srcA;
+  I8Src<BN, NT> srcB;
+  I8Src<BM, NT> srcA;
   srcB.init(n0, N, ldb);
   srcA.init(m0, M, lda);
   const signed char* Bp = B + (long)n0 * ldb;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   const unsigned char* lbase = smem + l31 * BK;
   unsigned co[KS];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) co[ks] = ((ks * 2 + half) ^ i8_swz<BK>(l31)) << 4;
+  for (int ks = 0; ks < KS; ++ks) co[ks] = ((ks * 2 + half) ^ i8_swz(l31)) << 4;
   auto frags = [&](i32x4(&b)[NI], i32x4(&a)[MJ], const unsigned char* buf, unsigned c) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) b[i] = *reinterpret_cast<const i32x4*>(buf + (wn * NI + i) * 32 * BK + c);
@@ -205,14 +205,14 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   else drain(std::false_type{});
 }
 
-template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int BK, int S, int OCC>
+template <typename TO, int EPI, int NI, int MJ, int WN, int WM, int S, int OCC>
 static int i8_launch(const signed char* A, long lda, const float* sa, const signed char* B, long ldb, const float* sb, TO* C, long ldc, int M, int N, int Kp,
                      const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
-  constexpr int BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + (BM + 2 * BN) * 4;
+  constexpr int BK = I8_BK, BN = 32 * NI * WN, BM = 32 * MJ * WM, LDS = S * (BN + BM) * BK + (BM + 2 * BN) * 4;
   static_assert(BM % 64 == 0 && BN % 64 == 0 && LDS * OCC <= 160 * 1024 && WN * WM * NI * 4096 <= S * (BN + BM) * BK, "LDS");
   const long tiles = (long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles * (64 * WN * WM) >= (1L << 32)) return CLIMB_EUNSUPPORTED;          // (a launch holds less than 2^32 threads)
-  auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, BK, S, OCC>;
+  auto k = gemm_i8_kernel<TO, EPI, NI, MJ, WN, WM, S, OCC>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return (int)e;
@@ -225,14 +225,14 @@ template <typename TO, int EPI>
 static int i8_pick(const signed char* A, long lda, const float* sa, const signed char* B, long ldb, const float* sb, TO* C, long ldc, int M, int N, int Kp,
                    const float* bias, const float* aux, long ldaux, int vec, hipStream_t st) {
   auto tiles = [&](int bm, int bn) { return (long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-#define I8_GO(NI_, MJ_, WN_, WM_, BK_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, BK_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
+#define I8_GO(NI_, MJ_, WN_, WM_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
   // 192 x 192 tiles (twelve waves of 32 x 96, one workgroup a CU) where they fill one round of the chip or K is long: 12288 x 3072 -> 768 + residual 40 us (128 x 128:
   // 49), 12288 x 768 -> 768 + residual 20.5 (23).  128 x 128, two workgroups a CU, one's epilogue beside the other's products: 12288 x 768 -> 3072 45 us (192: 51), with
   // GELU 54 (63), -> 2304 36 (39).  64 x 64, three a CU, where the larger tiles leave CUs idle: 1024 x 768 -> 768 6.0 us (128: 9.1), 185 x 768 -> 3072 5.9 (9.2).
   const long t192 = tiles(192, 192);
-  if (t192 >= 192 && (t192 <= 256 || Kp >= 1536)) I8_GO(3, 1, 2, 6, 128, 3, 1);
-  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 128, 2, 2);
-  I8_GO(1, 1, 2, 2, 128, 3, 3);
+  if (t192 >= 192 && (t192 <= 256 || Kp >= 1536)) I8_GO(3, 1, 2, 6, 3, 1);
+  if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 2, 2);
+  I8_GO(1, 1, 2, 2, 3, 3);
 #undef I8_GO
 }
 template <typename TO>
@@ -256,8 +256,7 @@ extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const 
   if (M == 0) return CLIMB_OK;
   if (!A || !sa || !B || !sb || !C || (epi == EPI_RESID && !aux)) return CLIMB_EINVAL;
   // whole 16-byte (16-bit C: 8-byte) pieces of 4 channels; anything else is read and written element by element
-  const int vec = ldc % 4 == 0 && !((uintptr_t)C & 15) && !((uintptr_t)sb & 15) && !((uintptr_t)bias & 15) &&
-                  (epi != EPI_RESID || (ldaux % 4 == 0 && !((uintptr_t)aux & 15)));
+  const int vec = ldc % 4 == 0 && !((uintptr_t)C & 15) && (epi != EPI_RESID || (ldaux % 4 == 0 && !((uintptr_t)aux & 15)));
   hipStream_t st = (hipStream_t)stream;
   const signed char *a = (const signed char*)A, *b = (const signed char*)B;
   if (c_dtype == CLIMB_DT_F32) return i8_epi<float>(a, lda, sa, b, ldb, sb, (float*)C, ldc, M, N, Kp, bias, epi, aux, ldaux, vec, st);
