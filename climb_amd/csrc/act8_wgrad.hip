@@ -1,6 +1,7 @@
 // Weight gradient of a linear layer whose input was kept as an 8-bit checkpoint (rows8.h):
 //   C[n,k] = beta C[n,k] + sum_m dY[m,n] code[m,k] 2^e(m, k / 64),      dbias[n] = beta dbias[n] + sum_m dY[m,n]
 // on the 16-bit MFMA.  code * 2^e is a number of the operand type, so the codes are expanded ONCE, on their way into LDS, and no product is rounded.
+#include <type_traits>
 #include "rows8.h"
 #include "gemm_bf16_nt.h"
 
@@ -8,19 +9,6 @@
 #define WG_PITCH 256        // bytes of an LDS row: 128 columns
 __device__ __forceinline__ int wg_swz(int row) { return (row & 3) << 2; }      // the 4 token rows of a transpose read lie in 4 different bank quarters
 
-// 16 bytes from any address (the hardware reads unaligned words; hipcc makes one load of it), elements past `left` zero
-__device__ __forceinline__ u32x4 wg_ld16(const bf16_t* __restrict__ p, int left) {
-  u32x4 r = (u32x4){0u, 0u, 0u, 0u};
-  if (left >= 8) __builtin_memcpy(&r, p, 16);
-  else if (left > 0) {
-    unsigned short h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) h[i] = p[i];
-    __builtin_memcpy(&r, h, 16);
-  }
-  return r;
-}
 // 8-token MFMA operand of output index col0 + (lane & 31), tokens mrow0 + (lane >> 5) * 8 + 0..7: two transpose reads
 __device__ __forceinline__ bf16x8 wg_frag(const unsigned char* __restrict__ S, int mrow0, int col0, int lane) {
   const int g16 = lane >> 4, i = lane & 15, row = mrow0 + (g16 >> 1) * 8 + (i >> 2), col = col0 + (g16 & 1) * 16 + 4 * (i & 3);
@@ -36,24 +24,51 @@ struct WgStage {
   u32x4 a[4], b[2];          // 8 gradients x 4 token rows, 16 codes x 2 token rows
   unsigned e[2];
 };
+// The loads of a tile go out together, all of them unconditional (a load under a condition is waited for inside it): tokens past the end are read as the last
+// one, pieces past the last column as the last piece; wg_store puts them right, or their results are not stored.  Any address: the hardware reads unaligned words.
+// MODE 1: N % 8 == 0;  0: N >= 8, the piece that crosses the end is the row's last 8 columns, shifted down;  2: shorter rows, element by element.
+template <int MODE>
 __device__ __forceinline__ void wg_load(WgStage& s, const bf16_t* __restrict__ dY, long lddy, const signed char* __restrict__ q, long ldq,
                                         const unsigned char* __restrict__ e, long lde, int m0, int mend, int n0, int N, int k0, int K) {
   const int t = threadIdx.x;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const int m = m0 + (t >> 4) + 16 * p, n = n0 + (t & 15) * 8;
-    s.a[p] = wg_ld16(dY + (long)m * lddy + n, m < mend ? N - n : 0);
+    const int m = min(m0 + (t >> 4) + 16 * p, mend - 1), n = n0 + (t & 15) * 8;
+    if constexpr (MODE == 2) {
+      unsigned short h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = dY[(long)m * lddy + min(n + i, N - 1)];
+      __builtin_memcpy(&s.a[p], h, 16);
+    } else {
+      __builtin_memcpy(&s.a[p], dY + (long)m * lddy + min(n, N - 8), 16);
+    }
   }
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    const int m = m0 + (t >> 3) + 32 * p, k = k0 + (t & 7) * 16;
-    const bool ok = m < mend && k < K;          // (a piece that starts inside the row lies inside ldq; tokens past the end are zero codes of step 2^0)
-    s.b[p] = ok ? *reinterpret_cast<const u32x4*>(q + (long)m * ldq + k) : (u32x4){0u, 0u, 0u, 0u};
-    s.e[p] = ok ? e[(long)m * lde + (k >> 6)] : 127u;
+    const int m = min(m0 + (t >> 3) + 32 * p, mend - 1), k = min(k0 + (t & 7) * 16, (K - 1) & ~15);          // (a piece that starts inside the row lies inside ldq)
+    s.b[p] = *reinterpret_cast<const u32x4*>(q + (long)m * ldq + k);
+    s.e[p] = e[(long)m * lde + (k >> 6)];
   }
 }
-__device__ __forceinline__ void wg_store(const WgStage& s, unsigned char* __restrict__ As, unsigned char* __restrict__ Bs) {
+template <int MODE>
+__device__ __forceinline__ void wg_store(WgStage& s, unsigned char* __restrict__ As, unsigned char* __restrict__ Bs, int left, int n0, int N) {
   const int t = threadIdx.x;
+  if (MODE == 0 && n0 + 128 > N) {
+    const int d = max(n0 + (t & 15) * 8 - (N - 8), 0);          // (8 and more: a piece past the end)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      u32x4 v = s.a[p];
+      if (d & 4) { v[0] = v[2]; v[1] = v[3]; }
+      if (d & 2) { v[0] = v[1]; v[1] = v[2]; v[2] = v[3]; }
+      if (d & 1) { v[0] = __builtin_amdgcn_alignbit(v[1], v[0], 16); v[1] = __builtin_amdgcn_alignbit(v[2], v[1], 16); v[2] = __builtin_amdgcn_alignbit(v[3], v[2], 16); v[3] >>= 16; }
+      s.a[p] = v;
+    }
+  }
+  if (left < WG_BR) {          // tokens past the end: gradients 0 (an infinity must not meet a zero code, and the bias sums run over all rows), codes of step 0
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      if ((t >> 4) + 16 * p >= left) s.a[p] = (u32x4){0u, 0u, 0u, 0u};
+  }
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int row = (t >> 4) + 16 * p;
@@ -62,7 +77,7 @@ __device__ __forceinline__ void wg_store(const WgStage& s, unsigned char* __rest
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const int row = (t >> 3) + 32 * p;
-    const float step = act8_step(s.e[p]);
+    const float step = row < left ? act8_step(s.e[p]) : 0.f;
     unsigned h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -78,7 +93,7 @@ __device__ __forceinline__ void wg_store(const WgStage& s, unsigned char* __rest
 
 // One workgroup: a 128 (n) x 128 (k) tile over the tokens [split * rows, + rows).  Four waves of 64 x 64.  PART: the sums go to `out` = [split][N * K]
 // (and [split][N] for the bias behind them) for act8_wgrad_reduce_kernel, which adds them in the order of the splits; else straight into C.
-template <bool PART>
+template <bool PART, int MODE>
 __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restrict__ dY, long lddy, const signed char* __restrict__ q, long ldq,
                                                          const unsigned char* __restrict__ e, long lde, float* __restrict__ out, long ldc, float* __restrict__ dbias,
                                                          int M, int N, int K, int rows, int splits, float beta) {
@@ -106,11 +121,11 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restric
   for (int i = 0; i < 8; ++i) bs[i] = 0.f;
   WgStage st;
   const int nt = (mend - mbeg + WG_BR - 1) / WG_BR;
-  if (nt > 0) wg_load(st, dY, lddy, q, ldq, e, lde, mbeg, mend, n0, N, k0, K);
+  if (nt > 0) wg_load<MODE>(st, dY, lddy, q, ldq, e, lde, mbeg, mend, n0, N, k0, K);
   for (int t = 0; t < nt; ++t) {
     unsigned char* As = smem + (t & 1) * (2 * WG_BR * WG_PITCH);
     unsigned char* Bs = As + WG_BR * WG_PITCH;
-    wg_store(st, As, Bs);
+    wg_store<MODE>(st, As, Bs, mend - mbeg - t * WG_BR, n0, N);
     if (do_bias) {
 #pragma unroll
       for (int p = 0; p < 4; ++p)
@@ -120,7 +135,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restric
           bs[2 * i + 1] += h16hi_to_f32(st.a[p][i]);
         }
     }
-    if (t + 1 < nt) wg_load(st, dY, lddy, q, ldq, e, lde, mbeg + (t + 1) * WG_BR, mend, n0, N, k0, K);
+    if (t + 1 < nt) wg_load<MODE>(st, dY, lddy, q, ldq, e, lde, mbeg + (t + 1) * WG_BR, mend, n0, N, k0, K);
     __syncthreads();          // (two buffers: the next store goes to the one that every wave has left by then)
 #pragma unroll
     for (int ms = 0; ms < WG_BR / 16; ++ms) {
@@ -135,23 +150,33 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restric
         for (int j = 0; j < 2; ++j) acc[i][j] = CLIMB_MFMA_H16(fa[i], fb[j], acc[i][j], 0, 0, 0);
     }
   }
-  // a wave instruction writes 2 rows of 32 consecutive floats
+  // a wave instruction writes 2 rows of 32 consecutive floats; old values are fetched 16 at a time, unconditionally (a place past the end: the last one)
   float* o = PART ? out + (long)split * N * K : out;
   const long ld = PART ? K : ldc;
+  const bool acc_c = !PART && beta != 0.f;
+  auto put = [&](auto full_) {
+    constexpr bool FULL = decltype(full_)::value;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int k = k0 + wk * 64 + j * 32 + l31;
+      for (int j = 0; j < 2; ++j) {
+        const int k = k0 + wk * 64 + j * 32 + l31;
+        float old[16];
+        if (acc_c) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-        if (n < N && k < K) {
-          float* p = o + (long)n * ld + k;
-          *p = (!PART && beta != 0.f) ? fmaf(beta, *p, acc[i][j][r]) : acc[i][j][r];
+          for (int r = 0; r < 16; ++r) old[r] = o[(long)min(n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half, N - 1) * ld + min(k, K - 1)];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(beta, old[r], acc[i][j][r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          if (FULL || (n < N && k < K)) o[(long)n * ld + k] = acc[i][j][r];
         }
       }
-    }
+  };
+  if (n0 + 128 <= N && k0 + 128 <= K) put(std::true_type{});
+  else put(std::false_type{});
   if (do_bias) {          // 16 threads a column group of 8: through LDS, added in a fixed order
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);          // [16][128]
@@ -226,7 +251,7 @@ __device__ __forceinline__ bf16x8 wb_frag(const unsigned char* __restrict__ p) {
   c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * WB_PITCH));
   return c.b;
 }
-// 16 codes -> 16 numbers of the operand type (a signed byte is one conversion, its multiple of the step one exact product)
+// 16 codes -> 16 numbers of the operand type
 __device__ __forceinline__ void wb_expand(u32x4 q, unsigned e4, bool live, unsigned char* __restrict__ Bs) {
   const int row = threadIdx.x >> 4, c16 = threadIdx.x & 15;
   const float step = live ? act8_step((e4 >> ((c16 >> 2) * 8)) & 255u) : 0.f;
@@ -384,17 +409,22 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
     unsigned char* x = img; img = img1; img1 = x;
   }
   float* o = out + (long)split * N * K;
+  auto put = [&](auto full_) {
+    constexpr bool FULL = decltype(full_)::value;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = k0 + wk * 128 + j * 32 + l31;
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + wk * 128 + j * 32 + l31;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-        if (n < N && k < K) o[(long)n * K + k] = acc[i][j][r];
+        for (int r = 0; r < 16; ++r) {
+          const int n = n0 + wn * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          if (FULL || (n < N && k < K)) o[(long)n * K + k] = acc[i][j][r];
+        }
       }
-    }
+  };
+  if (n0 + WB_T <= N && k0 + WB_T <= K) put(std::true_type{});
+  else put(std::false_type{});
   if (want_bias && wk == 0) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -445,8 +475,16 @@ extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, 
   const bf16_t* dy = (const bf16_t*)dY;
   const signed char* qc = (const signed char*)q;
   const unsigned char* ec = (const unsigned char*)e;
+#define WGL(PART_, MODE_, G_, O_, LD_, ...) \
+  hipLaunchKernelGGL((act8_wgrad_kernel<PART_, MODE_>), G_, dim3(256), 0, st, dy, lddy, qc, ldq, ec, lde, O_, LD_, dbias, M, N, K, __VA_ARGS__)
+#define WGS(PART_, ...)                               \
+  do {                                                \
+    if (N % 8 == 0) WGL(PART_, 1, __VA_ARGS__);       \
+    else if (N > 8) WGL(PART_, 0, __VA_ARGS__);       \
+    else WGL(PART_, 2, __VA_ARGS__);                  \
+  } while (0)
   if (p.ws == 0) {
-    hipLaunchKernelGGL((act8_wgrad_kernel<false>), dim3((unsigned)tiles), dim3(256), 0, st, dy, lddy, qc, ldq, ec, lde, C, ldc, dbias, M, N, K, M > 0 ? M : 1, 1, beta);
+    WGS(false, dim3((unsigned)tiles), C, ldc, M > 0 ? M : 1, 1, beta);
     LAUNCH_CHECK();
     return CLIMB_OK;
   }
@@ -461,8 +499,10 @@ extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, 
     hipLaunchKernelGGL(act8_wgrad_big_kernel, dim3((N + WB_T - 1) / WB_T * nbk * p.splits), dim3(512), lds, st, dy, lddy, qc, ldq, ec, lde, ws, dbias != nullptr, M, N, K, p.rows,
                        p.splits);
   } else {
-    hipLaunchKernelGGL((act8_wgrad_kernel<true>), dim3((unsigned)(tiles * p.splits)), dim3(256), 0, st, dy, lddy, qc, ldq, ec, lde, ws, K, dbias, M, N, K, p.rows, p.splits, 0.f);
+    WGS(true, dim3((unsigned)(tiles * p.splits)), ws, K, p.rows, p.splits, 0.f);
   }
+#undef WGS
+#undef WGL
   LAUNCH_CHECK();
   const bool v4 = K % 4 == 0 && ldc % 4 == 0;
   const long pieces = ((long)N * K / (v4 ? 4 : 1) + 255) / 256;

@@ -44,9 +44,13 @@ __device__ __forceinline__ unsigned act8_pack4(float a, float b, float c, float 
   const unsigned r = __builtin_amdgcn_perm(ub, ua, 0x0c0c0400u) | __builtin_amdgcn_perm(ud, uc, 0x04000c0cu);
   return e == ACT8_BAD ? 0u : r;
 }
+// ... and back: byte ^ 128 is code + 128 in 0 .. 255, put in the low byte of 2^23 and taken off again (one byte permute and one subtraction at full rate, where a
+// conversion is slower), then one exact product
 __device__ __forceinline__ float4 act8_unpack4(unsigned w, float step) {
-  return make_float4((float)(signed char)(w & 255u) * step, (float)(signed char)((w >> 8) & 255u) * step, (float)(signed char)((w >> 16) & 255u) * step,
-                     (float)(signed char)(w >> 24) * step);
+  const unsigned u = w ^ 0x80808080u;
+  const float off = 8388736.f;          // 2^23 + 128
+  return make_float4((__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060500u)) - off) * step, (__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060501u)) - off) * step,
+                     (__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060502u)) - off) * step, (__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060503u)) - off) * step);
 }
 
 // Phi(-|x|) = exp(-x^2 / 2) R(1 / (1 + p |x|)), R a polynomial without constant term fitted to erfcx(|x| / sqrt 2) / 2 on [0, 14] for the smallest largest
