@@ -93,6 +93,7 @@ __device__ __forceinline__ void wg_store(WgStage& s, unsigned char* __restrict__
 
 // One workgroup: a 128 (n) x 128 (k) tile over the tokens [split * rows, + rows).  Four waves of 64 x 64.  PART: the sums go to `out` = [split][N * K]
 // (and [split][N] for the bias behind them) for act8_wgrad_reduce_kernel, which adds them in the order of the splits; else straight into C.
+// Bound by latency on few tokens (768 x 768 over 185: 7.5 us, 36 workgroups with three tiles each one after the other), by the expansion on many.
 template <bool PART, int MODE>
 __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restrict__ dY, long lddy, const signed char* __restrict__ q, long ldq,
                                                          const unsigned char* __restrict__ e, long lde, float* __restrict__ out, long ldc, float* __restrict__ dbias,
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
 //   - expands the codes of tile t + 1 in its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
 //   - meets the workgroup in the second group; behind the barrier the ring slot of tile t takes the DMA of tile t + 5, and the first fragments of tile t + 1
 //     are read under the rest of the group.
-// Measured, 3072 x 768 over 12288 tokens: 72 us (0.81 PFLOP/s) + 14 us of reduction, against 125 + 9 for the 128-tile kernel and 118 us for the vendor library's
+// Measured, 3072 x 768 over 12288 tokens: 70 us (0.83 PFLOP/s) + 14 us of reduction, against 109 for the 128-tile kernel with its own and 118 us for the vendor library's
 // 16-bit product of the same shape.  Bounded by the loop: its LDS reads (taken out: - 16 us), its MFMAs (33 us at the clock the chip sustains), the expansion (- 8 us)
 // and the final stores (- 7 us) overlap between the two waves of a SIMD only.
 // As in gemm_i8.hip fragments are read behind the first MFMA of the group before, and no load goes to registers: hipcc would wait for all DMA with it.
@@ -438,16 +439,17 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
 // The plan of a problem: which kernel, and into how many token ranges the reduction is cut.
 //   small: 128 x 128 tiles, two workgroups a CU, no range below 256 tokens (below that the second launch costs more)
 //   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, tiles for at least 24 CUs, and tokens enough that
-//          every range has 512.  Its partial sums are 256 KB a workgroup whatever the problem, twice what the small tiles write: with fewer tiles (more ranges) that
-//          outweighs the faster loop.  Both kernels with the reduction, us, big / small, N x K over M tokens: 3072 x 768 over 12288 86 / 128, over 4096 47 / 51, over
-//          2048 38 / 34; 2304 x 768 over 12288 70 / 92; 768 x 768 over 12288 52 / 40; 512 x 512 over 12288 43 / 35.
+//          every range has 768.  Its partial sums are 256 KB a workgroup whatever the problem, twice what the small tiles write: with fewer tiles (more ranges) that
+//          outweighs the faster loop.  Both kernels with the reduction, us, big / small, N x K over M tokens: 3072 x 768 over 12288 85 / 109, over 4096 47 / 44, over
+//          2048 39 / 31; 2304 x 768 over 12288 70 / 79; 768 x 768 over 12288 58 / 38; 512 x 512 over 12288 60 / 31.
+// Ranges of 128 tokens in place of 256 (small): 2304 x 768 over 400 20 us (12), 768 x 768 over 1024 20 (15), 260 x 384 over 700 12 (14).
 struct WgPlan { bool big; int splits, rows; long ws; };
 static_assert(WB_LDS <= 160 * 1024, "LDS");
 static WgPlan wgrad_plan(int M, int N, int K, bool aligned) {
   WgPlan p;
   const long bt = (long)((N + WB_T - 1) / WB_T) * ((K + WB_T - 1) / WB_T), st = (long)((N + 127) / 128) * ((K + 127) / 128);
   const long mtiles = ((long)M + WG_BR - 1) / WG_BR, bs = bt <= 256 ? 256 / bt : 1;
-  p.big = aligned && N % 8 == 0 && bt >= 24 && bt <= 256 && bs * bt >= 192 && mtiles >= 8 * bs;
+  p.big = aligned && N % 8 == 0 && bt >= 24 && bt <= 256 && bs * bt >= 192 && mtiles >= 12 * bs;
   long s = 512 / st, most = M / 256;
   s = p.big ? bs : (s < most ? s : most);
   if (s < 1) s = 1;

@@ -333,7 +333,7 @@ def test_weight_gradient_keeps_nan_in_its_columns(dev):
     assert nan[64:128].all() and not nan[:64].any() and not nan[128:].any() and not torch.isnan(db).any()
 
 
-@pytest.mark.parametrize("M,K,N", [(100, 200, 50), (4609, 768, 2304)])
+@pytest.mark.parametrize("M,K,N", [(100, 200, 50), (4609, 768, 2304), (7000, 768, 2304)])
 def test_weight_gradient_of_the_largest_numbers(dev, M, K, N):
     """groups whose step is 2^121 or 2^122 (fp32 numbers next to the top of the range): 128 steps are beyond fp32, the values are not"""
     from climb_amd import rows8
