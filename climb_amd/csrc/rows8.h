@@ -209,7 +209,23 @@ __device__ __forceinline__ unsigned rowq(float x, float s, float rs) {
 __device__ __forceinline__ float row_scale(unsigned mx) {
   return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
 }
+// Four codes.  |x| / s <= 127, so x * rs is within 127 * 2^-24 < 2^-17 of the quotient, and its distance from the nearest integer is off by less than 2^-25 more: only where
+// that distance comes within 2^-16 of a half can the exact quotient round to the other side, and only a wave that holds such a one (0.8 % of the calls on random
+// numbers) takes the exact steps.  Row codes of 12288 x 3072 in 16 bits 20 us, 22 with the exact steps for all.
 __device__ __forceinline__ unsigned rowq4(const float (&v)[4], float s, float rs, bool bad) {
-  const unsigned w = __builtin_amdgcn_perm(rowq(v[1], s, rs), rowq(v[0], s, rs), 0x0c0c0400u) | __builtin_amdgcn_perm(rowq(v[3], s, rs), rowq(v[2], s, rs), 0x04000c0cu);
+  const float magic = 12582912.f;
+  unsigned k[4];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float u = fmaf(v[i], rs, magic);
+    k[i] = __float_as_uint(u);
+    far = fmaxf(far, fabsf(fmaf(v[i], rs, magic - u)));
+  }
+  if (__any(far > 0.5f - 0x1p-16f)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = rowq(v[i], s, rs);
+  }
+  const unsigned w = __builtin_amdgcn_perm(k[1], k[0], 0x0c0c0400u) | __builtin_amdgcn_perm(k[3], k[2], 0x04000c0cu);
   return bad ? 0u : w;
 }
