@@ -1,8 +1,8 @@
 // Row-wise kernels of the 8-bit formats (rows8.h): row codes for the int8 product, checkpoints, and the LayerNorm and GELU that write a checkpoint in
 // their forward and read it in their backward.  All are bound by HBM (a 1 GiB copy runs at 5.1 TB/s, one of 64 MiB, which the Infinity Cache holds, at 8.1); each input
-// is read once and each output written once.  Measured, 16-bit data unless said: row codes 12288 x 3072 22 us (5.1 TB/s; before the loads of a row went out together
-// 29), 12288 x 768 9.2 us; LayerNorm 12288 x 768 forward 13.5 us (4.9 TB/s), backward 20.8 us (5.0); GELU 12288 x 3072 forward 32 us (5.8), backward with the activation
-// 48 us (5.5); a checkpoint of 12288 x 768 6.3 us.
+// is read once and each output written once.  Measured, 16-bit data unless said: row codes 12288 x 3072 19 - 21 us (5.4 - 5.9 TB/s; before the loads of a row went out
+// together 29), 12288 x 768 8.1 us; LayerNorm 12288 x 768 forward 13.5 us (4.9 TB/s), backward 20.8 us (5.0); GELU 12288 x 3072 forward 32 us (5.8), backward with the activation
+// 47 us (5.6); a checkpoint of 12288 x 768 6.3 us.
 #include "rows8.h"
 
 // the launcher of a row_mode
