@@ -277,69 +277,87 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
 #define A8LN_WAVES 8
 // rows a wave: three where that still leaves two workgroups a CU (12288 rows: 512), else one -- fewer partial rows against more waves on a short launch
 static inline int a8ln_rpw(int M) { return M >= 8192 ? 3 : 1; }
+template <typename T> struct A8LnArgs {
+  const T* dy; long lddy;
+  const signed char* q; long ldq;
+  const unsigned char* e; long lde;
+  const float *mean, *rstd, *gamma, *dres; long ldr;
+  float* dx; long ldo;
+  T* dcast; long ldc;
+};
+template <int NV> struct A8LnRow { float d[NV][4], r[NV][4], mu, rs; unsigned w[NV], ex[NV]; };
+template <int MODE, bool RES, typename T, int NV>
+__device__ __forceinline__ void a8ln_load(A8LnRow<NV>& R, const A8LnArgs<T>& p, long row, int C) {
+  const int lane = threadIdx.x & 63;
+  R.mu = p.mean[row];
+  R.rs = p.rstd[row];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4, left = C - c;
+    row_ld<MODE, 4>(p.dy + row * p.lddy, c, C, R.d[i]);
+    R.w[i] = *reinterpret_cast<const unsigned*>(p.q + row * p.ldq + (left > 0 ? c : 0));          // (unconditional, as row_ld)
+    R.ex[i] = p.e[row * p.lde + (left > 0 ? i * 4 + (lane >> 4) : 0)];
+    if constexpr (RES) row_ld<MODE, 4>(p.dres + row * p.ldr, c, C, R.r[i]);
+    else
+#pragma unroll
+      for (int j = 0; j < 4; ++j) R.r[i][j] = 0.f;
+  }
+}
+// dx of a row; each(i, j, dy, xh, dx) for what the caller sums.  KEEP: gm is gamma, kept in registers; longer rows (24 columns a lane) have none left and read it
+// twice a row, from L1
+template <int MODE, bool KEEP, typename T, int NV, typename F>
+__device__ __forceinline__ void a8ln_finish(const A8LnRow<NV>& R, const A8LnArgs<T>& p, const float* __restrict__ gamma, long row, int C, float (&gm)[KEEP ? NV : 1][4],
+                                            F each) {
+  const int lane = threadIdx.x & 63;
+  float s1 = 0.f, s2 = 0.f, xh[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const bool in = (i * 64 + lane) * 4 < C;
+    const float4 xv = act8_unpack4(in ? R.w[i] : 0u, in ? act8_step(R.ex[i]) : 0.f);
+    const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
+    if constexpr (!KEEP) row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, gm[0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {          // (columns past C have d = gamma = 0: no contribution)
+      xh[i][j] = (xx[j] - R.mu) * R.rs;
+      s1 = fmaf(R.d[i][j], gm[KEEP ? i : 0][j], s1);          // (every fma written out: the kernels that share this give the same bits)
+      s2 = fmaf(R.d[i][j] * gm[KEEP ? i : 0][j], xh[i][j], s2);
+    }
+  }
+  const float m1 = lanes_sum(s1) / (float)C, m2 = lanes_sum(s2) / (float)C;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * 64 + lane) * 4, left = C - c;
+    float o[4];
+    if constexpr (!KEEP) row_ld<MODE, 4>(gamma, c, C, gm[0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] = fmaf(R.rs, fmaf(-m2, xh[i][j], fmaf(R.d[i][j], gm[KEEP ? i : 0][j], -m1)), R.r[i][j]);
+      each(i, j, R.d[i][j], xh[i][j], o[j]);
+    }
+    row_st<MODE, 4>(p.dx + row * p.ldo + c, left, o);
+    if (p.dcast) row_st<MODE, 4>(p.dcast + row * p.ldc + c, left, o);
+  }
+}
 template <typename T, int MODE, int NV, bool RES>
-__global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* __restrict__ dy, long lddy, const signed char* __restrict__ q, long ldq,
-                                                                      const unsigned char* __restrict__ e, long lde, const float* __restrict__ mean,
-                                                                      const float* __restrict__ rstd, const float* __restrict__ gamma, const float* dres, long ldr,
-                                                                      float* dx, long ldo, T* __restrict__ dcast, long ldc, float* __restrict__ part, int M, int C, int rpw) {
+__global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(A8LnArgs<T> p, float* __restrict__ part, int M, int C, int rpw) {
   __shared__ __attribute__((aligned(16))) float red[A8LN_WAVES][NV * 256];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  constexpr bool KEEP = NV <= 3;          // gamma stays in registers; longer rows (24 columns a lane) have none left and read it twice a row, from L1
+  constexpr bool KEEP = NV <= 3;
   float ag[NV][4], ab[NV][4], as[NV][4], gm[KEEP ? NV : 1][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if constexpr (KEEP) row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, gm[i]);
+    if constexpr (KEEP) row_ld<MODE, 4>(p.gamma, (i * 64 + lane) * 4, C, gm[i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) ag[i][j] = ab[i][j] = as[i][j] = 0.f;
   }
-  struct Row { float d[NV][4], r[NV][4], mu, rs; unsigned w[NV], ex[NV]; };
-  auto load = [&](Row& R, long row) {
-    R.mu = mean[row];
-    R.rs = rstd[row];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * 64 + lane) * 4, left = C - c;
-      row_ld<MODE, 4>(dy + row * lddy, c, C, R.d[i]);
-      R.w[i] = *reinterpret_cast<const unsigned*>(q + row * ldq + (left > 0 ? c : 0));          // (unconditional, as row_ld)
-      R.ex[i] = e[row * lde + (left > 0 ? i * 4 + (lane >> 4) : 0)];
-      if constexpr (RES) row_ld<MODE, 4>(dres + row * ldr, c, C, R.r[i]);
-      else
-#pragma unroll
-        for (int j = 0; j < 4; ++j) R.r[i][j] = 0.f;
-    }
-  };
+  using Row = A8LnRow<NV>;
+  auto load = [&](Row& R, long row) { a8ln_load<MODE, RES>(R, p, row, C); };
   auto finish = [&](const Row& R, long row) {
-    float s1 = 0.f, s2 = 0.f, xh[NV][4];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = (i * 64 + lane) * 4 < C;
-      const float4 xv = act8_unpack4(in ? R.w[i] : 0u, in ? act8_step(R.ex[i]) : 0.f);
-      const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
-      if constexpr (!KEEP) row_ld<MODE, 4>(gamma, (i * 64 + lane) * 4, C, gm[0]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {          // (columns past C have d = gamma = 0: no contribution)
-        xh[i][j] = (xx[j] - R.mu) * R.rs;
-        const float g = R.d[i][j] * gm[KEEP ? i : 0][j];
-        s1 += g;
-        s2 += g * xh[i][j];
-      }
-    }
-    const float m1 = lanes_sum(s1) / (float)C, m2 = lanes_sum(s2) / (float)C;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * 64 + lane) * 4, left = C - c;
-      float o[4];
-      if constexpr (!KEEP) row_ld<MODE, 4>(gamma, c, C, gm[0]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j] = R.r[i][j] + R.rs * (R.d[i][j] * gm[KEEP ? i : 0][j] - m1 - xh[i][j] * m2);
-        ag[i][j] += R.d[i][j] * xh[i][j];
-        ab[i][j] += R.d[i][j];
-        as[i][j] += o[j];
-      }
-      row_st<MODE, 4>(dx + row * ldo + c, left, o);
-      if (dcast) row_st<MODE, 4>(dcast + row * ldc + c, left, o);
-    }
+    a8ln_finish<MODE, KEEP>(R, p, p.gamma, row, C, gm, [&](int i, int j, float d, float xh, float o) {
+      ag[i][j] += d * xh;
+      ab[i][j] += d;
+      as[i][j] += o;
+    });
   };
   // a row's loads go out before the row in front of it is finished (dx may be dres: rows are disjoint, and a wave reads its row before it writes it); rows of
   // more than 768 columns would need more registers than two waves a SIMD have
@@ -380,14 +398,77 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_kernel(const T* _
     }
   }
 }
+// Few rows, and no column sums of dx wanted: everything in one launch.  dgamma = sum dy xh and dbeta = sum dy need the saved statistics only, not the rows' means
+// that dx is waiting for, so the first ceil(C / 64) workgroups sum a group's columns over all rows (32 rows side by side, added in a fixed order), the others make
+// dx, a row a wave; dy and the codes are read twice, from L2.
+#define A8LN_COLS 64
+template <typename T, int MODE, int NV, bool RES>
+__global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_few_kernel(A8LnArgs<T> p, float* __restrict__ dgamma, float* __restrict__ dbeta, float beta, int M, int C, int ncol) {
+  if ((int)blockIdx.x >= ncol) {
+    constexpr bool KEEP = NV <= 3;
+    const long row = (long)(blockIdx.x - ncol) * A8LN_WAVES + (threadIdx.x >> 6);
+    if (row >= M) return;
+    float gm[KEEP ? NV : 1][4];
+    if constexpr (KEEP)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) row_ld<MODE, 4>(p.gamma, (i * 64 + (threadIdx.x & 63)) * 4, C, gm[i]);
+    A8LnRow<NV> R;
+    a8ln_load<MODE, RES>(R, p, row, C);
+    a8ln_finish<MODE, KEEP>(R, p, p.gamma, row, C, gm, [](int, int, float, float, float) {});
+    return;
+  }
+  constexpr int SLOTS = 4 * A8LN_WAVES, U = 6;
+  __shared__ __attribute__((aligned(16))) float red[2][SLOTS][A8LN_COLS];
+  const int sub = threadIdx.x & 15, slot = threadIdx.x >> 4, c = blockIdx.x * A8LN_COLS + sub * 4;
+  float ag[4] = {0.f, 0.f, 0.f, 0.f}, ab[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int m0 = slot; m0 < M; m0 += SLOTS * U) {
+    float d[U][4], mu[U], rs[U];
+    unsigned w[U], ex[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long m = min(m0 + u * SLOTS, M - 1);
+      row_ld<MODE, 4>(p.dy + m * p.lddy, c, C, d[u]);
+      w[u] = *reinterpret_cast<const unsigned*>(p.q + m * p.ldq + (c < C ? c : 0));
+      ex[u] = p.e[m * p.lde + blockIdx.x];
+      mu[u] = p.mean[m];
+      rs[u] = p.rstd[m];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (m0 + u * SLOTS >= M) break;
+      const float4 xv = act8_unpack4(w[u], act8_step(ex[u]));
+      const float xx[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ag[j] += d[u][j] * ((xx[j] - mu[u]) * rs[u]);
+        ab[j] += d[u][j];
+      }
+    }
+  }
+  *reinterpret_cast<float4*>(&red[0][slot][sub * 4]) = make_float4(ag[0], ag[1], ag[2], ag[3]);
+  *reinterpret_cast<float4*>(&red[1][slot][sub * 4]) = make_float4(ab[0], ab[1], ab[2], ab[3]);
+  __syncthreads();
+  const int k = threadIdx.x >> 6, col = threadIdx.x & 63, n = blockIdx.x * A8LN_COLS + col;
+  float* out = k == 0 ? dgamma : dbeta;
+  if (k > 1 || !out || n >= C) return;
+  float t = red[k][0][col];
+#pragma unroll
+  for (int i = 1; i < SLOTS; ++i) t += red[k][i][col];
+  out[n] = beta != 0.f ? fmaf(beta, out[n], t) : t;
+}
+// Where that one launch is taken.  us on the GPU, one / two launches, 768 columns in 16 bits: 1 row 2.6 / 5.7, 185 3.7 / 7.0, 500 6.0 / 8.4, 768 8.0 / 8.0, 1024 10 / 7.3; 1536 in
+// fp32: 333 4.9 / 10.4, 768 8.1 / 10.8, 1024 15 / 10; 96 columns: 185 3.6 / 5.6, 768 7.8 / 6.3 -- and the second launch costs the host 3 us.
+static inline bool a8ln_few(int M, bool colsum) { return !colsum && M <= 768; }
 template <typename T, int MODE>
-static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long ldq, const unsigned char* e, long lde, const float* mean, const float* rstd,
-                              const float* gamma, const float* dres, long ldr, float* dx, long ldo, T* dcast, long ldc, float* part, int M, int C, hipStream_t st) {
-  const int rpw = a8ln_rpw(M);
-  const dim3 grid((M + A8LN_WAVES * rpw - 1) / (A8LN_WAVES * rpw)), blk(64 * A8LN_WAVES);
-#define LBK(NV_, RES_) \
-  hipLaunchKernelGGL((act8_ln_bwd_kernel<T, MODE, NV_, RES_>), grid, blk, 0, st, dy, lddy, q, ldq, e, lde, mean, rstd, gamma, dres, ldr, dx, ldo, dcast, ldc, part, M, C, rpw)
-#define LB(NV_) do { if (dres) LBK(NV_, true); else LBK(NV_, false); } while (0)
+static int act8_ln_bwd_launch(const A8LnArgs<T>& p, float* part, float* dgamma, float* dbeta, float beta, bool few, int M, int C, hipStream_t st) {
+  const int rpw = few ? 1 : a8ln_rpw(M), ncol = few && (dgamma || dbeta) ? (C + A8LN_COLS - 1) / A8LN_COLS : 0;
+  const dim3 grid((M + A8LN_WAVES * rpw - 1) / (A8LN_WAVES * rpw) + ncol), blk(64 * A8LN_WAVES);
+#define LBK(NV_, RES_)                                                                                                                        \
+  do {                                                                                                                                        \
+    if (few) hipLaunchKernelGGL((act8_ln_bwd_few_kernel<T, MODE, NV_, RES_>), grid, blk, 0, st, p, dgamma, dbeta, beta, M, C, ncol);           \
+    else hipLaunchKernelGGL((act8_ln_bwd_kernel<T, MODE, NV_, RES_>), grid, blk, 0, st, p, part, M, C, rpw);                                   \
+  } while (0)
+#define LB(NV_) do { if (p.dres) LBK(NV_, true); else LBK(NV_, false); } while (0)
   if constexpr (MODE == 2) LB(1);
   else if (C <= 256) LB(1);
   else if (C <= 768) LB(3);
@@ -399,6 +480,10 @@ static int act8_ln_bwd_launch(const T* dy, long lddy, const signed char* q, long
 }
 extern "C" int climb_colreduce3(const float* part, long stride, int nblk, float* out0, float* out1, float* out2, int ncols, float beta, void* stream);      // rowwise.hip
 extern "C" int climb_act8_layernorm_bwd_blocks(int M) { return M <= 0 ? 0 : (int)(((long)M + A8LN_WAVES * a8ln_rpw(M) - 1) / (A8LN_WAVES * a8ln_rpw(M))); }
+extern "C" long climb_act8_layernorm_bwd_workspace(int M, int C, int colsum) {
+  if (M < 0 || C <= 0) return CLIMB_EINVAL;
+  return a8ln_few(M, colsum != 0) ? 0 : (long)climb_act8_layernorm_bwd_blocks(M) * 3 * C * 4;
+}
 extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd,
                                         const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, float* dgamma, float* dbeta,
                                         float* colsum, float beta, int M, int C, void* stream) {
@@ -406,13 +491,14 @@ extern "C" int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, co
     return CLIMB_EINVAL;
   if (C > 1536 || M > (1 << 25)) return CLIMB_EUNSUPPORTED;
   if (M == 0) return CLIMB_OK;
-  if (!dy || !mean || !rstd || !gamma || !dx || !part) return CLIMB_EINVAL;
+  const bool few = a8ln_few(M, colsum != nullptr);
+  if (!dy || !mean || !rstd || !gamma || !dx || (!few && !part)) return CLIMB_EINVAL;
   const int mode = row_mode(al(dy, lddy, 4) && al(dx, ldo, 4) && al(gamma, 0, 4) && (!dres_in || al(dres_in, ldr, 4)) && (!dcast || al(dcast, ldc, 4)), C, 4);
   hipStream_t st = (hipStream_t)stream;
-#define LBL(MODE_, T_)                                                                                                                                                   \
-  act8_ln_bwd_launch<T_, MODE_>((const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc, \
-                                part, M, C, st)
+#define LBL(MODE_, T_)                                                                                                                                                     \
+  act8_ln_bwd_launch<T_, MODE_>(A8LnArgs<T_>{(const T_*)dy, lddy, (const signed char*)q, ldq, (const unsigned char*)e, lde, mean, rstd, gamma, dres_in, ldr, dx, ldo, (T_*)dcast, ldc}, \
+                                part, dgamma, dbeta, beta, few, M, C, st)
   const int rc = dtype == CLIMB_DT_F32 ? BY_MODE(mode, LBL, float) : BY_MODE(mode, LBL, bf16_t);
 #undef LBL
-  return rc != CLIMB_OK ? rc : climb_colreduce3(part, 3L * C, climb_act8_layernorm_bwd_blocks(M), dgamma, dbeta, colsum, C, beta, stream);
+  return rc != CLIMB_OK || few ? rc : climb_colreduce3(part, 3L * C, climb_act8_layernorm_bwd_blocks(M), dgamma, dbeta, colsum, C, beta, stream);
 }

@@ -58,11 +58,15 @@ class Checkpoint:
     __slots__ = ("buf", "rows", "cols", "ld", "groups", "lead", "dtype", "device", "_stats")
 
     def __init__(self, rows: int, cols: int, lead: Tuple[int, ...], dtype: torch.dtype, device: torch.device, stats: bool = False):
-        self.rows, self.cols, self.ld, self.groups = rows, cols, _up(cols, 16), _up(-(-cols // GROUP), 4)          # (whole words: the weight gradient fetches four at a time)
-        self.lead, self.dtype, self.device = lead, dtype, device
-        n = rows * (self.ld + self.groups)
-        self._stats = _up(n, 16) if stats else 0          # byte offset of mean [rows], rstd [rows]
-        self.buf = torch.empty(self._stats + 8 * rows if stats else n, dtype=torch.uint8, device=device)
+        ld, groups = (cols + 15) & ~15, ((cols + GROUP - 1) // GROUP + 3) & ~3          # (whole words of exponents: the weight gradient fetches four at a time)
+        self.rows, self.cols, self.ld, self.groups, self.lead, self.dtype, self.device = rows, cols, ld, groups, lead, dtype, device
+        n = rows * (ld + groups)
+        if stats:          # byte offset of mean [rows], rstd [rows]
+            self._stats = n = (n + 15) & ~15
+            n += 8 * rows
+        else:
+            self._stats = None
+        self.buf = torch.empty(n, dtype=torch.uint8, device=device)
 
     @property
     def q(self) -> torch.Tensor:
@@ -75,11 +79,11 @@ class Checkpoint:
 
     @property
     def mean(self) -> Optional[torch.Tensor]:
-        return self.buf[self._stats:self._stats + 4 * self.rows].view(_F32) if self._stats else None
+        return self.buf[self._stats:self._stats + 4 * self.rows].view(_F32) if self._stats is not None else None
 
     @property
     def rstd(self) -> Optional[torch.Tensor]:
-        return self.buf[self._stats + 4 * self.rows:].view(_F32) if self._stats else None
+        return self.buf[self._stats + 4 * self.rows:].view(_F32) if self._stats is not None else None
 
     @property
     def nbytes(self) -> int:
@@ -182,6 +186,8 @@ def _like(x: torch.Tensor, shape) -> torch.Tensor:
 
 
 def _vec(x: torch.Tensor, what: str, n: int, dev: torch.device) -> torch.Tensor:
+    if isinstance(x, torch.Tensor) and x.dtype is _F32 and x.device == dev and x.numel() == n and x.is_contiguous() and not (x.requires_grad and torch.is_grad_enabled()):
+        return x
     x, M, C, ld = _mat(x, what, dtype=_F32, dev=dev)
     if M * C != n:
         raise ValueError(f"rows8: {what} has {M * C} elements, {n} expected")
@@ -308,7 +314,7 @@ def layernorm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps:
     dev, dt = m.device, out_dtype or _F32
     code = _code(dt)
     g, b = _vec(gamma, "gamma", C, dev), _vec(beta, "beta", C, dev)
-    y = _like(x, x.shape) if dt is _F32 else torch.empty(x.shape, dtype=dt, device=dev)
+    y = torch.empty_like(x, dtype=dt) if x.is_contiguous() else torch.empty(x.shape, dtype=dt, device=dev)
     ck = Checkpoint(M, C, tuple(x.shape[:-1]), _F32, dev, stats=True)
     q, ldq, e, lde = ck._args()
     st = q + ck._stats
@@ -319,7 +325,7 @@ def layernorm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps:
 def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: Optional[torch.Tensor] = None, dgamma: Optional[torch.Tensor] = None,
                   dbeta: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dgamma, dbeta), dx = dres + d(LayerNorm)/dx^T dy in fp32; given `dgamma` / `dbeta` are added to."""
-    if not ck._stats:
+    if ck._stats is None:
         raise ValueError("rows8: this checkpoint holds no row statistics (layernorm_fwd makes one that does)")
     dev, M, C = ck.device, ck.rows, ck.cols
     d, _, _, ld = _mat(dy, "dy", cols=C, rows=M, dev=dev)
@@ -330,23 +336,25 @@ def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: O
         dres, _, _, ldr = _mat(dres, "dres", cols=C, rows=M, dtype=_F32, dev=dev)
         r = dres.data_ptr()
     acc = dgamma is not None or dbeta is not None
-    new = g.new_zeros if acc or M == 0 else g.new_empty
+    new = torch.zeros_like if acc or M == 0 else torch.empty_like
+    if g.dim() != 1:
+        g = g.view(C)
     if dgamma is None:
-        dgamma = new(C)
+        dgamma = new(g)
     else:
         _target(dgamma, "dgamma", (C,), _F32, dev)
     if dbeta is None:
-        dbeta = new(C)
+        dbeta = new(g)
     else:
         _target(dbeta, "dbeta", (C,), _F32, dev)
     dx = _like(g if dres is None else dres, (*ck.lead, C))
     if M == 0:
         return dx, dgamma, dbeta
-    nblk = _query("climb_act8_layernorm_bwd_blocks", M)
-    part = g.new_empty(nblk * 3 * C)
+    nb = _query("climb_act8_layernorm_bwd_workspace", M, C, 0)
+    part = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
     q, ldq, e, lde = ck._args()
     st = q + ck._stats
-    _launch(dev, "climb_act8_layernorm_bwd", d.data_ptr(), ld, code, q, ldq, e, lde, st, st + 4 * M, g.data_ptr(), r, ldr, dx.data_ptr(), C, 0, 0, part.data_ptr(),
+    _launch(dev, "climb_act8_layernorm_bwd", d.data_ptr(), ld, code, q, ldq, e, lde, st, st + 4 * M, g.data_ptr(), r, ldr, dx.data_ptr(), C, 0, 0, part.data_ptr() if nb > 0 else 0,
             dgamma.data_ptr(), dbeta.data_ptr(), 0, 1.0 if acc else 0.0, M, C)
     return dx, dgamma, dbeta
 

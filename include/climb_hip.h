@@ -277,10 +277,12 @@ int climb_act8_group(void);
 int climb_act8_save(const void* x, long ldx, int dtype, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
 int climb_act8_load(const void* q, long ldq, const void* e, long lde, void* y, long ldy, int dtype, int M, int C, void* stream);
 /* climb_layernorm_fwd that also keeps its input as a checkpoint (C <= 1536), and climb_layernorm_bwd with the checkpoint in place of x: dtype = that of dy and
- * dcast (may be NULL); dx fp32 (may be dres_in, which may be NULL).  part[climb_act8_layernorm_bwd_blocks(M)][3][C] is scratch of this call; its reduction
- * dgamma = beta dgamma + .., dbeta, and colsum = beta colsum + column sums of dx, follows in the same call (NULL: skipped; beta 0: not read) */
+ * dcast (may be NULL); dx fp32 (may be dres_in, which may be NULL).  dgamma = beta dgamma + .., dbeta, and colsum = beta colsum + column sums of dx (NULL: skipped;
+ * beta 0: not read) come from partial sums part[climb_act8_layernorm_bwd_blocks(M)][3][C], scratch of this call; few rows without colsum need none:
+ * climb_act8_layernorm_bwd_workspace(M, C, colsum != NULL) is the size of `part` in bytes (0: may be NULL).  No atomics */
 int climb_act8_layernorm_fwd(const float* x, long ldx, const float* gamma, const float* beta, float eps, void* y, long ldy, int y_dtype, float* mean, float* rstd, void* q, long ldq, void* e, long lde, int M, int C, void* stream);
 int climb_act8_layernorm_bwd_blocks(int M);
+long climb_act8_layernorm_bwd_workspace(int M, int C, int colsum);
 int climb_act8_layernorm_bwd(const void* dy, long lddy, int dtype, const void* q, long ldq, const void* e, long lde, const float* mean, const float* rstd, const float* gamma, const float* dres_in, long ldr, float* dx, long ldo, void* dcast, long ldc, float* part, float* dgamma, float* dbeta, float* colsum, float beta, int M, int C, void* stream);
 /* a = gelu(u) (erf form) and the checkpoint of u; du = da gelu'(checkpoint) and, if a != NULL, a = gelu(checkpoint) (the operand of the next layer's weight
  * gradient).  dtype = that of every matrix */

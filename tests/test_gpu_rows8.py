@@ -629,6 +629,44 @@ def test_offsets_beyond_32_bits(dev):
     assert torch.equal(dx[-t:], rows8.layernorm_bwd(y1, ck1, g, dres=tail)[0])
 
 
+@pytest.mark.parametrize("lead", [(0,), (3, 0)])
+def test_no_rows_at_all(dev, lead):
+    from climb_amd import rows8
+    C = 70
+    x, h = torch.zeros(*lead, C, device="cuda"), torch.zeros(*lead, C, device="cuda", dtype=_h16())
+    g = torch.ones(C, device="cuda")
+    y, ck = rows8.layernorm_fwd(x, g, g, 1e-5)
+    dx, dg, db = rows8.layernorm_bwd(x, ck, g, dres=x)
+    acc = rows8.layernorm_bwd(x, ck, g, dgamma=torch.full((C,), 2.0, device="cuda"))[1]
+    assert y.shape == dx.shape == x.shape and not dg.any() and not db.any() and (acc == 2).all() and ck.mean.shape == ck.rstd.shape == (0,)
+    a, uk = rows8.gelu_fwd(h)
+    du, a2 = rows8.gelu_bwd(h, uk, recompute=True)
+    assert a.shape == du.shape == a2.shape == uk.load().shape == h.shape and a.dtype is _h16()
+    w8 = rows8.quantize_rows(torch.ones(5, C, device="cuda"))
+    assert rows8.linear_i8(h, w8).shape == (*lead, 5) and rows8.linear_i8(rows8.quantize_rows(h), w8).shape == (*lead, 5)
+
+
+@pytest.mark.parametrize("M,C", [(1, 64), (30, 768), (767, 100), (768, 1536), (769, 1536), (200, 3)])
+def test_layernorm_gradients_in_one_launch_and_in_two(dev, M, C):
+    """column sums of dx wanted (two launches) or not (one, for few rows): the same dx, and dgamma, dbeta up to the order of their sums"""
+    from climb_amd import _lib, rows8
+    _, x = _make(M, C, torch.float32, M)
+    _, dy = _make(M, C, torch.float32, M + 1)
+    g = torch.rand(C, device="cuda") + 0.5
+    _, ck = rows8.layernorm_fwd(x, g, g, 1e-5)
+    dx, dg, db = rows8.layernorm_bwd(dy, ck, g, dgamma=torch.full((C,), 3.0, device="cuda"))
+    dx2, dg2, db2, cs = torch.empty_like(x), torch.full((C,), 3.0, device="cuda"), torch.zeros(C, device="cuda"), torch.zeros(C, device="cuda")
+    part = torch.empty(_lib.query_arg("climb_act8_layernorm_bwd_workspace", M, C, 1) // 4, device="cuda")
+    assert part.numel() == _lib.query_arg("climb_act8_layernorm_bwd_blocks", M) * 3 * C
+    _lib.call("climb_act8_layernorm_bwd", dy, C, 0, *ck._args(), ck.mean, ck.rstd, g, None, 0, dx2, C, None, 0, part, dg2, db2, cs, 1.0, M, C, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(dx, dx2)
+    xh = (ck.load() - ck.mean[:, None]) * ck.rstd[:, None]
+    for got, want, mag in ((dg, dg2, (dy * xh).abs().sum(0) + 3), (db, db2, dy.abs().sum(0)), (cs, dx.sum(0), dx.abs().sum(0))):
+        assert ((got - want).abs() <= 2 * (M + 8) * U * mag + 1e-30).all()          # two orders of M additions
+    again = rows8.layernorm_bwd(dy, ck, g, dgamma=torch.full((C,), 3.0, device="cuda"))
+    assert torch.equal(again[1], dg) and torch.equal(again[2], db)
+
+
 def test_rows_that_are_not_numbers_stay_in_their_rows(dev):
     """LayerNorm and GELU of rows with a NaN or an infinity: those rows' gradients are NaN where their groups are, the other rows' bits stay as they were"""
     from climb_amd import rows8
