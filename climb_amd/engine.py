@@ -993,7 +993,9 @@ class ViltEngine:
     # ------------------------------------------------------------------ deferred, grouped weight gradients
     def _dw_group_size(self, ws: Workspace, ad) -> int:
         """Layers per grouped weight-gradient launch for this backward; 0 = the immediate per-GEMM path."""
-        if (self.precision != "bf16" and not self.split) or (ws.M % 128) or self.overlap_dw or self.act8:          # (act8: weight gradients are taken layer by layer, from scratch tensors)
+        if (self.precision != "bf16" and not self.split) or (ws.M % 128) or self.overlap_dw:
+            return 0
+        if self.saved["act8"]:          # checkpoints (what the forward kept, not what `act8` says by now): weight gradients are taken layer by layer, from scratch tensors
             return 0
         if ad is not None:
             # under an active adapter the base is normally frozen (train_adapter); the backward then keeps one d(y) scratch for all layers,

@@ -260,3 +260,22 @@ def test_int8_evaluation_after_an_optimizer_step():
     fresh.load_state_dict(model.state_dict())
     want, _ = _evaluate(fresh, images, texts)
     assert _rel(after, want) < 1e-5 and _rel(after, before) > 1e-3
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_act8_switched_between_forward_and_backward(first):
+    """the backward reads what its forward kept, whatever the switch says by then (an even batch: the rows that the deferred weight gradients take)"""
+    images, texts, target = _batch(4, 13)
+    crit = torch.nn.BCEWithLogitsLoss(reduction="mean")
+    out = []
+    for switch in (False, True):
+        model, eng = _model(act8=first)
+        model.train()
+        _, logits = model("vqa", images, texts)
+        if switch:
+            eng.act8 = not first
+        (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+        out.append(grads_of(model))
+    assert set(out[0]) == set(out[1])
+    for n in out[0]:
+        assert _rel(out[1][n], out[0][n]) < 0.02 or n.endswith("key.bias"), n          # (0.02: two runs' last bits, as above)

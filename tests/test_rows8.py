@@ -144,3 +144,19 @@ def test_tensor_calls_refuse():
     ck = rows8.Checkpoint(3, 70, (3,), torch.float32, torch.device("cpu"), stats=True)
     assert ck.nbytes == 3 * 84 + 4 + 24 and ck.mean.shape == ck.rstd.shape == (3,)
     assert rows8.GROUP == _lib.query("climb_act8_group")
+
+
+def test_the_backward_takes_the_mode_of_its_forward():
+    """`act8` switched between a forward and its backward: whether weight gradients are deferred (and where d(x_L) goes) follows what the forward kept"""
+    from types import SimpleNamespace
+    from climb_amd.engine import ViltEngine
+    eng = object.__new__(ViltEngine)
+    eng.precision, eng.split, eng.overlap_dw, eng.grad_ready_hook, eng.cfg = "bf16", False, False, None, dict(layers=12)
+    ws = SimpleNamespace(M=256)
+    for kept in (False, True):
+        eng.saved = dict(act8=kept)
+        sizes = []
+        for now in (False, True):
+            eng.act8 = now
+            sizes.append(eng._dw_group_size(ws, None))
+        assert sizes[0] == sizes[1] and (sizes[0] == 0) == kept
