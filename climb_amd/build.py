@@ -44,6 +44,27 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _made_by(record) -> str:
+    """the command a product was made with ("" if none is on record): other flags make another object of the same source"""
+    try:
+        with open(record) as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
+def _run(cmd, record, what, verbose):
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    if os.path.exists(record):
+        os.remove(record)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
+    with open(record, "w") as f:
+        f.write(" ".join(cmd))
+
+
 def build_library(force: bool = False, verbose: bool = True) -> str:
     _build(LIB_F16, os.path.join(CSRC, "build", "f16"), ["-DCLIMB_H16_F16=1"], force, verbose)
     return _build(LIB, os.path.join(CSRC, "build"), [], force, verbose)
@@ -56,29 +77,16 @@ def _build(LIB: str, objdir: str, extra, force: bool, verbose: bool) -> str:
     for s, stem, fl in units():
         src = os.path.join(CSRC, s)
         obj = os.path.join(objdir, stem + ".o")
-        if force or _stale(obj, [src] + hdrs):
-            jobs.append((src, obj, fl))
-
-    def cc(job):
-        src, obj, fl = job
         cmd = [HIPCC] + FLAGS + extra + fl + ["-c", src, "-o", obj]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"hipcc failed on {src}:\n{r.stdout}\n{r.stderr}")
-        return obj
+        if force or _stale(obj, [src] + hdrs) or _made_by(obj + ".cmd") != " ".join(cmd):
+            jobs.append((cmd, obj + ".cmd", f"hipcc failed on {src}"))
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(cc, jobs))
+        list(ex.map(lambda job: _run(*job, verbose), jobs))
     objs = [os.path.join(objdir, stem + ".o") for _, stem, _ in units()]
-    if force or jobs or _stale(LIB, objs):
-        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    cmd, record = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs, os.path.join(objdir, "link.cmd")
+    if force or jobs or _stale(LIB, objs) or _made_by(record) != " ".join(cmd):
+        _run(cmd, record, "link failed", verbose)
     return LIB
 
 

@@ -407,3 +407,46 @@ def test_committed_traffic_figures_belong_to_this_tree():
     assert tj["csrc_sha16"] == bench.csrc_hash(), "the NT GEMM sources changed since the committed PMC passes: roofline.traffic would be null"
     assert tj.get("step_sha16") == bench.step_hash(), "a kernel source changed since the committed PMC passes: roofline.hbm_bytes_per_step would be null"
     assert tj["gemm_bf16_nt"]["hbm_bytes_per_launch"] > 0 and tj["hbm_bytes_per_step"] > 0
+
+
+def test_objects_are_rebuilt_when_their_flags_change(tmp_path, monkeypatch):
+    """what an object was compiled with is part of its freshness, as its source and the headers are (a stand-in for the compiler: writes its -o, logs its arguments)"""
+    from climb_amd import build
+    log, cc = tmp_path / "log", tmp_path / "cc"
+    cc.write_text(f'#!/bin/sh\necho "$@" >> {log}\nwhile [ "$1" != "-o" ]; do shift; done\ntouch "$2"\n')
+    cc.chmod(0o755)
+    (tmp_path / "a.hip").write_text("")
+    (tmp_path / "b.hip").write_text("")
+    for name, value in (("CSRC", str(tmp_path)), ("LIB", str(tmp_path / "l.so")), ("LIB_F16", str(tmp_path / "l16.so")), ("HIPCC", str(cc)), ("FLAGS", ["-O3"])):
+        monkeypatch.setattr(build, name, value)
+
+    def runs():
+        log.write_text("")
+        build.build_library(verbose=False)
+        return sorted(l.split()[-1] if "-shared" in l else l.split()[-3] for l in log.read_text().splitlines())
+    assert len(runs()) == 6          # two objects and a link, twice
+    assert runs() == []
+    monkeypatch.setattr(build, "FLAGS", ["-O3", "-mno-such-thing"])
+    assert len(runs()) == 6 and runs() == []
+    monkeypatch.setattr(build, "SRC_FLAGS", {"a.hip": ["-DX"]})
+    assert len(runs()) == 4 and runs() == []          # one object and the link, twice
+    os.remove(tmp_path / "build" / "a.o.cmd")
+    assert len(runs()) == 2 and runs() == []
+
+
+def test_the_hazard_scan_compiles_what_the_library_is_built_from():
+    """the source scan of tools/check_store_hazard.py uses the library's own flags"""
+    import importlib.util
+    from climb_amd.build import FLAGS
+    ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("check_store_hazard", os.path.join(ROOT, "tools", "check_store_hazard.py"))
+    ch = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ch)
+    seen = []
+
+    def run(cmd, **kw):
+        seen.append(cmd)
+        open(cmd[-1], "w").close()
+        return types.SimpleNamespace(returncode=0, stderr="")
+    ch.subprocess = types.SimpleNamespace(run=run)
+    assert ch.scan("x.hip") == [] and all(f in seen[0] for f in FLAGS)

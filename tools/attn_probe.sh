@@ -9,7 +9,7 @@ cd "$(dirname "$0")/.."
 OUT=tools/probe/build
 mkdir -p $OUT
 variant() {   # name, flags
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc $2 -c climb_amd/csrc/attention_bf16.hip -o $OUT/attention_$1.o
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Xclang -target-feature -Xclang -packed-fp32-ops $2 -c climb_amd/csrc/attention_bf16.hip -o $OUT/attention_$1.o
   /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT/libclimb_hip_$1.so $OUT/attention_$1.o $(ls climb_amd/csrc/build/*.o | grep -v attention_bf16)
 }
 if [ "$1" = build ]; then

@@ -19,7 +19,11 @@ import sys
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
-CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "climb_amd", "csrc")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from climb_amd.build import FLAGS          # what the library is built with: other flags make other code
+
+CSRC = os.path.join(ROOT, "climb_amd", "csrc")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 NOT_VALU = ("buffer_", "ds_", "global_", "flat_", "s_", "scratch_")
 KNOWN = ()
@@ -51,7 +55,7 @@ def scan(path):
     """one source file, compiled to assembly"""
     with tempfile.TemporaryDirectory() as tmp:
         out = os.path.join(tmp, "k.s")
-        r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "--cuda-device-only"] + EXTRA + ["-S", path, "-o", out],
+        r = subprocess.run([HIPCC] + FLAGS + ["--cuda-device-only"] + EXTRA + ["-S", path, "-o", out],
                            capture_output=True, text=True)
         if r.returncode:
             raise RuntimeError(r.stderr[-2000:])

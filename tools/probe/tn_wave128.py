@@ -14,7 +14,7 @@ _here = os.path.dirname(os.path.abspath(__file__))
 _so = os.path.join(_here, "csrc", "libtn_wave128.so")
 if not os.path.exists(_so) or os.path.getmtime(_so) < os.path.getmtime(os.path.join(_here, "csrc", "tn_wave128.hip")):
     import subprocess
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-shared", "-fPIC", "-I", os.path.join(_here, "..", "..", "climb_amd", "csrc"),
+    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-shared", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", os.path.join(_here, "..", "..", "climb_amd", "csrc"),
                            os.path.join(_here, "csrc", "tn_wave128.hip"), "-o", _so])
 lib = ctypes.CDLL(_so)
 lib.probe_tn_wave128_s32i.argtypes = lib.probe_tn_wave128_s32.argtypes = lib.probe_tn_wave128.argtypes = [ctypes.c_void_p, ctypes.c_long, ctypes.c_void_p, ctypes.c_long, ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_int,
