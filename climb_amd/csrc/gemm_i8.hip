@@ -115,6 +115,9 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
     if (more >= S - 1) wait_vmcnt<(S - 1) * LPT>();
     else if (S > 2 && more == 1) wait_vmcnt<LPT>();
     else wait_vmcnt<0>();
+    // ... and this wave's fragment reads of the stage before are back: behind the barrier the other waves' DMA overwrites that stage, while the first MFMA of a step
+    // needs two of its fragments only
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);

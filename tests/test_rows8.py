@@ -1,5 +1,8 @@
 """8-bit rows, host side: what the C entry points and the tensor calls refuse (nothing here reaches a GPU)."""
 import ctypes
+import importlib.util
+import os
+import re
 
 import pytest
 import torch
@@ -160,3 +163,45 @@ def test_the_backward_takes_the_mode_of_its_forward():
             eng.act8 = now
             sizes.append(eng._dw_group_size(ws, None))
         assert sizes[0] == sizes[1] and (sizes[0] == 0) == kept
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("name", ["gemm_i8.hip", "act8_wgrad.hip"])
+def test_a_stage_is_refilled_only_behind_its_last_reads(name):
+    """behind a raw barrier DMA overwrites the stage that was just read: the source itself asks for the LDS reads in front of each (a barrier waits for none)"""
+    lines = open(os.path.join(ROOT, "climb_amd", "csrc", name)).read().splitlines()
+    at = [i for i, l in enumerate(lines) if "__builtin_amdgcn_s_barrier()" in l]
+    assert at
+    for i in at:
+        before = [l.strip() for l in lines[max(0, i - 2):i]]
+        assert any("s_waitcnt lgkmcnt(0)" in l for l in before), (name, i + 1)
+
+
+def test_the_built_kernels_meet_with_their_reads_back():
+    """... and so it stands in the libraries: between a barrier of the int8 product or the large weight gradient and the last LDS read before it lies lgkmcnt(0)"""
+    spec = importlib.util.spec_from_file_location("check_store_hazard", os.path.join(ROOT, "tools", "check_store_hazard.py"))
+    ch = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ch)
+    libs = [l for l in (os.path.join(ROOT, "climb_amd", "csrc", f) for f in ("libclimb_hip.so", "libclimb_hip_f16.so")) if os.path.exists(l)]
+    if not libs or not os.path.exists(ch.HIPCC):
+        pytest.skip("needs the built libraries and the ROCm llvm tools")
+    for lib in libs:
+        kernels, barriers = set(), 0
+        for code in ch.library_code(lib):
+            kern, waited = None, True
+            for k, l in code:
+                if "gemm_i8_kernel" not in k and "act8_wgrad_big_kernel" not in k:
+                    continue
+                if k != kern:
+                    kern, waited = k, True
+                if l.startswith("ds_read"):
+                    waited = False
+                elif l.startswith("s_waitcnt") and re.search(r"lgkmcnt\(0\)", l):
+                    waited = True
+                elif l.startswith("s_barrier"):
+                    assert waited, k
+                    kernels.add(k)
+                    barriers += 1
+        assert len(kernels) == 19 and barriers >= 3 * 18, (lib, len(kernels), barriers)          # (18 instantiations of the product)

@@ -73,11 +73,10 @@ def scan(path):
     return _analyse(os.path.basename(path), ins)
 
 
-def scan_library(lib):
-    """the SHIPPED binary: every gfx950 code object bundled into the shared library's .hip_fatbin section, disassembled (seconds, no compiler run) --
-    what tests/test_host_logic.py checks after every build"""
+def library_code(lib):
+    """(kernel, instruction) lists of the SHIPPED binary: one for every gfx950 code object bundled into the shared library's .hip_fatbin section, disassembled
+    (seconds, no compiler run)"""
     llvm = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(HIPCC))), "lib", "llvm", "bin")
-    found, nobj, nins = [], 0, 0
     with tempfile.TemporaryDirectory() as tmp:
         fat = os.path.join(tmp, "fat.bin")
         subprocess.run([os.path.join(llvm, "llvm-objcopy"), "-O", "binary", "--only-section=.hip_fatbin", lib, fat], check=True)
@@ -98,9 +97,16 @@ def scan_library(lib):
                 l = l.split("//")[0].strip()
                 if l and kern and not l.endswith(":") and not l.startswith(("Disassembly", lib)):
                     ins.append((kern, l))
-            nobj += 1
-            nins += len(ins)
-            found += _analyse(os.path.basename(lib), ins)
+            yield ins
+
+
+def scan_library(lib):
+    """what tests/test_host_logic.py checks after every build"""
+    found, nobj, nins = [], 0, 0
+    for ins in library_code(lib):
+        nobj += 1
+        nins += len(ins)
+        found += _analyse(os.path.basename(lib), ins)
     return found, nobj, nins
 
 
