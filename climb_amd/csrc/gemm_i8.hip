@@ -124,6 +124,10 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
   };
   static_assert(S == 2 || S == 3, "arrive()");
   arrive(min(nk, S) - 1);
+  bool far = false;          // a token of this wave whose scale asks for the general scaled_sum (the scales have landed with the first stage)
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) far |= sas[wm * MJ * 32 + j * 32 + l31] > ROW_SCALE_PLAIN;
+  const bool plain = vec && m0 + BM <= M && n0 + BN <= N && !__any(far);
   frags(fb[0], fa[0], lbase, co[0]);
   int cur = 0;          // stage buffer
   for (int kt = 0; kt < nk; ++kt) {
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = fmaf((float)a[i], s * sbv[p % PERIOD][i], bv[p % PERIOD][i]);
+          v[i] = scaled_sum<FULL>(a[i], s, sbv[p % PERIOD][i], bv[p % PERIOD][i]);
           if (EPI == EPI_GELU) v[i] = gelu_phi<TO>(v[i]);
           if (EPI == EPI_RESID) v[i] += rv[EPI == EPI_RESID ? p : 0][i];
         }
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void gemm_i8_kernel(const signed
       }
     }
   };
-  if (vec && m0 + BM <= M && n0 + BN <= N) drain(std::true_type{});
+  if (plain) drain(std::true_type{});
   else drain(std::false_type{});
 }
 
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
   int sum = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) sum += red[(w * 16 + l15) * 17 + m];
-  float v = fmaf((float)sum, sc[m] * sw[n], bias ? bias[n] : 0.f);
+  float v = scaled_sum(sum, sc[m], sw[n], bias ? bias[n] : 0.f);
   if (epi == EPI_GELU) v = y_dtype == CLIMB_DT_F32 ? gelu_phi<float>(v) : gelu_phi<bf16_t>(v);
   if (epi == EPI_RESID) v += aux[(long)m * ldaux + n];
   if (y_dtype == CLIMB_DT_F32) static_cast<float*>(y)[(long)m * ldy + n] = v;

@@ -10,6 +10,7 @@
 #pragma once
 #include "common.h"
 
+#define ROW_SCALE_PLAIN 0x1p96f          // (scaled_sum)
 #define ACT8_GROUP 64
 #define ACT8_BAD 255u
 #define ACT8_EMAX 249u          // 2^122, the step of numbers above 127 * 2^121: their codes stop at 63, the largest that stands for a finite fp32 number
@@ -208,6 +209,14 @@ __device__ __forceinline__ unsigned rowq(float x, float s, float rs) {
 }
 __device__ __forceinline__ float row_scale(unsigned mx) {
   return mx >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(mx) / 127.f, 1.1754943508222875e-38f);
+}
+// sum s t + b for an int32 sum and two row scales (both at least 2^-126, or NaN): s t itself may leave fp32's range where the result does not, so the sum takes the
+// scales one after the other -- it is 0 or at least 1 in magnitude, so the first product keeps all its digits, and below 2^31, so it is finite for s <= 2^96.  Beyond
+// that t goes first: if that product overflows, so does the result.  PLAIN: the caller knows that s <= 2^96 (or NaN); the same bits.
+template <bool PLAIN = false>
+__device__ __forceinline__ float scaled_sum(int sum, float s, float t, float b) {
+  const bool far = !PLAIN && s > ROW_SCALE_PLAIN;
+  return fmaf((float)sum * (far ? t : s), far ? s : t, b);
 }
 // Four codes.  |x| / s <= 127, so x * rs is within 127 * 2^-24 < 2^-17 of the quotient, and its distance from the nearest integer is off by less than 2^-25 more: only where
 // that distance comes within 2^-16 of a half can the exact quotient round to the other side, and only a wave that holds such a one (0.8 % of the calls on random

@@ -265,7 +265,7 @@ int climb_attn_bwd_split(const float* qkv, const float* key_bias, const float* d
 /* row codes of x [M, C] (dtype 0 / 1); C <= 2^30 */
 int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);
 /* C[m,n] (c_dtype) = epi(sum_k A[m,k] B[n,k] sa[m] sb[n] + bias[n]); A / B row codes of the tokens and of the weight's rows (one scale an output channel), the
- * sum exact in int32 (K <= 2^17); sa[m] sb[n] is formed first, as an fp32 number (scales whose product overflows give infinities, or NaN for a sum of 0).  epi: 0 none, 1 GELU (erf form; no aux_out), 2 + aux (fp32 [M,N], may be C).  bias may be NULL. */
+ * sum exact in int32 (K <= 2^17); it takes the two scales one after the other, so that only a result beyond fp32 overflows or underflows.  epi: 0 none, 1 GELU (erf form; no aux_out), 2 + aux (fp32 [M,N], may be C).  bias may be NULL. */
 int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const void* B, long ldb, const float* sb, void* C, long ldc, int c_dtype, int M, int N, int K, const float* bias, int epi, const float* aux, long ldaux, void* stream);
 /* the same from tokens that are not quantised yet: y[m,n] (y_dtype) = epi(row codes of x (dtype) times W ...).  One launch for few tokens, else climb_rows8_quant
  * into `workspace` (16-byte aligned, at least climb_linear_i8_workspace(M, K) bytes, 0: none needed; scratch of this call alone) and climb_gemm_i8_nt; the

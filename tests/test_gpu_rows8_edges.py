@@ -1,0 +1,77 @@
+"""8-bit rows at the ends of the number range, at the borders of the launch rules and in the forms that only the engine calls, against their definitions in
+float64 (U = 2^-24, the rounding of fp32)."""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from tests.test_gpu_rows8 import ROOT, U, _h16, _half_step, _make, _phi, _tiny, dev, ref_checkpoint, ref_row_codes          # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ int8 product: scales far from one
+def _linear64(x, w, bias=None):
+    q, sx = ref_row_codes(x)
+    wq, sw = ref_row_codes(w)
+    acc = (q.double() @ wq.double().t()) * sx.double()[:, None] * sw.double()[None, :]
+    z = acc + (bias.double() if bias is not None else 0.0)
+    return z, 4 * U * acc.abs() + U * z.abs() + 2.0 ** -149          # the sum, two products, one of them with the addition; the last may be subnormal
+
+
+# one launch for few tokens, 64 x 64 tiles, 128 x 128, 192 x 192; whole tiles and ragged ones
+SHAPES = [(3, 3000, 48), (40, 3000, 48), (64, 4096, 128), (2560, 3000, 1280), (3072, 3000, 2304), (2500, 3000, 1201)]
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_a_scale_product_below_the_range(dev, M, K, N):
+    """x w of ~1e-41 summed 3000 times: ordinary numbers of ~3e-38, while the product of the two scales has two bits at most"""
+    from climb_amd import rows8
+    g = torch.Generator().manual_seed(M)
+    x, w = (1 + torch.rand(M, K, generator=g)) * 3e-21, (1 + torch.rand(N, K, generator=g)) * 2e-21
+    z, tol = _linear64(x, w)
+    assert float(ref_row_codes(x)[1].double().max() * ref_row_codes(w)[1].double().max()) < 2.0 ** -147 and float(z.min()) > 2.0 ** -126
+    y = rows8.linear_i8(x.cuda(), rows8.quantize_rows(w.cuda())).cpu().double()
+    assert ((y - z).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_scales_at_the_top_of_the_range(dev, M, K, N):
+    """a few tokens of 1e35 (a scale beyond 2^96) times channels of 1e-30: finite; times channels of 1e10: infinite, but a sum of 0 stays 0; the other tokens keep
+    their bits"""
+    from climb_amd import rows8
+    g = torch.Generator().manual_seed(M + 1)
+    x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g) * 1e-30
+    bias = torch.randn(N, generator=g)
+    w[0] = torch.rand(K, generator=g) * 1e10
+    w[1, : K // 2 * 2] = 1e10          # (and the rest, if any, stays tiny: its codes are 0)
+    clean = rows8.linear_i8(x.cuda(), rows8.quantize_rows(w.cuda()), bias.cuda())
+    far = torch.tensor([0, M // 2, M - 1])
+    x[far] = torch.randn(3, K, generator=g) * 1e35
+    x[0] = 1e35
+    x[0, 1::2] = -1e35
+    x[0, K // 2 * 2:] = 0
+    z, tol = _linear64(x, w, bias)
+    assert float(ref_row_codes(x)[1].double()[far].min()) > 2.0 ** 96
+    y = rows8.linear_i8(x.cuda(), rows8.quantize_rows(w.cuda()), bias.cuda())
+    keep = torch.ones(M, dtype=torch.bool)
+    keep[far] = False
+    assert torch.equal(y[keep.cuda()], clean[keep.cuda()])
+    y = y.cpu().double()
+    over = z.abs() > 3.5e38
+    assert over[M - 1, 0] and not over[:, 2:].any()
+    assert (y[over] == torch.sign(z[over]) * math.inf).all() and ((y - z).abs()[~over] <= tol[~over]).all()
+    assert y[0, 1] == bias[1]          # a sum of 0 under a scale product beyond fp32
+
+
+@pytest.mark.skipif(os.environ.get("CLIMB_AMD_H16") == "fp16", reason="this is the child run")
+def test_the_half_build(dev):
+    """this file on the library build whose 16-bit type is IEEE half (a process holds one of them)"""
+    env = dict(os.environ, CLIMB_AMD_H16="fp16", CLIMB_AMD_BACKGROUND_CHILD="1")
+    env.pop("CLIMB_AMD_LIB", None)
+    r = subprocess.run([sys.executable, "-m", "pytest", "tests/test_gpu_rows8_edges.py", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider"], cwd=ROOT, env=env, capture_output=True,
+                       text=True, timeout=110)
+    assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-3000:] + r.stderr[-1000:]
