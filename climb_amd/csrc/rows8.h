@@ -82,19 +82,23 @@ template <> __device__ __forceinline__ float gelu_phi<float>(float x) {
   const float q = phi_lower<8>(x, e2);
   return fmaf(-fminf(fabsf(x), 64.f), q, fmaxf(x, 0.f));
 }
-// For results stored in 16 bits: log2 Phi(-z) is close to a parabola, so one polynomial of degree 8 on [0, 10] (own fit, as above) and ONE exponential give q to
-// 2.6e-5 (relative; a 150th of bf16's half step, a 10th of half's): 11 full-rate operations and a transcendental, against 13 and two.  Beyond 10, where
-// x q is below 1e-22, z stays at 10.  minimum / maximum: the NaN of a NaN argument goes through.
+// For results stored in 16 bits: log2 Phi(-z) is close to a parabola, so one polynomial of degree 8 (own fit, as above) and ONE exponential give q: 11 full-rate
+// operations and a transcendental, against 13 and two.  bfloat16 holds x q down to z = 13.2 and its half step is 2^-9 of a number at least, so the fit spans
+// [0, 13.2] and may err more where q is small: relative error 1.8e-5 below 2, 8e-5 below 3, 3.8e-4 beyond; z stays at 14.5, where q underflows to the limit 0.
+// IEEE half ends at 2^-25 (z = 5.6) with a finer step: fitted on [0, 10] to 2.6e-5, z stays at 10.  minimum / maximum: the NaN of a NaN argument goes through.
+#if CLIMB_H16_F16
+#define GELU16_END 10.f
+#define GELU16_C {-1.00002384f, -1.15098619f, -0.458911031f, -0.0537272729f, 0.00850201212f, -0.000961354177f, 7.17434377e-05f, -3.12999009e-06f, 6.00354042e-08f}
+#else
+#define GELU16_END 14.5f
+#define GELU16_C {-1.0000207f, -1.1508853f, -0.4593939f, -0.053093407f, 0.00815379f, -0.00086898665f, 5.9202197e-05f, -2.2890285e-06f, 3.7937127e-08f}
+#endif
 template <> __device__ __forceinline__ float gelu_phi<bf16_t>(float x) {
-  const float z = __builtin_elementwise_minimum(__builtin_fabsf(x), 10.f);
-  float p = fmaf(6.00354042e-08f, z, -3.12999009e-06f);
-  p = fmaf(p, z, 7.17434377e-05f);
-  p = fmaf(p, z, -0.000961354177f);
-  p = fmaf(p, z, 0.00850201212f);
-  p = fmaf(p, z, -0.0537272729f);
-  p = fmaf(p, z, -0.458911031f);
-  p = fmaf(p, z, -1.15098619f);
-  p = fmaf(p, z, -1.00002384f);
+  constexpr float C[9] = GELU16_C;
+  const float z = __builtin_elementwise_minimum(__builtin_fabsf(x), GELU16_END);
+  float p = C[8];
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fmaf(p, z, C[i]);
   return fmaf(-z, __builtin_amdgcn_exp2f(p), __builtin_elementwise_maximum(x, 0.f));
 }
 // ... and gelu'(x) = Phi(x) + x exp(-x^2 / 2) / sqrt(2 pi)

@@ -67,6 +67,31 @@ def test_scales_at_the_top_of_the_range(dev, M, K, N):
     assert y[0, 1] == bias[1]          # a sum of 0 under a scale product beyond fp32
 
 
+# ------------------------------------------------------------------------------------------------ GELU in 16 bits
+def test_gelu_of_every_16_bit_number(dev):
+    """all 65536 arguments, through gelu_fwd and through the product's epilogue (tokens of zeros: the argument is the bias).  x q, q = Phi(-|x|) = 2^p: the fit of p gives q to
+    2e-5 below 2, 9e-5 below 3 and 4e-4 beyond (half: 2.7e-5), Horner's roundings of p 8 U x^2 and the rest 20 U, as in test_gelu; 2^p ends at 2^-126, times |x| <= 14.5"""
+    from climb_amd import rows8
+    dt = _h16()
+    u = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dt)
+    x = u.double()
+    ref = torch.where(x == -math.inf, torch.zeros_like(x), torch.where(x == math.inf, x, x * _phi(x)))
+    z = x.abs().clamp(max=40.0)
+    tail = z * _phi(-z)
+    fit = torch.where(z < 2, 2e-5, torch.where(z < 3, 9e-5, 4e-4)) if dt is torch.bfloat16 else torch.full_like(z, 2.7e-5)
+    tol = tail * (fit + U * (20 + 8 * z * z)) + U * ref.abs().nan_to_num(posinf=0.0) + _half_step(dt) * ref.abs().nan_to_num(posinf=0.0) + max(_tiny(dt), 2.0 ** -122)
+    nan = torch.isnan(x)
+    a, _ = rows8.gelu_fwd(u.cuda().view(256, 256))
+    w8 = rows8.quantize_rows(torch.ones(65536, 16, device="cuda"))
+    y = rows8.linear_i8(torch.zeros(9, 16, dtype=dt, device="cuda"), w8, u.float().cuda(), epi="gelu")
+    few = rows8.linear_i8(torch.zeros(2, 16, dtype=dt, device="cuda"), w8, u.float().cuda(), epi="gelu")
+    for got in (a.view(-1), y[0], y[8], few[1]):
+        got = got.cpu().double()
+        assert torch.equal(torch.isnan(got), nan)
+        ok = (got == ref) | ((got - ref).abs() <= tol) | nan
+        assert ok.all(), (x[~ok][:5], got[~ok][:5], ref[~ok][:5])
+
+
 @pytest.mark.skipif(os.environ.get("CLIMB_AMD_H16") == "fp16", reason="this is the child run")
 def test_the_half_build(dev):
     """this file on the library build whose 16-bit type is IEEE half (a process holds one of them)"""
