@@ -20,6 +20,17 @@ __device__ __forceinline__ bf16x8 wg_frag(const unsigned char* __restrict__ S, i
   return c.b;
 }
 
+// 16 codes of a group with exponent byte e -> 16 numbers of the operand type, zeros for a token that is not there
+__device__ __forceinline__ void wg_expand(u32x4 q, unsigned e, bool live, unsigned (&h)[8]) {
+  const float step = live ? act8_step(e) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 v = act8_values4<bf16_t>(q[i], e, step);
+    h[2 * i] = pack_bf16x2(v.x, v.y);
+    h[2 * i + 1] = pack_bf16x2(v.z, v.w);
+  }
+}
+
 struct WgStage {
   u32x4 a[4], b[2];          // 8 gradients x 4 token rows, 16 codes x 2 token rows
   unsigned e[2];
@@ -77,14 +88,8 @@ __device__ __forceinline__ void wg_store(WgStage& s, unsigned char* __restrict__
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const int row = (t >> 3) + 32 * p;
-    const float step = row < left ? act8_step(s.e[p]) : 0.f;
     unsigned h[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = act8_unpack4(s.b[p][i], step);
-      h[2 * i] = pack_bf16x2(v.x, v.y);
-      h[2 * i + 1] = pack_bf16x2(v.z, v.w);
-    }
+    wg_expand(s.b[p], s.e[p], row < left, h);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       *reinterpret_cast<u32x4*>(Bs + row * WG_PITCH + ((((t & 7) * 2 + i) ^ wg_swz(row)) << 4)) = (u32x4){h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]};
@@ -252,17 +257,10 @@ __device__ __forceinline__ bf16x8 wb_frag(const unsigned char* __restrict__ p) {
   c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * WB_PITCH));
   return c.b;
 }
-// 16 codes -> 16 numbers of the operand type
 __device__ __forceinline__ void wb_expand(u32x4 q, unsigned e4, bool live, unsigned char* __restrict__ Bs) {
   const int row = threadIdx.x >> 4, c16 = threadIdx.x & 15;
-  const float step = live ? act8_step((e4 >> ((c16 >> 2) * 8)) & 255u) : 0.f;
   unsigned h[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 v = act8_unpack4(q[i], step);
-    h[2 * i] = pack_bf16x2(v.x, v.y);
-    h[2 * i + 1] = pack_bf16x2(v.z, v.w);
-  }
+  wg_expand(q, (e4 >> ((c16 >> 2) * 8)) & 255u, live, h);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     *reinterpret_cast<u32x4*>(Bs + row * WB_PITCH + (((c16 * 2 + i) ^ wg_swz(row)) << 4)) = (u32x4){h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]};

@@ -54,6 +54,20 @@ __device__ __forceinline__ float4 act8_unpack4(unsigned w, float step) {
                      (__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060502u)) - off) * step, (__uint_as_float(__builtin_amdgcn_perm(0x4b000000u, u, 0x07060503u)) - off) * step);
 }
 
+// ... as numbers of type T, of a group with exponent byte e.  A number of IEEE half above 65024 is kept as 64 steps of 2^10 = 65536, one step beyond the type's largest:
+// where the half build reads that in 16 bits (a load, an MFMA operand, a recomputed activation) it is the largest again and no infinity
+template <typename T>
+__device__ __forceinline__ float4 act8_values4(unsigned w, unsigned e, float step) {
+  float4 v = act8_unpack4(w, step);
+#if CLIMB_H16_F16
+  if (sizeof(T) == 2 && e == 127u + 10u) {
+    auto top = [](float x) { return fabsf(x) == 65536.f ? copysignf(65504.f, x) : x; };
+    v = make_float4(top(v.x), top(v.y), top(v.z), top(v.w));
+  }
+#endif
+  return v;
+}
+
 // Phi(-|x|) = exp(-x^2 / 2) R(1 / (1 + p |x|)), R a polynomial without constant term fitted to erfcx(|x| / sqrt 2) / 2 on [0, 14] for the smallest largest
 // RELATIVE error (weighted least squares, own fit): the tail keeps its digits, where 1 + erf would cancel them.  DEG 6: 8.3e-6 (results that are stored
 // in 16 bits: a 470th of their half step), DEG 8: 1.5e-7 (fp32 results).  e2 returns exp(-x^2 / 2).

@@ -123,9 +123,10 @@ __global__ __launch_bounds__(256) void act8_kernel(const T* __restrict__ x, long
   } else {
     if (left <= 0) return;          // (so that every load below is unconditional)
     const uint2 w = *reinterpret_cast<const uint2*>(q + row * ldq + c);
-    const float step = act8_step(e[row * lde + g]);
+    const unsigned ex = e[row * lde + g];
     if constexpr (OP == 3) row_ld<MODE, 8>(x + row * ldx, c, C, v);
-    const float4 a = act8_unpack4(w.x, step), b = act8_unpack4(w.y, step);
+    const float step = act8_step(ex);
+    const float4 a = act8_values4<T>(w.x, ex, step), b = act8_values4<T>(w.y, ex, step);
     const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     if constexpr (OP == 2) {
       row_st<MODE, 8>(y + row * ldy + c, left, d);

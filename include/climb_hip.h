@@ -261,7 +261,7 @@ int climb_attn_bwd_split(const float* qkv, const float* key_bias, const float* d
  *                numbers beyond 63 2^122 are kept as that.  ldq % 16 == 0,
  *                ldq >= C.  Code matrices are 16-byte aligned; the other matrices may have any row stride and alignment of their type.
  * Rows M <= 2^30 (LayerNorm: 2^25), and a launch of 2^32 threads or more -- some 10^10 elements -- is refused (-2).  In the fp16 build a 16-bit result beyond 65504 is
- * infinite, a checkpoint's too.  An output overlaps no input and no other output unless its entry says so.  M = 0 is allowed everywhere (nothing is launched, except that climb_act8_weight_grad still scales C and dbias by beta). */
+ * infinite, a checkpoint's too, but for 65536, which a number above 65024 may be kept as: read in 16 bits that is 65504.  An output overlaps no input and no other output unless its entry says so.  M = 0 is allowed everywhere (nothing is launched, except that climb_act8_weight_grad still scales C and dbias by beta). */
 /* row codes of x [M, C] (dtype 0 / 1); C <= 2^30 */
 int climb_rows8_quant(const void* x, long ldx, int dtype, void* q, long ldq, float* s, int M, int C, void* stream);
 /* C[m,n] (c_dtype) = epi(sum_k A[m,k] B[n,k] sa[m] sb[n] + bias[n]); A / B row codes of the tokens and of the weight's rows (one scale an output channel), the

@@ -92,6 +92,38 @@ def test_gelu_of_every_16_bit_number(dev):
         assert ok.all(), (x[~ok][:5], got[~ok][:5], ref[~ok][:5])
 
 
+# ------------------------------------------------------------------------------------------------ checkpoints at the top of the 16-bit type
+@pytest.mark.parametrize("M,K,N", [(70, 130, 48), (7000, 768, 2304)])          # both kernels of the weight gradient
+def test_the_largest_16_bit_activations_stay_finite(dev, M, K, N):
+    """a finite activation next to the largest of its type reads back finite, in a load, as a recomputed activation and as an operand; beyond it, it is infinite"""
+    from climb_amd import rows8
+    dt = _h16()
+    half = dt is torch.float16
+    top = 65504.0 if half else torch.finfo(torch.bfloat16).max
+    x = _make(M, K, dt, 5)[0]
+    for r, f in ((3, 1.0), (4, -1.0), (5, 0.9985), (6, -0.994)):          # (of half: 65504, 65408, 65120)
+        x[r, 7 * r] = f * top
+    assert torch.isfinite(x).all()
+    _, _, v = ref_checkpoint(x, half)
+    if half:
+        assert (v.abs() == 65536).any()
+        v = torch.where(v.abs() == 65536, torch.sign(v) * top, v)
+    ck = rows8.checkpoint_save(x.cuda())
+    assert torch.equal(ck.load().cpu().double(), v)
+    da = torch.ones(M, K, dtype=dt, device="cuda")
+    du, a = rows8.gelu_bwd(da, ck, recompute=True)
+    assert torch.isfinite(a).all() and torch.isfinite(du).all() and float(a[3, 21]) == float(v[3, 21])
+    dy = _make(M, N, dt, 6)[0]
+    dy[3:7] = (2.0 ** -13 if half else 2.0 ** -100)
+    dw, _ = rows8.weight_grad(dy.cuda(), ck)
+    ref, mag = dy.double().t() @ v, dy.double().abs().t() @ v.abs()
+    assert ((dw.cpu().double() - ref).abs() <= 2 * (M + 16) * U * mag + 1e-30).all()
+    if half:          # fp32 numbers beyond the type are what they were: infinite in 16 bits
+        y = torch.full((2, 64), 66100.0, device="cuda")
+        y[1] = -70000.0
+        assert torch.isinf(rows8.checkpoint_save(y).load(dt)).all()
+
+
 @pytest.mark.skipif(os.environ.get("CLIMB_AMD_H16") == "fp16", reason="this is the child run")
 def test_the_half_build(dev):
     """this file on the library build whose 16-bit type is IEEE half (a process holds one of them)"""
