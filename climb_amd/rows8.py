@@ -14,7 +14,7 @@ pass keeps for its backward: half the bytes of a 16-bit activation, a quarter of
 Matrices are [..., C] in fp32 or the library's 16-bit type, on one HIP device, any row stride; an input whose last dimension is strided or whose rows overlap
 (a broadcast view) is copied first.  Work goes to the current stream of the inputs' device; nothing synchronises, and every scratch buffer is the call's
 own (torch's allocator), so the calls can be captured.  Forward and backward are explicit calls as in climb_amd.engine: inputs that require grad are
-refused while autograd records.
+refused while autograd records, and so are forward-mode tangents.
 
 The host's share of a call is kept small (a launch alone is 3 us, and a batch of one sequence runs in less): one allocation per code matrix with its scales,
 contiguous inputs taken as they are, the stream read as a plain number."""
@@ -23,6 +23,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 
@@ -149,13 +150,19 @@ def _query(name: str, *args) -> int:
     return fn(*args)
 
 
+def _recorded(x: torch.Tensor) -> bool:
+    """whether autograd would have to see what is done with x, in reverse mode or (inside forward_ad.dual_level()) in forward mode"""
+    return (x.requires_grad and torch.is_grad_enabled()) or (_fwd._current_level >= 0 and _fwd.unpack_dual(x).tangent is not None)
+
+
 def _mat(x: torch.Tensor, what: str, cols: Optional[int] = None, rows: Optional[int] = None, dtype: Optional[torch.dtype] = None,
          dev: Optional[torch.device] = None) -> Tuple[torch.Tensor, int, int, int]:
     """(x, rows, cols, row stride) of x as a matrix with unit column stride and rows that do not overlap"""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"rows8: {what} must be a tensor")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"rows8: {what} requires grad, and these calls record nothing for autograd: detach it (forward and backward are explicit calls)")
+    if _recorded(x):
+        raise RuntimeError(f"rows8: {what} requires grad or carries a forward-mode tangent, and these calls record nothing for autograd: detach it (forward and backward are "
+                           "explicit calls)")
     if not x.is_cuda or (dev is not None and x.device != dev):
         raise ValueError(f"rows8: {what} is on {x.device}; every tensor of a call must be on one HIP device")
     shape = x.shape
@@ -186,7 +193,7 @@ def _like(x: torch.Tensor, shape) -> torch.Tensor:
 
 
 def _vec(x: torch.Tensor, what: str, n: int, dev: torch.device) -> torch.Tensor:
-    if isinstance(x, torch.Tensor) and x.dtype is _F32 and x.device == dev and x.numel() == n and x.is_contiguous() and not (x.requires_grad and torch.is_grad_enabled()):
+    if isinstance(x, torch.Tensor) and x.dtype is _F32 and x.device == dev and x.numel() == n and x.is_contiguous() and not _recorded(x):
         return x
     x, M, C, ld = _mat(x, what, dtype=_F32, dev=dev)
     if M * C != n:
@@ -198,8 +205,8 @@ def _target(x: torch.Tensor, what: str, shape: Tuple[int, ...], dtype: torch.dty
     """row stride of a tensor that the call writes: never copied"""
     if not isinstance(x, torch.Tensor) or tuple(x.shape) != tuple(shape) or x.dtype is not dtype or x.device != dev:
         raise ValueError(f"rows8: {what} must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"rows8: {what} requires grad and would be written in place")
+    if _recorded(x):
+        raise RuntimeError(f"rows8: {what} requires grad or carries a forward-mode tangent, and would be written in place")
     if x.is_contiguous():
         return shape[-1]
     if x.dim() != 2 or (shape[1] > 1 and x.stride(1) != 1) or (shape[0] > 1 and x.stride(0) < shape[1]):

@@ -205,3 +205,18 @@ def test_the_built_kernels_meet_with_their_reads_back():
                     kernels.add(k)
                     barriers += 1
         assert len(kernels) == 19 and barriers >= 3 * 18, (lib, len(kernels), barriers)          # (18 instantiations of the product)
+
+
+def test_forward_mode_tangents_are_refused():
+    """a tangent that a call would drop without a word: for matrices, vectors and tensors that are written in place"""
+    import torch.autograd.forward_ad as fwd
+    x, v, dev = torch.ones(4, 8), torch.ones(8), torch.device("cpu")
+    with fwd.dual_level():
+        for call in (lambda: rows8.gelu_fwd(fwd.make_dual(x, x)), lambda: rows8.quantize_rows(fwd.make_dual(x, x)), lambda: rows8._vec(fwd.make_dual(v, v), "bias", 8, dev),
+                     lambda: rows8._target(fwd.make_dual(x, x), "out", (4, 8), torch.float32, dev)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert rows8._vec(v, "bias", 8, dev) is v          # inside a level, but without a tangent
+        with pytest.raises(ValueError, match="HIP device"):
+            rows8.gelu_fwd(x)
+    assert rows8._vec(v, "bias", 8, dev) is v
