@@ -144,13 +144,7 @@ class Workspace:
         self.u = per_layer(lambda: buf((M, Fd), adt), L)
         self.a = per_layer(lambda: opbuf(M, Fd), L)
         self.i8 = None               # scratch of the int8 products (eval_i8), allocated by the first forward that runs them
-        if eng.act8:
-            from .rows8 import Checkpoint
-            self.ck = [{n: Checkpoint(M, c, (M,), adt, dev) for n, c in (("x", H), ("h1", H), ("xn", H), ("hn", H), ("u", Fd))} for _ in range(L)]
-            self.du_a = buf((M, Fd), adt)          # d(gelu output) before x gelu'(checkpoint)
-            self.part8 = buf((_lib.query_arg("climb_act8_layernorm_bwd_blocks", M) * 3 * H,))
-            self.wg8_bytes = max(_lib.query_arg("climb_act8_weight_grad_workspace", M, n, H) for n in (3 * H, Fd))
-            self.wg8 = torch.empty((max(self.wg8_bytes, 16),), dtype=torch.uint8, device=dev)
+        self.ck = None               # 8-bit checkpoints (act8): ensure_act8
         if sp:      # split twins of the fp32 tensors that something besides a GEMM reads too (attention output / gradient, im2col, d(projection))
             self.a_patch_s = opbuf(B * self.NP, cfg["channels"] * cfg["patch"] ** 2)
             self.ctx_s = [opbuf(M, H) for _ in range(L)]
@@ -208,6 +202,19 @@ class Workspace:
         self.red_plans = {}          # batched column reductions: segment tables in HBM
         self.part_l = None
         self.dx_c = self.dh_c = self.du_l = self.dqkv_l = None
+
+    def ensure_act8(self, eng: "ViltEngine"):
+        """The 8-bit checkpoints of every layer and the scratch of the backward that reads them: for a forward that saves (one without gradients keeps nothing)."""
+        if self.ck is not None:
+            return
+        from .rows8 import Checkpoint
+        cfg, dev, M, adt = eng.cfg, eng.device, self.M, self.u[0].dtype
+        H, Fd = cfg["hidden"], cfg["ffn"]
+        self.du_a = torch.empty((M, Fd), dtype=adt, device=dev)          # d(gelu output) before x gelu'(checkpoint)
+        self.part8 = torch.empty((_lib.query_arg("climb_act8_layernorm_bwd_blocks", M) * 3 * H,), dtype=torch.float32, device=dev)
+        self.wg8_bytes = max(_lib.query_arg("climb_act8_weight_grad_workspace", M, n, H) for n in (3 * H, Fd))
+        self.wg8 = torch.empty((max(self.wg8_bytes, 16),), dtype=torch.uint8, device=dev)
+        self.ck = [{n: Checkpoint(M, c, (M,), adt, dev) for n, c in (("x", H), ("h1", H), ("xn", H), ("hn", H), ("u", Fd))} for _ in range(cfg["layers"])]
 
     def ensure_deferred(self, eng: "ViltEngine"):
         """Per-LAYER copies of the four weight-gradient operands the backward produces (d(x_{i+1}), d(u_i), d(h1_i), d(qkv_i), 16 bit): the
@@ -875,6 +882,8 @@ class ViltEngine:
             raise NotImplementedError(f"act8 / eval_i8 in {'bf16x3' if self.split else 'fp32'}: 8-bit rows go with the 16-bit operand types")
         if act8 and (ad is not None or prune):
             raise NotImplementedError("8-bit activation checkpoints (act8) with an active adapter or cls_only_last")
+        if act8:
+            ws.ensure_act8(self)
         self._i8_pass = ws if (self.eval_i8 and not save and not prune) else False
         for i in range(cfg["layers"]):
             l = f"{ENC}encoder.layer.{i}."

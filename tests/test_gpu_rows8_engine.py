@@ -279,3 +279,28 @@ def test_act8_switched_between_forward_and_backward(first):
     assert set(out[0]) == set(out[1])
     for n in out[0]:
         assert _rel(out[1][n], out[0][n]) < 0.02 or n.endswith("key.bias"), n          # (0.02: two runs' last bits, as above)
+
+
+def test_forwards_without_gradients_hold_no_checkpoints():
+    """act8 keeps memory down: an evaluation's workspace -- of its own batch size, or beside a pending backward -- has neither checkpoints nor the backward's scratch"""
+    model, eng = _model(act8=True)
+    images, texts, target = _batch(3, 17)
+    other = _batch(5, 18)
+    p0, _ = _evaluate(model, other[0], other[1])
+    names = ("ck", "part8", "wg8", "du_a")
+    assert [w for w in eng._ws.values()] and not any(getattr(w, n, None) is not None for w in eng._ws.values() for n in names)
+    model.train()
+    crit = torch.nn.BCEWithLogitsLoss(reduction="mean")
+    _, logits = model("vqa", images, texts)
+    with torch.no_grad():
+        model("vqa", images, texts)
+    assert sorted(getattr(w, "ck", None) is not None for w in eng._ws.values()) == [False, False, True]
+    (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+    G = grads_of(model)
+    plain, _ = _model()
+    assert _rel(p0, _evaluate(plain, other[0], other[1])[0]) < 1e-2
+    plain.train()
+    _, logits = plain("vqa", images, texts)
+    (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+    for n, r in grads_of(plain).items():
+        assert n.endswith("key.bias") or _rel(G[n], r) < 0.08, n
