@@ -317,8 +317,7 @@ class ViltEngine:
         if self.act8 and (layout.adapters or self.cls_only_last):
             raise NotImplementedError("CLIMB_AMD_ACT8: no 8-bit checkpoints with adapters or CLIMB_AMD_CLS_ONLY_LAST")
         self._i8_pass = False          # inside a forward that eval_i8 covers
-        self._i8_weights: Dict[str, object] = {}          # weight name -> rows8.RowCodes
-        self._i8_version = None
+        self._i8_weights: Dict[str, tuple] = {}          # weight name -> (rows8.RowCodes, the parameter version they were laid out from)
         self._param_epoch = 0          # parameter updates that bump no version counter (FusedAdamW writes through the C ABI)
 
     # ------------------------------------------------------------------ buffers
@@ -473,27 +472,28 @@ class ViltEngine:
         _lib.call("climb_split_f32", src, C, dst, C, M * C, M, C, mode, aux, C, _stream())
 
     def _i8_weight(self, wname, N, K):
-        """row codes of the fp32 master weight, one scale an output channel; laid out once per parameter version"""
-        ver = (self.flat.data_ptr(), self.flat._version, self._param_epoch)
-        if ver != self._i8_version:
-            self._i8_weights.clear()
-            self._i8_version = ver
-        w = self._i8_weights.get(wname)
-        if w is None:
-            from . import rows8
-            o = self.layout.offset[wname]
-            with torch.no_grad():
-                w = self._i8_weights[wname] = rows8.quantize_rows(self.flat[o:o + N * K].view(N, K).detach())
+        """row codes of the fp32 master weight, one scale an output channel; laid out once per parameter version, in the same buffer each time (a captured forward holds
+        its address).  A capture records the layout with the product, so that its replays follow the parameters; it has not run by then, so the next eager
+        forward lays the weight out itself."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        now = (self.flat.data_ptr(), self.flat._version, self._param_epoch)
+        w, ver = self._i8_weights.get(wname, (None, None))
+        if ver != now or capturing:
+            if w is None:
+                from .rows8 import RowCodes
+                w = RowCodes(N, K, (N,), self.device)
+            p = w.buf.data_ptr()
+            _lib.call("climb_rows8_quant", self.p(wname), K, F32, p, w.ld, p + N * w.ld, N, K, _stream())
+            self._i8_weights[wname] = (w, None if capturing else now)
         return w
 
     def _i8_fwd(self, ws, X, wname, bname, Y, M, N, K, epi, aux, out_f32):
         w = self._i8_weight(wname, N, K)
-        nb = _lib.query_arg("climb_linear_i8_workspace", M, K)
-        if ws.i8 is None or ws.i8.numel() < nb:
-            ws.i8 = torch.empty((nb,), dtype=torch.uint8, device=self.device)
+        if ws.i8 is None:          # once, for the longest reduction: a captured forward holds its address
+            ws.i8 = torch.empty((max(_lib.query_arg("climb_linear_i8_workspace", M, k) for k in (self.cfg["hidden"], self.cfg["ffn"])),), dtype=torch.uint8, device=self.device)
         p = w.buf.data_ptr()
         self._timed_call("linear_i8", 2.0 * M * N * K, "climb_linear_i8", X, K, BF16, p, w.ld, p + N * w.ld, Y, N, F32 if out_f32 else BF16, M, N, K,
-                         self.p(bname) if bname else None, epi, aux, N, ws.i8, nb, _stream())
+                         self.p(bname) if bname else None, epi, aux, N, ws.i8, ws.i8.numel(), _stream())
 
     def linear_fwd(self, X, wname, bname, Y, M, N, K, epi=EPI_NONE, aux=None, aux_out=None, aux2=None, out_f32=False):
         if self._i8_pass and epi in (EPI_NONE, self.epi_gelu) and aux2 is None:

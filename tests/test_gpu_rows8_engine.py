@@ -304,3 +304,54 @@ def test_forwards_without_gradients_hold_no_checkpoints():
     (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
     for n, r in grads_of(plain).items():
         assert n.endswith("key.bias") or _rel(G[n], r) < 0.08, n
+
+
+@pytest.mark.parametrize("eager_first", [True, False])
+def test_int8_evaluation_captured(eager_first):
+    """a captured evaluation, with or without an eager one before it: replays beside eager work and after parameter updates (through torch and through the fused
+    optimizer) multiply by the parameters of their time, and so do the eager evaluations after a capture"""
+    images, texts, target = _batch(4, 21)
+    other = _batch(4, 22)
+    model, eng = _model(eval_i8=True)
+    model.eval()
+    opt = model.create_optimizer({"lr": 1e-2, "weight_decay": 0.0, "adam_epsilon": 1e-8})
+    eng.refresh_shadow()          # (what the 16-bit parts of the forward read)
+    im, tx = images.cuda(), {k: v.cuda() for k, v in texts.items()}
+    if eager_first:
+        _evaluate(model, images, texts)
+    eng.eval_i8 = False          # (the first run of everything else: workspaces, LDS limits)
+    _evaluate(model, im, tx)
+    eng.eval_i8 = True
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g), torch.no_grad():
+        pooled, logits = model("vqa", im, tx)
+
+    def fresh(i, t):
+        m, _ = _model(eval_i8=True)
+        m.load_state_dict(model.state_dict())
+        return _evaluate(m, i, t)[0]
+    first = None
+    for step in range(3):
+        for i, t in ((images, texts), (other[0], other[1])):
+            want = fresh(i, t)
+            im.copy_(i)
+            for k in tx:
+                tx[k].copy_(t[k])
+            g.replay()
+            torch.cuda.synchronize()
+            assert _rel(pooled.cpu(), want) < 1e-5, step
+            if first is None:
+                first = want
+            assert _rel(_evaluate(model, i, t)[0], want) < 1e-5, step
+        if step == 0:
+            with torch.no_grad():
+                for n, p in model.named_parameters():
+                    if n.endswith("output.dense.weight") or n.endswith("query.weight"):
+                        p.mul_(1.5)
+        else:
+            model.train()
+            model.fused_forward_backward("vqa", images, texts, target)
+            opt.step()
+            opt.zero_grad()
+            model.eval()
+    assert _rel(fresh(images, texts), first) > 1e-3
