@@ -31,6 +31,12 @@ __device__ __forceinline__ void wg_expand(u32x4 q, unsigned e, bool live, unsign
   }
 }
 
+// XCD-contiguous chunks of the launch: the workgroups of an XCD belong to the same token range, whose panels its L2 then holds once
+__device__ __forceinline__ int wg_chunk() {
+  const int id = blockIdx.x, nwg = gridDim.x, c = nwg / 8, rr = nwg % 8, xcd = id % 8;
+  return (xcd < rr ? xcd * (c + 1) : rr * (c + 1) + (xcd - rr) * c) + id / 8;
+}
+
 struct WgStage {
   u32x4 a[4], b[2];          // 8 gradients x 4 token rows, 16 codes x 2 token rows
   unsigned e[2];
@@ -106,11 +112,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(const bf16_t* __restric
   __shared__ __attribute__((aligned(16))) unsigned char smem[4 * WG_BR * WG_PITCH];          // two buffers of { dY, expanded codes }
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wn = wid >> 1, wk = wid & 1, half = lane >> 5, l31 = lane & 31;
   const int nbn = (N + 127) / 128, nbk = (K + 127) / 128, tiles = nbn * nbk;
-  int bid = blockIdx.x;
-  {          // XCD-contiguous chunks: the workgroups of an XCD belong to the same token range, whose panels its L2 then holds once
-    const int nwg = gridDim.x, c = nwg / 8, rr = nwg % 8, xcd = bid % 8, idx = bid / 8;
-    bid = (xcd < rr ? xcd * (c + 1) : rr * (c + 1) + (xcd - rr) * c) + idx;
-  }
+  const int bid = wg_chunk();
   const int split = bid / tiles, tile = bid - split * tiles;
   const int ntile = nbn > nbk ? tile / nbk : tile % nbn, ktile = nbn > nbk ? tile % nbk : tile / nbn;      // the narrower operand is spanned first
   const int n0 = ntile * 128, k0 = ktile * 128, mbeg = split * rows, mend = min(M, mbeg + rows);
@@ -271,15 +273,11 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];          // the ring, then the two expanded images
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wid >> 1, wk = wid & 1, half = lane >> 5, l31 = lane & 31;
   const int nbn = (N + WB_T - 1) / WB_T, nbk = (K + WB_T - 1) / WB_T, tiles = nbn * nbk;
-  int bid = blockIdx.x;
-  {          // XCD-contiguous chunks: the workgroups of an XCD belong to the same token range, whose panels its L2 then holds once
-    const int nwg = gridDim.x, c = nwg / 8, rr = nwg % 8, xcd = bid % 8, idx = bid / 8;
-    bid = (xcd < rr ? xcd * (c + 1) : rr * (c + 1) + (xcd - rr) * c) + idx;
-  }
+  const int bid = wg_chunk();
   const int split = bid / tiles, tile = bid - split * tiles;
   const int ntile = nbn > nbk ? tile / nbk : tile % nbn, ktile = nbn > nbk ? tile % nbk : tile / nbn;
   const int n0 = ntile * WB_T, k0 = ktile * WB_T, mbeg = split * rows, mend = min(M, mbeg + rows);
-  const int nt = (mend - mbeg + WB_BR - 1) / WB_BR;          // (the launcher leaves no split empty)
+  const int nt = (mend - mbeg + WB_BR - 1) / WB_BR;          // at least WB_RING (wgrad_plan)
   // DMA sources of a lane, relative to the first token of a stage; columns past the end repeat the last piece (their results are not stored), tokens past the
   // end the last one (their codes expand to zeros, their gradients are cleared)
   const int arow = threadIdx.x >> 5;          // rows arow and arow + 16 of the gradients
@@ -346,14 +344,12 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
     for (int i = 0; i < 2; ++i)
       if (arow + 16 * i >= valid) *reinterpret_cast<u32x4*>(stage + i * 8192 + threadIdx.x * 16) = (u32x4){0u, 0u, 0u, 0u};
   };
-  for (int t = 0; t < WB_RING && t < nt; ++t) dma(smem + t * WB_STAGE);
-  if (nt >= WB_RING) wait_vmcnt<(WB_RING - 2) * WB_LPT>();          // stages 0 and 1 have landed
-  else wait_vmcnt<0>();
-  if (valid < WB_BR && nt <= 2) clear_tail(smem + (nt - 1) * WB_STAGE);
+  for (int t = 0; t < WB_RING; ++t) dma(smem + t * WB_STAGE);
+  wait_vmcnt<(WB_RING - 2) * WB_LPT>();          // stages 0 and 1 have landed
   raw_read(smem);
   int qm = mend - mbeg - qrow;          // > 0: this lane's token of the tile it expands exists
   wb_expand(raw, e4, qm > 0, bimg);
-  raw_read(smem + (nt > 1 ? WB_STAGE : 0));
+  raw_read(smem + WB_STAGE);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
@@ -435,9 +431,10 @@ __global__ __launch_bounds__(512) void act8_wgrad_big_kernel(const bf16_t* __res
 }
 
 // The plan of a problem: which kernel, and into how many token ranges the reduction is cut.
-//   small: 128 x 128 tiles, two workgroups a CU, no range below 256 tokens (below that the second launch costs more)
-//   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, tiles for at least 24 CUs, and tokens enough that
-//          every range has 768.  Its partial sums are 256 KB a workgroup whatever the problem, twice what the small tiles write: with fewer tiles (more ranges) that
+//   small: 128 x 128 tiles, two workgroups a CU, ranges of 256 tokens or more on average (with less the second launch costs more), the last one shorter
+//   big:   256 x 256 tiles, one workgroup a CU; needs whole 16-byte pieces of the gradients, whole words of exponents, tiles for at least 24 CUs, and tokens for
+//          ranges of 768 or more on average.  At most ten ranges of 64-token tiles, 12 or more a range before rounding up, leave the last one 4 tiles or more: 193
+//          tokens, which fill the ring.  Its partial sums are 256 KB a workgroup whatever the problem, twice what the small tiles write: with fewer tiles (more ranges) that
 //          outweighs the faster loop.  Both kernels with the reduction, us, big / small, N x K over M tokens: 3072 x 768 over 12288 85 / 109, over 4096 47 / 44, over
 //          2048 39 / 31; 2304 x 768 over 12288 70 / 79; 768 x 768 over 12288 58 / 38; 512 x 512 over 12288 60 / 31.
 // Ranges of 128 tokens in place of 256 (small): 2304 x 768 over 400 20 us (12), 768 x 768 over 1024 20 (15), 260 x 384 over 700 12 (14).
@@ -493,6 +490,7 @@ extern "C" int climb_act8_weight_grad(const void* dY, long lddy, const void* q, 
   int bplanes = p.splits;
   if (p.big) {
     const int nbk = (K + WB_T - 1) / WB_T, lds = WB_LDS;
+    if ((long)M - (long)(p.splits - 1) * p.rows <= (WB_RING - 1) * WB_BR) return CLIMB_EUNSUPPORTED;          // (the kernel fetches a whole ring ahead)
     bplanes *= nbk;
     hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(act8_wgrad_big_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return (int)err;

@@ -124,6 +124,28 @@ def test_the_largest_16_bit_activations_stay_finite(dev, M, K, N):
         assert torch.isinf(rows8.checkpoint_save(y).load(dt)).all()
 
 
+# ------------------------------------------------------------------------------------------------ weight gradient at the borders of its plan
+# 256-tile kernel from 12 tiles of 64 tokens a range on (25 tiles: ten ranges, 27: nine, 36: seven); one token more than whole ranges leaves a last one of 193
+@pytest.mark.parametrize("M,K,N", [(7616, 1280, 1280), (7617, 1280, 1280), (7680, 1280, 1280), (7681, 1280, 1280), (6848, 768, 2304), (6912, 768, 2304), (6913, 768, 2304), (5377, 1281, 1288)])
+def test_weight_gradient_ranges(dev, M, K, N):
+    from climb_amd import rows8
+    x, d = _make(M, K, _h16(), M + K)
+    dy, dd = _make(M, N, _h16(), M + N + 1)
+    v = ref_checkpoint(x, _h16() is torch.float16)[2].cuda()
+    dw, db = rows8.weight_grad(dd, rows8.checkpoint_save(d))
+    g = dd.double().t().contiguous()
+    ref, mag = g @ v, g.abs() @ v.abs()
+    assert ((dw.double() - ref).abs() <= 2 * (M + 16) * U * mag + 1e-30).all()          # exact products, at most M + 16 additions (twice: MFMA sums may truncate)
+    assert ((db.double() - g.sum(1)).abs() <= (M + 16) * U * g.abs().sum(1) + 1e-30).all()
+    # the sum over whole ranges alone cannot hide a token: one gradient row at a time
+    for t in (0, M - 1, M // 2):
+        one = torch.zeros_like(dd)
+        one[t] = dd[t]
+        w1, b1 = rows8.weight_grad(one, rows8.checkpoint_save(d))
+        want = one[t].double()[:, None] * v[t][None]
+        assert ((w1.double() - want).abs() <= U * want.abs()).all() and torch.equal(b1, dd[t].float())
+
+
 @pytest.mark.skipif(os.environ.get("CLIMB_AMD_H16") == "fp16", reason="this is the child run")
 def test_the_half_build(dev):
     """this file on the library build whose 16-bit type is IEEE half (a process holds one of them)"""
