@@ -308,8 +308,7 @@ __global__ __launch_bounds__(256) void linear_i8_few_kernel(const T* __restrict_
     mx = lanes_umax<64>(mx);
     const float s = row_scale(mx), rs = 1.f / s;
     if (lane == 0) sc[r] = s;
-#pragma unroll 3
-    for (int c = lane * 4; c < Kp; c += 256) {
+    for (int c = lane * 4; c < Kp; c += 256) {          // (rowq4 asks the whole wave, so hipcc does not unroll this one; its loads hit L1)
       row_ld<MODE, 4>(xr, c, K, v);
       *reinterpret_cast<unsigned*>(smem + r * pitch + c) = rowq4(v, s, rs, mx >= 0x7f800000u);
     }
