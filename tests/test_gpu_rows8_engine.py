@@ -355,3 +355,196 @@ def test_int8_evaluation_captured(eager_first):
             opt.zero_grad()
             model.eval()
     assert _rel(fresh(images, texts), first) > 1e-3
+
+
+def _ewc(model, P):
+    import types
+    from climb_amd.cl_algorithms import EWC
+    from tests.test_gpu_parity import _ewc_state
+    ewc = EWC(types.SimpleNamespace(ewc_fisher_sample_percentage=0.01, ewc_loss_weight=100.0))
+    ewc.set_task_state("nlvr2", model, *_ewc_state(P, 5))
+    return ewc
+
+
+@pytest.mark.parametrize("config", ["plain", "frozen9", "ewc", "accumulate"])
+def test_training_steps_with_checkpoints_and_the_optimizer(config):
+    """two steps with the optimizer named (its promise to run next holds weight-gradient launches back in the plain mode; with checkpoints there are none to hold):
+    after the first the moments are the gradients, so they agree as gradients do (8 %, as above; the EWC term is fp32 in both); all 16-bit shadows are the images
+    of the fp32 parameters; the second step's loss, through those shadows, agrees to 2 % -- a step of AdamW moves a weight by lr whatever its gradient's size, and
+    where 3 % of noise turns a gradient's sign the two models move apart by 2 lr of it"""
+    import random
+    res = {}
+    for name in ("plain", "act8"):
+        torch.manual_seed(0)
+        random.seed(0)
+        model, P = make_model(["vqa", "nlvr2"], 42, precision=H16)
+        eng = model._host.engine()
+        eng.act8 = name == "act8"
+        model.train()
+        if config == "frozen9":
+            model.get_encoder().freeze_bottom_k_layers(9)
+        ewc = _ewc(model, P) if config == "ewc" else None
+        opt = model.create_optimizer({"lr": 2e-5, "weight_decay": 1e-2, "adam_epsilon": 1e-8})
+        opt.zero_grad()
+        names, orig = [], eng._timed_call
+
+        def spy(kernel, flops, call, *a, _o=orig, _l=names):
+            _l.append(call)
+            return _o(kernel, flops, call, *a)
+        eng._timed_call = spy
+        losses, extra, m1 = [], [], None
+        for step in range(2):
+            images, texts, target = _batch(4, 30 + step)
+            if config == "accumulate" and step == 0:
+                model.fused_forward_backward("vqa", images, texts, target, ewc, optimizer=opt)
+            loss, _, _, el = model.fused_forward_backward("vqa", images, texts, target, ewc, optimizer=opt)
+            opt.step()
+            opt.zero_grad()
+            assert not bool(eng.grad.any())
+            losses.append(float(loss))
+            extra.append(float(el) if el is not None else 0.0)
+            if m1 is None:
+                m1 = {n: opt._m[eng.layout.offset[n]:eng.layout.offset[n] + eng.layout.numel(n)].cpu() for n in eng.layout.shapes}
+        eng.refresh_shadow()
+        torch.cuda.synchronize()
+        t16 = eng.t16
+        assert torch.equal(eng._shadow, eng.flat.to(t16))
+        for n, N, K in eng._linear_weight_names():
+            o, ot = eng.layout.offset[n], eng._t_off[n]
+            assert torch.equal(eng._shadow_t[ot:ot + N * K].view(K, N), eng._shadow[o:o + N * K].view(N, K).t()), n
+        assert bool(torch.isfinite(eng.flat).all()) and bool((opt._v >= 0).all())
+        grouped = [n for n in names if "grouped" in n]
+        assert not grouped if name == "act8" else grouped, grouped
+        assert ("climb_act8_weight_grad" in names) == (name == "act8")
+        res[name] = (losses, extra, m1)
+        del model, opt, eng
+    (l0, e0, m0), (l1, e1, m1) = res["plain"], res["act8"]
+    for a, b in zip(l0, l1):
+        assert abs(a - b) <= 2e-2 * abs(a), (l0, l1)
+    for a, b in zip(e0, e1):
+        assert abs(a - b) <= 1e-3 * max(1.0, abs(a)), (e0, e1)
+    moved = [n for n in m0 if bool(m0[n].any())]
+    assert moved == [n for n in m1 if bool(m1[n].any())] and any("layer.11" in n for n in moved)
+    assert any("layer.8." in n for n in moved) == (config != "frozen9")
+    for n in moved:
+        assert n.endswith("key.bias") or _rel(m1[n], m0[n]) < 0.08, (n, _rel(m1[n], m0[n]))
+
+
+def _two_modes(make, run):
+    """gradients of one step of the same model without and with checkpoints"""
+    out = []
+    for on in (False, True):
+        model = make()
+        model._host.engine().act8 = on
+        out.append(run(model) + (grads_of(model),))
+        del model
+    return out
+
+
+@pytest.mark.parametrize("task", ["nlvr2", "vcr"])
+def test_checkpointed_steps_of_tasks_with_several_images_or_choices(task):
+    """two images an example (two sequences, one joint head) and four choices (four sequences); 8 % as above"""
+    b, n = 3, dict(nlvr2=2, vcr=4)[task]
+    e = vo.synthetic_encodings(n * b, seed=41, ragged_text=True)
+    if task == "nlvr2":
+        images, texts = e["pixel_values"], {k: e[k][:b] for k in ("input_ids", "token_type_ids", "attention_mask")}
+    else:
+        images, texts = e["pixel_values"][:b], {k: e[k] for k in ("input_ids", "token_type_ids", "attention_mask")}
+    labels = torch.tensor([1, 0, 1])
+
+    def run(model):
+        model.eval()          # (no dropout mask in the choices' head)
+        loss, (pooled, logits), _, _ = model.fused_forward_backward(task, images, texts, labels)
+        return float(loss), logits.cpu()
+    (l0, o0, G0), (l1, o1, G1) = _two_modes(lambda: make_model([task], 42, precision=H16)[0], run)
+    assert abs(l1 - l0) < 2e-2 * abs(l0) and _rel(o1, o0) < 0.05 and set(G0) == set(G1)
+    for k in G0:
+        if k == "task_layer.vcr.1.bias":          # one number added to all choices of a softmax: its gradient is the sum of (p - y) over them, 1 - 1 = 0 up to rounding
+            assert float(G0[k].abs().max()) < 1e-6 and float(G1[k].abs().max()) < 1e-6
+            continue
+        assert k.endswith("key.bias") or _rel(G1[k], G0[k]) < 0.08, (k, _rel(G1[k], G0[k]))
+
+
+def test_checkpointed_step_of_vilt_on_bert_features():
+    """the embeddings come from a frozen text encoder: their gradient ends at LayerNorm's input; 8 % as above"""
+    from oracle import bert_oracle as bo
+    from climb_amd.modeling import create_continual_learner_map
+    from climb_amd.configs.task_configs import task_configs
+    from climb_amd.configs.model_configs import model_configs
+    P, PB = vo.init_params(["vqa"], 42), bo.init_bert_params(7)
+    sd = {k.replace("vilt_encoder.", "viltbert_encoder."): v for k, v in P.items()}
+    sd.update({"viltbert_encoder.bert." + k: v for k, v in PB.items()})
+    images, texts, target = _batch(4, 43)
+
+    def make():
+        model = create_continual_learner_map["viltbert"](model_name_or_path="random-init:0", ordered_cl_tasks=["vqa"], model_config=model_configs["viltbert"],
+                                                         task_configs=task_configs, device=torch.device("cuda:0"), precision=H16)
+        model.load_state_dict(sd, strict=True)
+        return model.to(torch.device("cuda:0"))
+
+    def run(model):
+        model.eval()          # (no dropout masks in the text encoder)
+        loss, (pooled, logits), _, _ = model.fused_forward_backward("vqa", images, texts, target)
+        return float(loss), logits.cpu()
+    (l0, o0, G0), (l1, o1, G1) = _two_modes(make, run)
+    assert abs(l1 - l0) < 2e-3 * abs(l0) and _rel(o1, o0) < 0.05 and set(G0) == set(G1) and not any("word_embeddings" in k or ".bert." in k for k in G1)
+    for k in G0:
+        assert k.endswith("key.bias") or _rel(G1[k], G0[k]) < 0.08, (k, _rel(G1[k], G0[k]))
+
+
+def test_ranges_reported_by_a_checkpointed_backward_are_final():
+    """what a data-parallel reducer hooks: every range of the gradient buffer is reported once, and holds by then what it holds at the end; the groups are those of
+    the plain mode (ranks may run different paths, but have to issue the same collectives)"""
+    images, texts, target = _batch(4, 47)
+    seen = {}
+    for name in ("plain", "act8"):
+        model, eng = _model(act8=name == "act8")
+        model.train()
+        model.fused_forward_backward("vqa", images, texts, target)          # (workspaces)
+        model.zero_grad(set_to_none=True)
+        reports = []
+        eng.grad_ready_hook = lambda lo, hi: reports.append((lo, hi, eng.grad[lo:hi].clone()))
+        model.fused_forward_backward("vqa", images, texts, target)
+        eng.grad_ready_hook = None
+        torch.cuda.synchronize()
+        for lo, hi, g in reports:
+            assert torch.equal(g, eng.grad[lo:hi]), (name, lo, hi)
+        spans = sorted((lo, hi) for lo, hi, _ in reports)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        seen[name] = [(lo, hi) for lo, hi, _ in reports]
+        assert bool(eng.grad.any())
+    assert seen["plain"] == seen["act8"] and len(seen["act8"]) >= 4
+
+
+def test_int8_evaluation_under_an_active_adapter():
+    """the base's products in int8, the adapter's bottleneck in 16 bits; 10 % allowed as without one"""
+    import types
+    from climb_amd.cl_algorithms import AdapterHandler
+    images, texts, _ = _batch(5, 51)
+    out = []
+    for on in (False, True):
+        model, _ = make_model(["vqa", "nlvr2"], 42, precision=H16)
+        handler = AdapterHandler("vanilla", types.SimpleNamespace(adapter_config="houlsby", adapter_reduction_factor=16, ordered_cl_tasks=["vqa", "nlvr2"]))
+        handler.add_adapters_to_model(model)
+        g = torch.Generator().manual_seed(7)
+        with torch.no_grad():
+            for n, p in model.named_parameters():
+                if ".adapters." in n:
+                    p.copy_((torch.randn(p.shape, generator=g) * (0.05 if n.endswith("weight") else 0.02)).to(p.device))
+        handler.activate_adapter_for_eval("vqa", model)
+        eng = model._host.engine()
+        eng.eval_i8 = on
+        names, orig = [], eng._timed_call
+
+        def spy(kernel, flops, call, *a, _o=orig, _l=names):
+            _l.append(call)
+            return _o(kernel, flops, call, *a)
+        eng._timed_call = spy
+        p, o = _evaluate(model, images, texts)
+        out.append((p, o))
+        assert names.count("climb_linear_i8") == (48 if on else 0)
+        handler.activate_adapter_for_eval("nlvr2", model)
+        q, _ = _evaluate(model, images, texts)
+        assert _rel(q, p) > 0.05          # another adapter, another function
+    print("int8 evaluation under an adapter: pooled %.4f logits %.4f" % (_rel(out[1][0], out[0][0]), _rel(out[1][1], out[0][1])))
+    assert 0 < _rel(out[1][0], out[0][0]) < 0.1 and _rel(out[1][1], out[0][1]) < 0.1
