@@ -23,7 +23,7 @@ def _linear64(x, w, bias=None):
 
 
 # one launch for few tokens, 64 x 64 tiles, 128 x 128, 192 x 192; whole tiles and ragged ones
-SHAPES = [(3, 3000, 48), (40, 3000, 48), (64, 4096, 128), (2560, 3000, 1280), (3072, 3000, 2304), (2500, 3000, 1201)]
+SHAPES = [(3, 3000, 48), (40, 3000, 48), (64, 4096, 128), (2560, 3000, 1280), (3264, 3000, 2304), (2500, 3000, 1201)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
@@ -144,6 +144,52 @@ def test_weight_gradient_ranges(dev, M, K, N):
         w1, b1 = rows8.weight_grad(one, rows8.checkpoint_save(d))
         want = one[t].double()[:, None] * v[t][None]
         assert ((w1.double() - want).abs() <= U * want.abs()).all() and torch.equal(b1, dd[t].float())
+
+
+# ------------------------------------------------------------------------------------------------ LayerNorm backward as the engine calls it
+def _layernorm_bwd(M, C, dt, seed, colsum, beta, gamma_off=0):
+    """climb_act8_layernorm_bwd in place (dx over dres_in) with a 16-bit copy of dx and, if asked for, its column sums"""
+    from climb_amd import _lib, rows8
+    g = torch.Generator().manual_seed(seed)
+    x, dy, res = torch.randn(M, C, generator=g).cuda(), torch.randn(M, C, generator=g).to(dt).cuda(), torch.randn(M, C, generator=g).cuda()
+    gamma = torch.empty(C + gamma_off, device="cuda")[gamma_off:]          # (an offset of one float: the unaligned path)
+    gamma.copy_(1 + 0.1 * torch.randn(C, generator=g))
+    _, ck = rows8.layernorm_fwd(x, gamma, gamma, 1e-5)
+    v, mu, rs = ck.load(torch.float32).double(), ck.mean.double()[:, None], ck.rstd.double()[:, None]
+    sums = [torch.full((C,), float(i + 2), device="cuda") for i in range(3)]
+    dx, cast = res.clone(), torch.empty(M, C, dtype=dt, device="cuda")
+    n = _lib.query_arg("climb_act8_layernorm_bwd_workspace", M, C, 1 if colsum else 0)
+    part = torch.full((max(n // 4, 1),), float("nan"), device="cuda")
+    code = 0 if dt is torch.float32 else 1
+    _lib.call("climb_act8_layernorm_bwd", dy, C, code, *ck._args(), ck.mean, ck.rstd, gamma, dx, C, dx, C, cast, C, part if n else None, sums[0], sums[1], sums[2] if colsum else None,
+              beta, M, C, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    d, ga = dy.double(), gamma.double()
+    xh, G = (v - mu) * rs, d * ga
+    want = res.double() + rs * (G - G.mean(1, keepdim=True) - xh * (G * xh).mean(1, keepdim=True))
+    wide = (v.abs() + mu.abs()) * rs
+    mag = res.double().abs() + rs * (G.abs() + G.abs().mean(1, keepdim=True) + wide * (G.abs() * wide).mean(1, keepdim=True))
+    assert ((dx.double() - want).abs() <= 96 * U * mag + 1e-30).all()          # (as in test_layernorm: ~30 additions on a path, twice, and a handful)
+    assert torch.equal(cast, dx.to(dt))
+    # column sums: at most M + 96 additions on a path (dx itself errs by 96 U of its terms), one fma with the old value
+    for i, (terms, size) in enumerate(((d * xh, d.abs() * wide), (d, d.abs()), (want, mag))[:3 if colsum else 2]):
+        old = beta * (i + 2)
+        assert ((sums[i].double() - old - terms.sum(0)).abs() <= (M + 200) * U * size.sum(0) + 4 * U * abs(old) + 1e-30).all(), i
+    if not colsum:
+        assert (sums[2] == 4).all()          # not asked for, not touched
+    return dx, sums
+
+
+# three rows a wave from 8192 on (24 a workgroup), one below; one launch up to 768 rows without column sums; all widths a wave holds, ragged and whole
+@pytest.mark.parametrize("M,C", [(8191, 70), (8192, 768), (8209, 129), (12301, 768), (8200, 1536), (8215, 3), (8193, 257), (769, 768), (768, 768), (5, 1535), (1, 1)])
+@pytest.mark.parametrize("name", ["f32", "h16"])
+def test_layernorm_backward_in_place_with_a_copy_and_column_sums(dev, M, C, name):
+    dt = torch.float32 if name == "f32" else _h16()
+    for colsum in (True, False):
+        a = _layernorm_bwd(M, C, dt, M + C, colsum, 1.0)
+        b = _layernorm_bwd(M, C, dt, M + C, colsum, 1.0)
+        assert torch.equal(a[0], b[0]) and all(torch.equal(s, t) for s, t in zip(a[1], b[1]))          # no atomics: the same bits
+        _layernorm_bwd(M, C, dt, M + C, colsum, 0.0, gamma_off=1)
 
 
 @pytest.mark.skipif(os.environ.get("CLIMB_AMD_H16") == "fp16", reason="this is the child run")
