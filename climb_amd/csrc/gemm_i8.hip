@@ -255,6 +255,7 @@ static int i8_epi(const signed char* A, long lda, const float* sa, const signed 
 
 extern "C" int climb_gemm_i8_nt(const void* A, long lda, const float* sa, const void* B, long ldb, const float* sb, void* C, long ldc, int c_dtype, int M, int N, int K,
                                 const float* bias, int epi, const float* aux, long ldaux, void* stream) {
+  if (K > (1 << 30)) return CLIMB_EUNSUPPORTED;          // (before it is rounded up)
   const int Kp = (K + I8_BK - 1) / I8_BK * I8_BK;
   if (M < 0 || N <= 0 || K <= 0 || M > (1 << 30) || N > (1 << 30) || lda < Kp || ldb < Kp || lda % 16 || ldb % 16 || ldc < N || ((uintptr_t)A & 15) || ((uintptr_t)B & 15)) return CLIMB_EINVAL;
   if (epi != EPI_NONE && epi != EPI_GELU && epi != EPI_RESID) return CLIMB_EINVAL;

@@ -187,6 +187,12 @@ def _mat(x: torch.Tensor, what: str, cols: Optional[int] = None, rows: Optional[
     return x, M, C, ld
 
 
+def _kept(ck: "Checkpoint") -> "Checkpoint":
+    if not isinstance(ck, Checkpoint):
+        raise TypeError(f"rows8: ck must be a Checkpoint (checkpoint_save, gelu_fwd and layernorm_fwd make one), not {type(ck).__name__}")
+    return ck
+
+
 def _like(x: torch.Tensor, shape) -> torch.Tensor:
     """an empty contiguous tensor of x's dtype (empty_like is the cheapest of torch's allocations)"""
     return torch.empty_like(x) if x.shape == shape and x.is_contiguous() else x.new_empty(shape)
@@ -256,6 +262,8 @@ def linear_i8(x: Union[torch.Tensor, RowCodes], w: RowCodes, bias: Optional[torc
         ycode = _code(dt)
         y, ldy = (m.new_empty((*lead, N)) if not codes and dt is m.dtype else torch.empty((*lead, N), dtype=dt, device=dev)), N
     else:
+        if not isinstance(out, torch.Tensor):
+            raise TypeError("rows8: out must be a tensor")
         y, dt = out, out_dtype or out.dtype
         ycode, ldy = _code(dt), _target(out, "out", (*lead, N), dt, dev)
     b = 0
@@ -292,7 +300,7 @@ def weight_grad(dy: torch.Tensor, ck: Checkpoint, dw: Optional[torch.Tensor] = N
                 bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw [N, K], dbias [N]) of y = x w^T + b from dy (16 bit) and the checkpoint of x.  Given `dw` / `dbias` are added to (fp32, in place); `bias` False:
     no bias gradient."""
-    dev, K = ck.device, ck.cols
+    dev, K = _kept(ck).device, ck.cols
     d, M, N, ld = _mat(dy, "dy", rows=ck.rows, dtype=_h16_type(), dev=dev)
     if dbias is not None and not bias:
         raise ValueError("rows8: dbias given, bias=False")
@@ -332,7 +340,7 @@ def layernorm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps:
 def layernorm_bwd(dy: torch.Tensor, ck: Checkpoint, gamma: torch.Tensor, dres: Optional[torch.Tensor] = None, dgamma: Optional[torch.Tensor] = None,
                   dbeta: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dgamma, dbeta), dx = dres + d(LayerNorm)/dx^T dy in fp32; given `dgamma` / `dbeta` are added to."""
-    if ck._stats is None:
+    if _kept(ck)._stats is None:
         raise ValueError("rows8: this checkpoint holds no row statistics (layernorm_fwd makes one that does)")
     dev, M, C = ck.device, ck.rows, ck.cols
     d, _, _, ld = _mat(dy, "dy", cols=C, rows=M, dev=dev)
@@ -378,7 +386,7 @@ def gelu_fwd(u: torch.Tensor) -> Tuple[torch.Tensor, Checkpoint]:
 
 def gelu_bwd(da: torch.Tensor, ck: Checkpoint, recompute: bool = False):
     """du = da gelu'(u) in da's dtype; recompute: (du, gelu(u)) -- the activation itself, which the next layer's weight gradient reads, is not kept."""
-    dev, M, C = ck.device, ck.rows, ck.cols
+    dev, M, C = _kept(ck).device, ck.rows, ck.cols
     d, _, _, ld = _mat(da, "da", cols=C, rows=M, dev=dev)
     code = _code(d.dtype)
     du = _like(d, (*ck.lead, C))

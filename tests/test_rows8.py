@@ -220,3 +220,17 @@ def test_forward_mode_tangents_are_refused():
         with pytest.raises(ValueError, match="HIP device"):
             rows8.gelu_fwd(x)
     assert rows8._vec(v, "bias", 8, dev) is v
+
+
+def test_arguments_of_another_kind_are_named(mem):
+    x = torch.zeros(4, 8)
+    for call in (lambda: rows8.weight_grad(x, x), lambda: rows8.layernorm_bwd(x, None, x[0]), lambda: rows8.gelu_bwd(x, x), lambda: rows8.gelu_bwd(x, rows8.RowCodes(4, 8, (4,), torch.device("cpu")))):
+        with pytest.raises(TypeError, match="Checkpoint"):
+            call()
+    w = rows8.RowCodes(3, 8, (3,), torch.device("cpu"))
+    with pytest.raises(TypeError, match="out"):
+        rows8.linear_i8(rows8.RowCodes(4, 8, (4,), torch.device("cpu")), w, out=[1.0])
+    p = mem[0]
+    for K in ((1 << 30) + 1, 2 ** 31 - 1):          # rounding them up would leave the type
+        assert _rc("climb_gemm_i8_nt", p, 1 << 32, p, p, 1 << 32, p, p, 32, 0, 4, 32, K, None, 0, None, 0, None) == EUNSUPPORTED
+        assert _rc("climb_linear_i8", p, 1 << 32, 1, p, 1 << 32, p, p, 32, 0, 4, 32, K, None, 0, None, 0, p, 1 << 30, None) == EUNSUPPORTED
