@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_reduce_kernel(const float* __r
 //   - expands the codes of tile t + 1 in its first group (each lane expands the 16 codes it fetched itself, read from LDS a group earlier),
 //   - meets the workgroup in the second group; behind the barrier the ring slot of tile t takes the DMA of tile t + 5, and the first fragments of tile t + 1
 //     are read under the rest of the group.
-// Measured, 3072 x 768 over 12288 tokens: 70 us (0.83 PFLOP/s) + 14 us of reduction, against 109 for the 128-tile kernel with its own and 118 us for the vendor library's
+// Measured, 3072 x 768 over 12288 tokens: 74 us (0.78 PFLOP/s) + 14 us of reduction in a trace, 85 together in a graph, against 109 for the 128-tile kernel with its own and 118 us for the vendor library's
 // 16-bit product of the same shape.  Bounded by the loop: its LDS reads (taken out: - 16 us), its MFMAs (33 us at the clock the chip sustains), the expansion (- 8 us)
 // and the final stores (- 7 us) overlap between the two waves of a SIMD only.
 // As in gemm_i8.hip fragments are read behind the first MFMA of the group before, and no load goes to registers: hipcc would wait for all DMA with it.

@@ -1,7 +1,7 @@
 // int8 product with a scale for each token and each output channel:
 //   C[m,n] = epi( (sum_k qa[m,k] qb[n,k]) sa[m] sb[n] + bias[n] ),   the sum in int32 (exact: K <= 2^17), everything after it in fp32, rounded once.
 // v_mfma_i32_32x32x32_i8 (twice the 16-bit MFMA rate).  Measured: 12288 x 768 -> 3072 with GELU to 16 bits 53 us (1.09 PFLOP/s; the matrix unit is busy 12 us of it at
-// its peak clock, the epilogue's VALU ~20 us, 85 MB leave and enter HBM in ~15), 12288 x 3072 -> 768 + fp32 residual 40 us (1.45 PFLOP/s).  What bounds it is that these
+// its peak clock, the epilogue's VALU ~20 us, 85 MB leave and enter HBM in ~15), 12288 x 3072 -> 768 + fp32 residual 41 us (1.41 PFLOP/s).  What bounds it is that these
 // phases of a tile overlap only across the workgroups of a CU, at the 1.9 GHz the chip sustains under MFMA load.  The weights are the MFMA's A operand and the tokens its B operand, so a lane of the accumulator
 // owns ONE token and groups of 4 consecutive channels.
 #include <type_traits>
@@ -235,7 +235,7 @@ static int i8_pick(const signed char* A, long lda, const float* sa, const signed
 #define I8_GO(NI_, MJ_, WN_, WM_, S_, OCC_) return i8_launch<TO, EPI, NI_, MJ_, WN_, WM_, S_, OCC_>(A, lda, sa, B, ldb, sb, C, ldc, M, N, Kp, bias, aux, ldaux, vec, st)
   // 192 x 192 tiles (twelve waves of 32 x 96, one workgroup a CU) where they fill one round of the chip or K is long: 12288 x 3072 -> 768 + residual 40 us (128 x 128:
   // 49), 12288 x 768 -> 768 + residual 20.5 (23).  128 x 128, two workgroups a CU, one's epilogue beside the other's products: 12288 x 768 -> 3072 45 us (192: 51), with
-  // GELU 54 (63), -> 2304 36 (39).  64 x 64, three a CU, where the larger tiles leave CUs idle: 1024 x 768 -> 768 6.0 us (128: 9.1), 185 x 768 -> 3072 5.9 (9.2).
+  // GELU 54 (63), -> 2304 36 (39).  64 x 64, three a CU, where the larger tiles leave CUs idle: 1024 x 768 -> 768 4.8 - 6.0 us (128: 9.1), 185 x 768 -> 3072 5.0 - 5.9 (9.2).
   const long t192 = tiles(192, 192);
   if (t192 >= 192 && (t192 <= 256 || Kp >= 1536)) I8_GO(3, 1, 2, 6, 3, 1);
   if (tiles(128, 128) >= 192) I8_GO(2, 2, 2, 2, 2, 2);

@@ -1,8 +1,9 @@
 // Row-wise kernels of the 8-bit formats (rows8.h): row codes for the int8 product, checkpoints, and the LayerNorm and GELU that write a checkpoint in
 // their forward and read it in their backward.  All are bound by HBM (a 1 GiB copy runs at 5.1 TB/s, one of 64 MiB, which the Infinity Cache holds, at 8.1); each input
-// is read once and each output written once.  Measured, 16-bit data unless said: row codes 12288 x 3072 19 - 21 us (5.4 - 5.9 TB/s; before the loads of a row went out
-// together 29), 12288 x 768 8.1 us; LayerNorm 12288 x 768 forward 13.5 us (4.9 TB/s), backward 20.8 us (5.0); GELU 12288 x 3072 forward 32 us (5.8), backward with the activation
-// 47 us (5.6); a checkpoint of 12288 x 768 6.3 us.
+// is read once and each output written once.  Measured in a kernel trace, 16-bit data unless said: row codes 12288 x 3072 19 - 21 us (5.4 - 5.9 TB/s; before the loads of a
+// row went out together 29), 12288 x 768 8.0 us (3.5 TB/s: 8-byte loads and 4-byte stores a lane, where a checkpoint has 16 and 8); rows over 3072 columns, read twice:
+// 8192 x 4096 22 us (4.6), 4096 x 8192 in fp32 43 (3.9); LayerNorm 12288 x 768 forward 13.4 us (5.0 TB/s), backward 20.6 us (5.1); GELU 12288 x 3072 forward 32 us (5.8),
+// backward with the activation 47 us (5.6), in fp32 61 (5.6) and 93 (5.3); a checkpoint of 12288 x 768 6.3 us, reading it back 5.6.
 #include "rows8.h"
 
 // the launcher of a row_mode
@@ -276,7 +277,8 @@ extern "C" int climb_act8_layernorm_fwd(const float* x, long ldx, const float* g
 // dx = dres + rstd (g - mean_c(g) - xh mean_c(g xh)),  g = dy gamma,  xh = (codes - mean) rstd;  partial column sums {dgamma, dbeta, colsum(dx)} of the
 // workgroup's rows in part[workgroup][3][C], summed in a fixed order by the column reduction that follows.
 #define A8LN_WAVES 8
-// rows a wave: three where that still leaves two workgroups a CU (12288 rows: 512), else one -- fewer partial rows against more waves on a short launch
+// rows a wave: three from 8192 rows on (342 workgroups on 256 CUs there, 512 at 12288), else one -- fewer partial rows against more waves on a short launch.  768 columns in 16
+// bits with the reduction, calls in a graph: 8191 rows 26.5 us with one, 8192 rows 20.2 with three
 static inline int a8ln_rpw(int M) { return M >= 8192 ? 3 : 1; }
 template <typename T> struct A8LnArgs {
   const T* dy; long lddy;
@@ -457,8 +459,9 @@ __global__ __launch_bounds__(64 * A8LN_WAVES) void act8_ln_bwd_few_kernel(A8LnAr
   for (int i = 1; i < SLOTS; ++i) t += red[k][i][col];
   out[n] = beta != 0.f ? fmaf(beta, out[n], t) : t;
 }
-// Where that one launch is taken.  us on the GPU, one / two launches, 768 columns in 16 bits: 1 row 2.6 / 5.7, 185 3.7 / 7.0, 500 6.0 / 8.4, 768 8.0 / 8.0, 1024 10 / 7.3; 1536 in
-// fp32: 333 4.9 / 10.4, 768 8.1 / 10.8, 1024 15 / 10; 96 columns: 185 3.6 / 5.6, 768 7.8 / 6.3 -- and the second launch costs the host 3 us.
+// Where that one launch is taken.  us a call of twenty in a graph (a trace, which counts each launch from its start to its end, has 1.4 to 2.4 more), one / two launches, 768
+// columns in 16 bits: 1 row 2.6 / 5.7, 185 3.7 / 7.1, 500 6.0 / 8.4, 768 8.1 / 8.1, 1024 10 / 7.4; 1536 in fp32: 333 4.7 / 10.4, 768 8.3 / 10.9, 1024 15 / 10; 96 columns: 185
+// 3.5 / 5.6, 768 7.8 / 6.3 -- and the second launch costs the host 3 us.
 static inline bool a8ln_few(int M, bool colsum) { return !colsum && M <= 768; }
 template <typename T, int MODE>
 static int act8_ln_bwd_launch(const A8LnArgs<T>& p, float* part, float* dgamma, float* dbeta, float beta, bool few, int M, int C, hipStream_t st) {
