@@ -45,12 +45,17 @@ def _stale(target, deps):
 
 
 def _made_by(record) -> str:
-    """the command a product was made with ("" if none is on record): other flags make another object of the same source"""
+    """what a product was made with ("" if none is on record): other flags make another object of the same source.  Without the tree's place: a copied tree is as fresh
+    as the original"""
     try:
         with open(record) as f:
             return f.read()
     except OSError:
         return ""
+
+
+def _text(cmd) -> str:
+    return " ".join(cmd).replace(CSRC + os.sep, "")
 
 
 def _run(cmd, record, what, verbose):
@@ -62,7 +67,7 @@ def _run(cmd, record, what, verbose):
     if r.returncode != 0:
         raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
     with open(record, "w") as f:
-        f.write(" ".join(cmd))
+        f.write(_text(cmd))
 
 
 def build_library(force: bool = False, verbose: bool = True) -> str:
@@ -78,14 +83,14 @@ def _build(LIB: str, objdir: str, extra, force: bool, verbose: bool) -> str:
         src = os.path.join(CSRC, s)
         obj = os.path.join(objdir, stem + ".o")
         cmd = [HIPCC] + FLAGS + extra + fl + ["-c", src, "-o", obj]
-        if force or _stale(obj, [src] + hdrs) or _made_by(obj + ".cmd") != " ".join(cmd):
+        if force or _stale(obj, [src] + hdrs) or _made_by(obj + ".cmd") != _text(cmd):
             jobs.append((cmd, obj + ".cmd", f"hipcc failed on {src}"))
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(lambda job: _run(*job, verbose), jobs))
     objs = [os.path.join(objdir, stem + ".o") for _, stem, _ in units()]
     cmd, record = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs, os.path.join(objdir, "link.cmd")
-    if force or jobs or _stale(LIB, objs) or _made_by(record) != " ".join(cmd):
+    if force or jobs or _stale(LIB, objs) or _made_by(record) != _text(cmd):
         _run(cmd, record, "link failed", verbose)
     return LIB
 

@@ -434,6 +434,29 @@ def test_objects_are_rebuilt_when_their_flags_change(tmp_path, monkeypatch):
     assert len(runs()) == 2 and runs() == []
 
 
+def test_a_copied_tree_is_as_fresh_as_the_original(tmp_path, monkeypatch):
+    """what is built travels with a copy of the tree to another place, and is not compiled again there"""
+    import shutil
+    from climb_amd import build
+    log, cc = tmp_path / "log", tmp_path / "cc"
+    cc.write_text(f'#!/bin/sh\necho "$@" >> {log}\nwhile [ "$1" != "-o" ]; do shift; done\ntouch "$2"\n')
+    cc.chmod(0o755)
+    src = tmp_path / "one" / "csrc"
+    src.mkdir(parents=True)
+    (src / "a.hip").write_text("")
+    monkeypatch.setattr(build, "HIPCC", str(cc))
+
+    def runs(d):
+        log.write_text("")
+        for name, value in (("CSRC", str(d)), ("LIB", str(d / "l.so")), ("LIB_F16", str(d / "l16.so"))):
+            monkeypatch.setattr(build, name, value)
+        build.build_library(verbose=False)
+        return len(log.read_text().splitlines())
+    assert runs(src) == 4 and runs(src) == 0
+    shutil.copytree(src, tmp_path / "two", copy_function=shutil.copy2)
+    assert runs(tmp_path / "two") == 0
+
+
 def test_the_hazard_scan_compiles_what_the_library_is_built_from():
     """the source scan of tools/check_store_hazard.py uses the library's own flags"""
     import importlib.util
