@@ -1,9 +1,9 @@
 // Row-wise kernels of the 8-bit formats (rows8.h): row codes for the int8 product, checkpoints, and the LayerNorm and GELU that write a checkpoint in
 // their forward and read it in their backward.  All are bound by HBM (a 1 GiB copy runs at 5.1 TB/s, one of 64 MiB, which the Infinity Cache holds, at 8.1); each input
 // is read once and each output written once.  Measured in a kernel trace, 16-bit data unless said: row codes 12288 x 3072 19 - 21 us (5.4 - 5.9 TB/s; before the loads of a
-// row went out together 29), 12288 x 768 8.0 us (3.5 TB/s: 8-byte loads and 4-byte stores a lane, where a checkpoint has 16 and 8); rows over 3072 columns, read twice:
-// 8192 x 4096 22 us (4.6), 4096 x 8192 in fp32 43 (3.9); LayerNorm 12288 x 768 forward 13.4 us (5.0 TB/s), backward 20.6 us (5.1); GELU 12288 x 3072 forward 32 us (5.8),
-// backward with the activation 47 us (5.6), in fp32 61 (5.6) and 93 (5.3); a checkpoint of 12288 x 768 6.3 us, reading it back 5.6.
+// row went out together 29), 12288 x 768 8.0 us (3.5 TB/s: 8-byte loads and 4-byte stores a lane, where a checkpoint has 16 and 8); LayerNorm 12288 x 768 forward 13.4 us (5.0 TB/s),
+// backward 20.6 us (5.1); GELU 12288 x 3072 forward 32 us (5.8), backward with the activation 47 us (5.6); a checkpoint of 12288 x 768 6.3 us.  Calls in a graph: rows over 3072 columns,
+// read twice, 8192 x 4096 22 us (4.6), 4096 x 8192 in fp32 43 (3.9); GELU 12288 x 3072 in fp32 61 (5.6) and 93 (5.3); a checkpoint of 12288 x 768 read back 5.6.
 #include "rows8.h"
 
 // the launcher of a row_mode
