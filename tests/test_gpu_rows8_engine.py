@@ -548,3 +548,26 @@ def test_int8_evaluation_under_an_active_adapter():
         assert _rel(q, p) > 0.05          # another adapter, another function
     print("int8 evaluation under an adapter: pooled %.4f logits %.4f" % (_rel(out[1][0], out[0][0]), _rel(out[1][1], out[0][1])))
     assert 0 < _rel(out[1][0], out[0][0]) < 0.1 and _rel(out[1][1], out[0][1]) < 0.1
+
+
+def test_both_uses_in_one_model():
+    """int8 evaluations in the checkpointed training's workspace (activations in buffers that the layers share), between a training forward and its backward and after"""
+    images, texts, target = _batch(4, 61)
+    crit = torch.nn.BCEWithLogitsLoss(reduction="mean")
+    only, _ = _model(eval_i8=True)
+    want, _ = _evaluate(only, images, texts)
+    ck, _ = _model(act8=True)
+    ck.train()
+    _, logits = ck("vqa", images, texts)
+    (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+    G = grads_of(ck)
+    model, eng = _model(act8=True, eval_i8=True)
+    assert _rel(_evaluate(model, images, texts)[0], want) < 1e-5
+    model.train()
+    _, logits = model("vqa", images, texts)
+    assert _rel(_evaluate(model, images, texts)[0], want) < 1e-5
+    model.train()
+    (crit(logits, target.to(logits.device).float()) * target.shape[1]).backward()
+    for n, g in grads_of(model).items():
+        assert _rel(g, G[n]) < 0.02 or n.endswith("key.bias"), n          # (0.02: two runs' last bits, as above)
+    assert _rel(_evaluate(model, images, texts)[0], want) < 1e-5
